@@ -22,7 +22,7 @@
 extern "C" {
 #endif
 
-#define RFX_ABI_VERSION 5
+#define RFX_ABI_VERSION 6
 
 enum {
     RFX_OK = 0,
@@ -425,6 +425,82 @@ int rfx_lowrank_product(void* ctx, int row_begin, int row_end, float* out_host);
 /* Y_dev = S X_dev for the trees stored in low-rank mode (this context's trees only), X and
  * Y device [R][ncols] row-major, ncols <= 128; nout_dev as in rfx_lowrank_build. */
 int rfx_prox_apply(void* ctx, const float* X_dev, int ncols, const int* nout_dev, float* Y_dev);
+
+/* ---- Matrices in microscaled 4 bits ---------------------------------------------------
+ * No counterpart in the reference beyond its "nf4" factor storage
+ * (cuda/rf_proximity_lowrank.cu:199-400): rows of e2m1 codes (0, .5, 1, 1.5, 2, 3, 4, 6 with a
+ * sign) with one scale per block of neighbouring columns, in the two forms that the tensor
+ * cores multiply directly.
+ *   RFX_FP4_MX  blocks of 32, scale a power of two (e8m0): the smallest of which the block's
+ *               largest magnitude is at most 6 times (not below 2^-127).
+ *   RFX_FP4_NV  blocks of 16, scale e4m3, times one scale g of the matrix: g the smallest
+ *               power of two of which the largest magnitude is at most 6 * 448 times (not
+ *               below 2^-126, 1 for zeros), block scale = e4m3(largest magnitude / (6 g)).
+ * Codes are value / scale rounded to the nearest, ties to the even code, at most 6.  A block
+ * with an infinity or NaN gets a NaN scale (its values read back as NaN); g ignores it.
+ *
+ * These functions need no context: device pointers, the caller's current device and stream
+ * (NULL = the legacy default stream).  They enqueue and return, allocate nothing, and can be
+ * captured into a graph once each has run before on the device.  The caller owns every buffer;
+ * calls that share none may run at the same time. */
+enum { RFX_FP4_MX = 0, RFX_FP4_NV = 1 };
+enum { RFX_F32 = 0, RFX_BF16 = 1, RFX_F16 = 2 };
+
+/* A matrix's device buffers, sized by rfx_fp4_sizes, 16-byte aligned.  The layout is the
+ * library's (tiles of 128 rows); a view of rows [r, r + n) with r a multiple of 128 is the same
+ * struct with codes_dev + r * pitch, scales_dev + r / 128 * tile_bytes, bounds_dev + r / 128. */
+typedef struct {
+    int format, rows, cols;
+    uint8_t* codes_dev;
+    uint8_t* scales_dev;
+    float* scale_dev;  /* [2]: the matrix scale, scratch */
+    float* bounds_dev; /* per 128 rows, when cols <= 256 */
+} rfx_fp4_matrix;
+typedef struct {
+    long long codes, scales, scale, bounds; /* bytes */
+    long long pitch, tile_bytes;            /* bytes of a row of codes, of 128 rows' scales */
+} rfx_fp4_layout;
+int rfx_fp4_sizes(int format, int rows, int cols, rfx_fp4_layout* out);
+
+/* out <- x: x_dev [rows][row_stride >= cols] of RFX_F32 / RFX_BF16 / RFX_F16 (row_stride in
+ * elements; shape and format as in `out`). */
+int rfx_fp4_quantize(const void* x_dev, int dtype, long long row_stride, const rfx_fp4_matrix* out,
+                     void* stream);
+/* Values of rows [row_begin, row_end), rounded once to `dtype` (RFX_F32 and RFX_BF16 hold what
+ * rfx_fp4_quantize made exactly): out_dev [rows][ld >= cols]. */
+int rfx_fp4_dequantize(const rfx_fp4_matrix* m, int row_begin, int row_end, void* out_dev, int dtype,
+                       long long ld, void* stream);
+/* out <- caller-supplied codes [rows][(cols + 1) / 2] (two a byte, even column low), scale bytes
+ * [rows][ceil(cols / block)] (e8m0, or e4m3 whose top bit is ignored) and matrix scale (device,
+ * one positive float; NULL = 1), all row-major on the device; and the inverse. */
+int rfx_fp4_pack(const uint8_t* codes_dev, const uint8_t* scales_dev, const float* scale_dev,
+                 const rfx_fp4_matrix* out, void* stream);
+int rfx_fp4_unpack(const rfx_fp4_matrix* m, uint8_t* codes_dev, uint8_t* scales_dev, void* stream);
+/* out_dev[i][j] = a_i . b_j, [a.rows][ld >= b.rows] of `dtype`: block-scaled tensor-core
+ * products, fp32 accumulation.  a and b share format and cols. */
+int rfx_fp4_product(const rfx_fp4_matrix* a, const rfx_fp4_matrix* b, void* out_dev, int dtype,
+                    long long ld, void* stream);
+/* The k <= 64 rows of b with the largest a_i . b_j for every row of a, by exact value
+ * descending, then index ascending: idx_dev / val_dev [a.rows][k].  The value is the sum over
+ * the blocks, in order, in 64 bits, rounded once to float at the end.  self >= 0: row i of a
+ * is row self + i of b and not its own neighbour (-1: no such rows).  Rows whose value is NaN
+ * are nobody's neighbours; slots without one hold -1 / -inf.  cols <= 256.  ws_dev: ws_bytes
+ * >= rfx_fp4_topk_workspace bytes of scratch for this call alone, 16-byte aligned. */
+int rfx_fp4_topk_workspace(const rfx_fp4_matrix* a, const rfx_fp4_matrix* b, int k, long long* bytes);
+int rfx_fp4_topk(const rfx_fp4_matrix* a, const rfx_fp4_matrix* b, int k, long long self, int* idx_dev,
+                 float* val_dev, void* ws_dev, long long ws_bytes, void* stream);
+/* Waits for the current device; RFX_ERR_DEVICE when a product or top-k kernel has reported a
+ * pipeline wait that timed out since the last call (its outputs are then incomplete). */
+int rfx_fp4_status(void);
+
+/* ---- Low-rank proximity in 4 bits (quant_mode "mxfp4" / "nvfp4") ------------------------
+ * rfx_lowrank_pack4 quantises the float factors of the last rfx_lowrank_build to `format`
+ * (beside the int8 factors); the others are rfx_lowrank_factors / _topk / _product on them:
+ * A_host [R][rank]; idx_host / val_host [rows][k]; out_host [rows][R]. */
+int rfx_lowrank_pack4(void* ctx, int format);
+int rfx_lowrank4_factors(void* ctx, float* A_host, int* rank_out, int* rows_out);
+int rfx_lowrank4_topk(void* ctx, int k, int row_begin, int row_end, int* idx_host, float* val_host);
+int rfx_lowrank4_product(void* ctx, int row_begin, int row_end, float* out_host);
 
 /* Wait for the context's stream. */
 int rfx_sync(void* ctx);

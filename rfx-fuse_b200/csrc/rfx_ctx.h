@@ -227,10 +227,13 @@ struct Ctx {
     int lr_k = 0, lr_Rpad = 0;  // factor rank and rows padded to the product tile
     int lr_R = 0;               // factor rows
     bool lr_ready = false;
+    bool lr_float = false;      // lr_X holds the float factors of the last build
+    bool lr4_ready = false;     // lr4_m holds them in 4 bits (rfx_fp4_host.cu)
+    rfx_fp4_matrix lr4_m{};
     std::vector<int> lr_pos;    // stored position of every original row (product order)
     DBuf lr_code, lr_order, lr_goff, lr_ngroups, lr_tmp;
     DBuf lr_X, lr_Z, lr_CZ, lr_Y, lr_ls, lr_part, lr_small, lr_A, lr_q, lr_qb, lr_s, lr_qbp, lr_sp, lr_perm, lr_blocks, lr_np, lr_norm, lr_ids, lr_keys, lr_order_s, lr_cub,
-        lr_err, lr_out_i, lr_out_v;
+        lr_err, lr_out_i, lr_out_v, lr4_buf;
 
     // stored forest for prediction (rfx_predict.cu)
     int f_T = 0, f_cap = 0, f_M = 0, f_p = 0, f_nclass = 0, f_task = 0;
@@ -269,7 +272,7 @@ struct Ctx {
                        &p_xc, &p_vote, &p_val, &p_cls, &p_proba, &p_pred, &i_x, &i_miss, &i_cat,
                        &i_S, &i_scratch, &i_cells, &i_out, &i_prof, &l_leaf, &l_oob, &l_rows, &l_gs, &l_ge,
                        &l_keys, &l_cub, &l_cnt, &l_cidx, &l_cval, &l_nnz, &l_q, &l_out, &l_f,
-                       &lr_err, &lr_out_i, &lr_out_v, &ts_status, &ts_bestvar, &ts_xbest, &ts_treemap,
+                       &lr_err, &lr_out_i, &lr_out_v, &lr4_buf, &ts_status, &ts_bestvar, &ts_xbest, &ts_treemap,
                        &ts_nodeclass, &ts_nnode, &ts_nodepred, &ts_tnodewt};
         cudaSetDevice(device);
         const bool drained = !st || cudaStreamSynchronize(st) == cudaSuccess;

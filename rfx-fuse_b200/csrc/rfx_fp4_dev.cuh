@@ -1,0 +1,91 @@
+// Device arithmetic of the 4-bit formats.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "rfx_fp4.h"
+
+namespace rfx {
+
+namespace {
+
+// Two floats -> two e4m3 bytes (nearest, ties to even, saturating at 448), lo in the low byte.
+__device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
+    uint16_t d;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+
+// e4m3 byte -> float, exactly (0x7F: NaN).
+__device__ __forceinline__ float e4m3_value(uint32_t byte) {
+    uint32_t h2;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"((uint16_t)byte));
+    return __half2float(__ushort_as_half((unsigned short)(h2 & 0xFFFF)));
+}
+
+// e8m0 byte -> 2^(byte - 127) (0: the denormal 2^-127; 255: NaN).
+__device__ __forceinline__ float e8m0_value(uint32_t byte) {
+    if (byte == 255u) return __int_as_float(0x7fc00000);
+    return __int_as_float(byte ? (int)(byte << 23) : 0x00400000);
+}
+
+__device__ __forceinline__ float f4_scale_value(int nv, uint32_t byte) {
+    return nv ? e4m3_value(byte) : e8m0_value(byte);
+}
+
+// Eight floats -> eight e2m1 codes in a word, v[0] in the lowest nibble (nearest, ties to the
+// even code, saturating at 6).
+__device__ __forceinline__ uint32_t cvt_e2m1x8(const float* v) {
+    uint32_t d;
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+        "mov.b32 %0, {b0, b1, b2, b3};\n\t}\n"
+        : "=r"(d)
+        : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+    return d;
+}
+
+// Twice the magnitudes (0, 1, 2, 3, 4, 6, 8, 12) of the four codes in the low half of w, as bytes.
+__device__ __forceinline__ uint32_t e2m1_mag4(uint32_t w) {
+    return __byte_perm(0x03020100u, 0x0C080604u, w & 0x7777u);
+}
+
+// 0x7F in the bytes whose code (low half of w) has its sign bit set, else 0.
+__device__ __forceinline__ uint32_t e2m1_neg4(uint32_t w) {
+    // a selector of 8 replicates the sign of byte 0 (0xFF), 0 copies it (0x80)
+    return __byte_perm(0x80u, 0u, w & 0x8888u) & 0x7F7F7F7Fu;
+}
+
+// Value of one e2m1 code.
+__device__ __forceinline__ float e2m1_value(uint32_t code) {
+    const float m = 0.5f * (float)(e2m1_mag4(code & 7u) & 0xFFu);
+    return (code & 8u) ? -m : m;
+}
+
+// Four times the dot product of eight codes with eight codes, exactly.
+__device__ __forceinline__ int e2m1_dot8(uint32_t a, uint32_t b, int acc) {
+    const uint32_t s = a ^ b;
+    const uint32_t mb0 = e2m1_mag4(b), mb1 = e2m1_mag4(b >> 16);
+    const uint32_t ma0 = e2m1_mag4(a), ma1 = e2m1_mag4(a >> 16);
+    uint32_t all = __dp4a(ma0, mb0, 0u), neg = __dp4a(ma0, mb0 & e2m1_neg4(s), 0u);
+    all = __dp4a(ma1, mb1, all);
+    neg = __dp4a(ma1, mb1 & e2m1_neg4(s >> 16), neg);
+    return acc + (int)all - 2 * (int)neg;
+}
+
+template <class T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+
+template <class T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+}  // namespace
+
+}  // namespace rfx

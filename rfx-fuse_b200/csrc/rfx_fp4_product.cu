@@ -1,0 +1,268 @@
+// Product of two matrices in microscaled 4 bits, out[i][j] = a_i . b_j, on the block-scaled
+// tcgen05 tensor cores (fp32 accumulation, one rounding to the output type).
+//
+// The 128 rows of the instruction's A are rows of b (columns of the output): an accumulator lane
+// is then an output column, so a warp's store of one register is 32 neighbouring outputs and
+// needs no transpose; the instruction's N holds up to 256 rows of a, and shrinks to the rows
+// there are (16 at least), so that a product of a few rows only reads b.
+//
+// A CTA walks the tiles t = blockIdx.x, + gridDim.x, ...
+//   warps 0-7  read an accumulator (quarter warp & 3) and store it.  With up to 128 rows of a the
+//              accumulators form a ring and the two groups of four warps take alternate tiles;
+//              with more, both take the one accumulator, half the columns each, and release it as
+//              soon as it is in registers, so the next tile's products run under the stores;
+//   warp 8     one thread loads code rows by TMA and scale atoms by bulk copies into a ring of
+//              chunks of 256 columns (64 when the matrix has no more);
+//   warp 9     allocates TMEM; one thread copies the chunk's atoms to TMEM (its columns belong to
+//              the ring stage, so a stage's "empty" barrier also frees them) and multiplies.
+// Every wait is bounded; on expiry the CTA records it in *err, drains its copies, frees TMEM and
+// returns.
+#include <algorithm>
+
+#include "rfx_fp4_mma.cuh"
+
+namespace rfx {
+
+namespace {
+
+constexpr int kPThreads = 320;
+constexpr int kPMaxStage = 16;
+constexpr int kPSmem = 227 * 1024;
+constexpr int kPBars = 1024;  // barriers and flags
+
+template <int kNv, int kCB, class T>
+__global__ void __launch_bounds__(kPThreads, 1)
+k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUtensorMap tmb, F4ProductArgs p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint64_t* bars = (uint64_t*)sm;
+    // full[16], empty[16], acc_full[8], acc_empty[8]
+    uint32_t* tmem_slot = (uint32_t*)(bars + 48);
+    volatile int* abort = (volatile int*)(tmem_slot + 1);
+    const uint32_t bar0 = smem_u32(bars);
+    auto full = [&](int s) { return bar0 + 8u * s; };
+    auto empty = [&](int s) { return bar0 + 8u * (16 + s); };
+    auto accf = [&](int b) { return bar0 + 8u * (32 + b); };
+    auto acce = [&](int b) { return bar0 + 8u * (40 + b); };
+    const uint32_t stage0 = bar0 + kPBars;
+    constexpr int kAtoms = kCB == 32 ? 1 : (kNv ? 4 : 2);  // scale atoms of a whole chunk
+    const int nrt = p.bn > kF4Tile ? 2 : 1;                // scale tiles of a's rows
+    const uint32_t off_b = 128 * kCB;
+    const uint32_t off_sb = off_b + (uint32_t)((p.bn * kCB + 1023) / 1024 * 1024);  // scales of b, then of a
+    const uint32_t off_sa = off_sb + kAtoms * kF4Atom;
+    const int ntiles = p.njt * p.nit;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < p.nstage; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), 1);
+        }
+        for (int b = 0; b < p.nacc; ++b) {
+            mbar_init(accf(b), 1);
+            mbar_init(acce(b), p.nacc > 1 ? 128 : 256);
+        }
+        *abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_u32(tmem_slot)),
+                     "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 8) {
+        if (lane == 0) {
+            int step = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
+                const int jt = t % p.njt, i0 = t / p.njt * p.bn;
+                const int rt0 = i0 / kF4Tile;
+                const int rts = min(nrt, p.a.tiles() - rt0);
+                for (int c = 0; c < p.nchunk; ++c, ++step) {
+                    const int s = step % p.nstage;
+                    if (mbar_wait(empty(s), ((uint32_t)(step / p.nstage) & 1u) ^ 1u, abort) != kWaitOk) {
+                        if (!*abort) atomicExch(p.err, 1);
+                        *abort = 1;
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t st = stage0 + (uint32_t)(s * p.stage_bytes);
+                    const int left = (p.b.Kp - c * 2 * kCB) / 64;
+                    const int steps = min(left, kCB / 32);
+                    const int atoms = kNv ? steps : (steps + 1) / 2;
+                    const uint32_t sfb = (uint32_t)(atoms * kF4Atom);
+                    mbar_expect_tx(full(s), (uint32_t)((128 + p.bn) * kCB) + sfb * (1 + rts));
+                    tma_load(st, &tmb, c * kCB, jt * 128, full(s));
+                    tma_load(st + off_b, &tma, c * kCB, i0, full(s));
+                    bulk_load(st + off_sb, p.b.scales + ((long long)jt * p.b.natoms + c * kAtoms) * kF4Atom, sfb, full(s));
+                    for (int r = 0; r < rts; ++r)
+                        bulk_load(st + off_sa + r * kAtoms * kF4Atom,
+                                  p.a.scales + ((long long)(rt0 + r) * p.a.natoms + c * kAtoms) * kF4Atom, sfb, full(s));
+                }
+            }
+            // drain this thread's copies still in flight
+            for (int i = step > p.nstage ? step - p.nstage : 0; i < step; ++i)
+                mbar_wait(full(i % p.nstage), (uint32_t)(i / p.nstage) & 1u, nullptr);
+        }
+        __syncwarp();
+    } else if (warp == 9) {
+        if (lane == 0) {
+            int step = 0, n = 0;
+            bool ok = true;
+            const uint32_t sfc = (uint32_t)(4 * kAtoms * (1 + nrt));  // TMEM columns of a stage's scales
+            for (int t = blockIdx.x; ok && t < ntiles; t += gridDim.x, ++n) {
+                const int b = n % p.nacc;
+                if (mbar_wait(acce(b), ((uint32_t)(n / p.nacc) & 1u) ^ 1u, abort) != kWaitOk) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t d = tmem + (uint32_t)(b * p.acc_cols);
+                for (int c = 0; c < p.nchunk; ++c, ++step) {
+                    const int s = step % p.nstage;
+                    if (mbar_wait(full(s), (uint32_t)(step / p.nstage) & 1u, abort) != kWaitOk) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t st = stage0 + (uint32_t)(s * p.stage_bytes);
+                    const int left = (p.b.Kp - c * 2 * kCB) / 64;
+                    const int steps = min(left, kCB / 32);
+                    const int atoms = kNv ? steps : (steps + 1) / 2;
+                    const uint32_t tsb = tmem + 256u + (uint32_t)s * sfc, tsa = tsb + 4 * kAtoms;
+                    for (int k = 0; k < atoms; ++k) {
+                        f4_copy_atom(tsb + 4 * k, f4_atom_desc(st + off_sb + k * kF4Atom));
+                        for (int r = 0; r < nrt; ++r)
+                            f4_copy_atom(tsa + 4 * (k * nrt + r), f4_atom_desc(st + off_sa + (r * kAtoms + k) * kF4Atom));
+                    }
+                    const uint64_t db = f4_operand_desc<kCB>(st), da = f4_operand_desc<kCB>(st + off_b);
+                    for (int k = 0; k < steps; ++k) {
+                        const int at = kNv ? k : k >> 1;
+                        f4_mma<kNv>(d, db + 2 * k, da + 2 * k, f4_idesc<kNv>(p.bn, kNv ? 0 : k & 1),
+                                    tsb + 4 * at, tsa + 4 * nrt * at, (c | k) ? 1u : 0u);
+                    }
+                    mma_commit(empty(s));
+                }
+                if (ok) mma_commit(accf(b));
+            }
+            if (!ok) {
+                if (!*abort) atomicExch(p.err, 2);
+                *abort = 1;
+            }
+            // the last products must finish before the accumulators are freed
+            if (step > 0) mbar_wait(empty((step - 1) % p.nstage), (uint32_t)((step - 1) / p.nstage) & 1u, nullptr);
+        }
+        __syncwarp();
+    } else {
+        const int group = warp >> 2;
+        const int jl = 32 * (warp & 3) + lane;
+        const uint32_t lane_addr = (uint32_t)(32 * (warp & 3)) << 16;
+        const float alpha = __ldg(p.a.gs) * __ldg(p.b.gs);
+        T* out = (T*)p.out;
+        int n = 0;
+        for (int t = blockIdx.x; t < ntiles; t += gridDim.x, ++n) {
+            if (p.nacc > 1 && (n & 1) != group) continue;
+            const int b = n % p.nacc;
+            const int w = mbar_wait<false>(accf(b), (uint32_t)(n / p.nacc) & 1u, abort);
+            if (__any_sync(0xFFFFFFFFu, w != kWaitOk)) {
+                if (!*abort) atomicExch(p.err, 3);
+                *abort = 1;
+                break;
+            }
+            tc_fence_after();
+            const int jt = t % p.njt, i0 = t / p.njt * p.bn;
+            const int cb = p.nacc > 1 ? 0 : 128 * group;   // first of this warp's columns (rows of a)
+            const int ce = min(min(p.bn, cb + 128), p.a.rows - i0);
+            uint32_t r[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (cb + 32 * c < ce) tmem_ld32_issue(tmem + lane_addr + (uint32_t)(b * p.acc_cols + cb + 32 * c), r[c]);
+            tmem_wait();
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_pin32(r[c]);
+            tc_fence_before();
+            mbar_arrive(acce(b));
+            const long long j = (long long)jt * 128 + jl;
+            if (j < p.b.rows) {
+                T* o = out + (long long)(i0 + cb) * p.ld + j;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        if (cb + 32 * c + e < ce) {
+                            *o = from_f32<T>(__uint_as_float(r[c][e]) * alpha);
+                            o += p.ld;
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512)
+                     : "memory");
+    }
+}
+
+template <int kNv, int kCB, class T>
+cudaError_t launch(const CUtensorMap& ta, const CUtensorMap& tb, const F4ProductArgs& p, int grid, cudaStream_t st) {
+    const int smem = 1024 + kPBars + p.nstage * p.stage_bytes;
+    auto f = k_f4_product<kNv, kCB, T>;
+    cudaError_t e = cudaFuncSetAttribute((const void*)f, cudaFuncAttributeMaxDynamicSharedMemorySize, kPSmem);
+    if (e != cudaSuccess) return e;
+    f<<<grid, kPThreads, smem, st>>>(ta, tb, p);
+    return cudaGetLastError();
+}
+
+template <int kNv, int kCB>
+cudaError_t launch_t(const CUtensorMap& ta, const CUtensorMap& tb, const F4ProductArgs& p, int grid, cudaStream_t st) {
+    if (p.dtype == RFX_F32) return launch<kNv, kCB, float>(ta, tb, p, grid, st);
+    if (p.dtype == RFX_BF16) return launch<kNv, kCB, __nv_bfloat16>(ta, tb, p, grid, st);
+    return launch<kNv, kCB, __half>(ta, tb, p, grid, st);
+}
+
+}  // namespace
+
+cudaError_t f4_product(const F4& a, const F4& b, void* out, int dtype, long long ld, int* err, int sms,
+                       cudaStream_t st, int* launches) {
+    F4ProductArgs p;
+    p.a = a;
+    p.b = b;
+    p.out = out;
+    p.ld = ld;
+    p.dtype = dtype;
+    p.err = err;
+    p.bn = std::min(256, (a.rows + 15) / 16 * 16);
+    p.nit = (int)(((long long)a.rows + p.bn - 1) / p.bn);
+    p.njt = b.tiles();
+    const int cb = b.Kp == 64 ? 32 : 128;
+    p.nchunk = (b.Kp + 2 * cb - 1) / (2 * cb);
+    const int atoms = cb == 32 ? 1 : (b.nv ? 4 : 2);
+    const int nrt = p.bn > kF4Tile ? 2 : 1;
+    p.stage_bytes = ((128 * cb + (p.bn * cb + 1023) / 1024 * 1024 + atoms * kF4Atom * (1 + nrt)) + 1023) / 1024 * 1024;
+    const int sfc = 4 * atoms * (1 + nrt);
+    p.nstage = std::min(std::min(kPMaxStage, 256 / sfc), (kPSmem - 1024 - kPBars) / p.stage_bytes);
+    p.acc_cols = 32;
+    while (p.acc_cols < p.bn) p.acc_cols *= 2;
+    p.nacc = 256 / p.acc_cols;
+    const long long ntiles = (long long)p.nit * p.njt;
+    const int grid = (int)std::min<long long>(ntiles, sms);
+    CUtensorMap ta, tb;
+    if (!f4_map(&ta, a, p.bn, cb) || !f4_map(&tb, b, 128, cb)) return cudaErrorInvalidValue;
+    *launches += 1;
+    if (cb == 32) return b.nv ? launch_t<1, 32>(ta, tb, p, grid, st) : launch_t<0, 32>(ta, tb, p, grid, st);
+    return b.nv ? launch_t<1, 128>(ta, tb, p, grid, st) : launch_t<0, 128>(ta, tb, p, grid, st);
+}
+
+}  // namespace rfx

@@ -17,6 +17,7 @@
 
 #include "rfx_ctx.h"
 #include "rfx_lowrank.h"
+#include "rfx_tma_host.h"
 
 namespace rfxh {
 
@@ -126,6 +127,8 @@ void orth(Ctx& c, float* Y, int r, float* Q, double* G, double* Uinv) {
     RFX_CUDA(cudaMemcpyAsync(Q, src, (size_t)R * r * 4, cudaMemcpyDeviceToDevice, st));
 }
 
+}  // namespace
+
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     static std::mutex mu;
     static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
@@ -140,6 +143,8 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     }
     return fn;
 }
+
+namespace {
 
 // Tensor map of the bf16 factor rows [Rpad][64]: boxes of 128 rows x 64 columns, 128-byte
 // swizzle (one box row is exactly one 128-byte swizzle span).
@@ -404,6 +409,7 @@ int rfx_lowrank_build(void* ctx, int rank, int oversample, int power_iters, uint
         cudaStream_t st = c.st;
         const int R = c.R;
         const int* nout = nout_dev ? nout_dev : (const int*)c.nout.p;
+        c.lr_float = c.lr4_ready = false;
         float* X = (float*)c.lr_X.get((size_t)R * r * 4);
         float* Y = (float*)c.lr_Y.get((size_t)R * r * 4);
         float* Q = (float*)c.lr_A.get((size_t)R * r * 4);
@@ -439,6 +445,7 @@ int rfx_lowrank_build(void* ctx, int rank, int oversample, int power_iters, uint
         RFX_LAUNCH("k_lr_quantize");
         c.launches += 4;
         order_factors(c, R, rank);
+        c.lr_float = true;
     });
 }
 
@@ -455,6 +462,7 @@ int rfx_lowrank_set_factors(void* ctx, const int8_t* q_host, const float* scale_
                     "scales must be finite and non-negative");
         cudaStream_t st = c.st;
         const int Rpad = (int)round_up(rows, rfx::kTkCols);
+        c.lr_float = c.lr4_ready = false;
         int8_t* qin = (int8_t*)c.lr_X.get((size_t)rows * rank);
         float* sin = (float*)c.lr_Y.get((size_t)rows * 4);
         RFX_CUDA(cudaMemcpyAsync(qin, q_host, (size_t)rows * rank, cudaMemcpyHostToDevice, st));

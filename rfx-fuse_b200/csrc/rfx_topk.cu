@@ -39,114 +39,16 @@
 #include <cstdint>
 
 #include "rfx_lowrank.h"
+#include "rfx_tc.cuh"
 
 namespace rfx {
 
 namespace {
 
-constexpr unsigned long long kWaitNs = 1000000000ull;
-// A sleeping waiter stays in try_wait until the phase completes or this many nanoseconds pass.
-constexpr uint32_t kSuspendNs = 2000;
 #ifndef RFX_TK_CHECK
 #define RFX_TK_CHECK 4
 #endif
 constexpr int kTkCheck = RFX_TK_CHECK;  // tiles between flush + finality checks
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-    return (uint32_t)__cvta_generic_to_shared(p);
-}
-
-__device__ __forceinline__ unsigned long long now_ns() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-
-template <bool kSleep>
-__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    if (kSleep) {
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}\n"
-            : "=r"(ok)
-            : "r"(bar), "r"(parity), "r"(kSuspendNs)
-            : "memory");
-    } else {
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}\n"
-            : "=r"(ok)
-            : "r"(bar), "r"(parity)
-            : "memory");
-    }
-    return ok != 0;
-}
-
-// Wait for the phase of `parity` to complete.  Returns kWaitOk, or kWaitFail on timeout or
-// when another role of the CTA has aborted (abort may be null: wait regardless), or
-// kWaitStop once step `it` is at or beyond the CTA's stop limit (limit may be null).
-constexpr int kWaitFail = 0, kWaitOk = 1, kWaitStop = 2;
-
-template <bool kSleep = true>
-__device__ int mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort,
-                         unsigned long long* polls = nullptr, volatile int* limit = nullptr,
-                         int it = 0) {
-    const unsigned long long t0 = now_ns();
-    for (uint32_t spin = 1;; ++spin) {
-        if (polls) ++*polls;
-        if (mbar_try<kSleep>(bar, parity)) return kWaitOk;
-        if (limit && it >= *limit) return kWaitStop;
-        if (abort && *abort) return kWaitFail;
-        if ((spin & 15u) == 0 && now_ns() - t0 > kWaitNs) return kWaitFail;
-    }
-}
-
-// mbar_wait that also adds the cycles it spent to *cyc.
-template <bool kSleep = true>
-__device__ __forceinline__ int mbar_wait_t(uint32_t bar, uint32_t parity, volatile int* abort,
-                                           unsigned long long* polls, unsigned long long* cyc,
-                                           volatile int* limit = nullptr, int it = 0) {
-    const long long t0 = clock64();
-    const int r = mbar_wait<kSleep>(bar, parity, abort, polls, limit, it);
-    *cyc += (unsigned long long)(clock64() - t0);
-    return r;
-}
-
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
-                 : "memory");
-}
-
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-
-// 2-D tiled TMA load (box 64 x 128 of bf16) into shared memory, completing on `bar`.
-__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* tm, int x, int y,
-                                         uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-        "l"((unsigned long long)tm), "r"(x), "r"(y), "r"(bar)
-        : "memory");
-}
-
-// Shared-memory matrix descriptor: K-major, 128-byte swizzle, 8-row groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t addr) {
-    uint64_t d = (uint64_t)((addr & 0x3FFFFu) >> 4);  // start address
-    d |= (uint64_t)1 << 16;                           // leading offset (unused when swizzled)
-    d |= (uint64_t)(1024 >> 4) << 32;                 // stride offset
-    d |= (uint64_t)1 << 46;                           // descriptor version
-    d |= (uint64_t)2 << 61;                           // 128-byte swizzle
-    return d;
-}
 
 // Instruction descriptor of kind::f16: bf16 x bf16 -> fp32, both K-major, M = 128, N = 256.
 constexpr uint32_t kIdesc = (1u << 4)            // D fp32
@@ -162,48 +64,6 @@ __device__ __forceinline__ void mma_bf16(uint32_t tmem_d, uint64_t da, uint64_t 
         "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d),
         "l"(da), "l"(db), "r"(kIdesc), "r"(acc)
         : "memory");
-}
-
-__device__ __forceinline__ void mma_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
-                 : "memory");
-}
-
-__device__ __forceinline__ void tc_fence_before() {
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-
-// Issue a load of 32 consecutive fp32 accumulator columns of this thread's TMEM lane; the
-// registers are valid after tmem_wait().
-__device__ __forceinline__ void tmem_ld32_issue(uint32_t taddr, uint32_t* r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-          "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
-          "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
-          "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-}
-
-__device__ __forceinline__ void tmem_wait() {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-
-// Ties 32 loaded registers to a point after tmem_wait() so no use moves above the wait.
-__device__ __forceinline__ void tmem_pin32(uint32_t* r) {
-    asm volatile(""
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
-                   "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
-                   "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]),
-                   "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
-                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
-                   "+r"(r[30]), "+r"(r[31]));
 }
 
 // The best k of one row are kept as a 4-ary heap in shared memory whose root is the
@@ -260,13 +120,6 @@ __device__ __forceinline__ void heap_replace_root(float* v, int* j, int n, float
     }
     v[i * kTkRows] = val;
     j[i * kTkRows] = col;
-}
-
-// Largest of three floats (the three-input max.f32 of sm_100).
-__device__ __forceinline__ float fmax3(float x, float y, float z) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(x), "f"(y), "f"(z));
-    return d;
 }
 
 // Two fp32 products in one packed instruction (mul.rn.f32x2 of sm_100; each lane of the pair

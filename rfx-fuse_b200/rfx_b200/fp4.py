@@ -1,0 +1,292 @@
+"""Matrices in microscaled 4 bits on the device: quantisation, products, nearest rows.
+
+    A = rfx_b200.fp4_quantize(x)              # x: CUDA tensor [rows, cols], float32/bfloat16/float16
+    A.dequantize()                            # float32 [rows, cols]
+    rfx_b200.fp4_product(A, B)                # A B^T, float32 [A.rows, B.rows]
+    rfx_b200.fp4_topk(A, B, 50)               # (indices int32, values float32) [A.rows, 50]
+
+Rows are e2m1 codes with one scale per block of columns: "nvfp4" (16 columns, e4m3 scales and one
+power of two for the matrix; the closer of the two) or "mxfp4" (32 columns, power-of-two scales).
+include/rfx_b200.h states the formats and the operators exactly.
+
+Calls run on the current torch stream of the tensors' device, allocate from torch's caching
+allocator, do not synchronise, and can be captured into a CUDA graph once they have run before.
+Tensors made on another stream need the caller's event or ``wait_stream``, as with torch's own
+operators.  There is no gradient: results never require one.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+from . import _abi as A
+
+FORMATS = {"mxfp4": 0, "nvfp4": 1}
+_BLOCK = {"mxfp4": 32, "nvfp4": 16}
+TOPK_MAX_COLS = 256
+TOPK_MAX_K = 64
+
+
+class _Matrix(C.Structure):
+    _fields_ = [("format", C.c_int), ("rows", C.c_int), ("cols", C.c_int), ("codes_dev", C.c_void_p),
+                ("scales_dev", C.c_void_p), ("scale_dev", C.c_void_p), ("bounds_dev", C.c_void_p)]
+
+
+class _Layout(C.Structure):
+    _fields_ = [(n, C.c_longlong) for n in ("codes", "scales", "scale", "bounds", "pitch", "tile_bytes")]
+
+
+_LIB = None
+
+
+def _lib():
+    global _LIB
+    if _LIB is None:
+        L = A.load_library()
+        vp, i, ll, pm = C.c_void_p, C.c_int, C.c_longlong, C.POINTER(_Matrix)
+        L.rfx_fp4_sizes.argtypes = [i, i, i, C.POINTER(_Layout)]
+        L.rfx_fp4_quantize.argtypes = [vp, i, ll, pm, vp]
+        L.rfx_fp4_dequantize.argtypes = [pm, i, i, vp, i, ll, vp]
+        L.rfx_fp4_pack.argtypes = [vp, vp, vp, pm, vp]
+        L.rfx_fp4_unpack.argtypes = [pm, vp, vp, vp]
+        L.rfx_fp4_product.argtypes = [pm, pm, vp, i, ll, vp]
+        L.rfx_fp4_topk_workspace.argtypes = [pm, pm, i, C.POINTER(ll)]
+        L.rfx_fp4_topk.argtypes = [pm, pm, i, ll, vp, vp, vp, ll, vp]
+        for n in ("sizes", "quantize", "dequantize", "pack", "unpack", "product", "topk_workspace",
+                  "topk", "status"):
+            getattr(L, "rfx_fp4_" + n).restype = C.c_int
+        _LIB = L
+    return _LIB
+
+
+def _dtype_code(dtype):
+    import torch
+    code = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}.get(dtype)
+    if code is None:
+        raise TypeError(f"dtype must be float32, bfloat16 or float16, not {dtype}")
+    return code
+
+
+def _check_format(format):
+    if format not in FORMATS:
+        raise ValueError(f"format must be 'mxfp4' or 'nvfp4', not {format!r}")
+
+
+class _on:
+    """The tensors' device as the current one, and its current stream's handle."""
+
+    def __init__(self, device):
+        import torch
+        self._torch = torch
+        self._device = device
+        self._before = None
+
+    def __enter__(self):
+        cuda = self._torch.cuda
+        before = cuda.current_device()
+        if before != self._device.index:
+            self._before = before
+            cuda.set_device(self._device)
+        return cuda.current_stream(self._device).cuda_stream
+
+    def __exit__(self, *exc):
+        if self._before is not None:
+            self._torch.cuda.set_device(self._before)
+
+
+class Fp4Matrix:
+    """A [rows, cols] matrix in 4 bits on a CUDA device.  Made by ``fp4_quantize`` or
+    ``from_parts``; its layout is the library's.  Treated as constant once made."""
+
+    __slots__ = ("format", "shape", "device", "_c", "_layout", "_keep")
+
+    def __init__(self, *_):
+        raise TypeError("use fp4_quantize or Fp4Matrix.from_parts")
+
+    @classmethod
+    def _empty(cls, rows, cols, format, device):
+        import torch
+        m = object.__new__(cls)
+        lay = _Layout()
+        A.check(_lib().rfx_fp4_sizes(FORMATS[format], rows, cols, C.byref(lay)))
+        codes = (lay.codes + 255) & ~255
+        buf = torch.empty(codes + lay.scales + 256 + lay.bounds, dtype=torch.uint8, device=device)
+        p = buf.data_ptr()
+        m.format, m.shape, m.device = format, (rows, cols), buf.device
+        m._layout, m._keep = lay, buf
+        m._c = _Matrix(FORMATS[format], rows, cols, p, p + codes, p + codes + lay.scales,
+                       p + codes + lay.scales + 256)
+        return m
+
+    @classmethod
+    def from_parts(cls, codes, scales, scale=None, *, cols, format="nvfp4"):
+        """From codes uint8 [rows, ceil(cols / 2)] (two a byte, even column in the low half),
+        scale bytes uint8 [rows, ceil(cols / block)] (e8m0 for "mxfp4", unsigned e4m3 for
+        "nvfp4") and the matrix scale: a positive number or one-element float32 tensor on the
+        same device ("nvfp4" only; None: 1)."""
+        import torch
+        _check_format(format)
+        cols = int(cols)
+        if cols < 1:
+            raise ValueError("cols must be at least 1")
+        for name, t, width in (("codes", codes, (cols + 1) // 2), ("scales", scales, -(-cols // _BLOCK[format]))):
+            if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.uint8:
+                raise TypeError(f"{name} must be a CUDA uint8 tensor")
+            if t.dim() != 2 or t.shape[1] != width:
+                raise ValueError(f"{name} must be [rows, {width}], not {tuple(t.shape)}")
+        if codes.shape[0] != scales.shape[0] or codes.device != scales.device:
+            raise ValueError("codes and scales must have the same rows and device")
+        if isinstance(scale, torch.Tensor):
+            if scale.device != codes.device or scale.dtype != torch.float32 or scale.numel() != 1:
+                raise ValueError("scale must be one float32 on the codes' device")
+            if format == "mxfp4":
+                raise ValueError("mxfp4 has no matrix scale")
+        elif scale is not None:
+            scale = float(scale)
+            if not 0.0 < scale < float("inf"):
+                raise ValueError("scale must be positive and finite")
+            if format == "mxfp4" and scale != 1.0:
+                raise ValueError("mxfp4 has no matrix scale")
+        m = cls._empty(codes.shape[0], cols, format, codes.device)
+        with _on(m.device) as st:
+            codes, scales = codes.contiguous(), scales.contiguous()
+            if scale is not None and not isinstance(scale, torch.Tensor):
+                scale = None if scale == 1.0 else torch.full((1,), scale, dtype=torch.float32, device=m.device)
+            A.check(_lib().rfx_fp4_pack(codes.data_ptr(), scales.data_ptr(),
+                                        None if scale is None else scale.data_ptr(), C.byref(m._c), st))
+        return m
+
+    def parts(self):
+        """(codes, scales, scale), the arguments of ``from_parts``."""
+        import torch
+        rows, cols = self.shape
+        codes = torch.empty((rows, (cols + 1) // 2), dtype=torch.uint8, device=self.device)
+        scales = torch.empty((rows, -(-cols // _BLOCK[self.format])), dtype=torch.uint8, device=self.device)
+        with _on(self.device) as st:
+            A.check(_lib().rfx_fp4_unpack(C.byref(self._c), codes.data_ptr(), scales.data_ptr(), st))
+        if self.format == "mxfp4":
+            return codes, scales, None
+        at = self._c.scale_dev - self._keep.data_ptr()
+        return codes, scales, self._keep[at:at + 4].view(torch.float32).clone()
+
+    def rows(self, begin, end):
+        """Rows [begin, end) as a matrix that shares this one's memory; begin a multiple of 128."""
+        n = self.shape[0]
+        if not 0 <= begin <= end <= n:
+            raise ValueError(f"rows [{begin}, {end}) are not in [0, {n}]")
+        if begin % 128:
+            raise ValueError("a view starts at a multiple of 128 rows")
+        m = object.__new__(Fp4Matrix)
+        m.format, m.shape, m.device = self.format, (end - begin, self.shape[1]), self.device
+        m._layout, m._keep = self._layout, self._keep
+        c, lay = self._c, self._layout
+        m._c = _Matrix(c.format, end - begin, c.cols, c.codes_dev + begin * lay.pitch,
+                       c.scales_dev + begin // 128 * lay.tile_bytes, c.scale_dev, c.bounds_dev + begin // 128 * 4)
+        return m
+
+    def dequantize(self, dtype=None, *, out=None):
+        """The values [rows, cols]; exact in float32 and bfloat16 for a quantised matrix."""
+        import torch
+        dtype = torch.float32 if dtype is None and out is None else (out.dtype if dtype is None else dtype)
+        code = _dtype_code(dtype)
+        out = _out(out, self.shape, dtype, self.device)
+        with _on(self.device) as st:
+            A.check(_lib().rfx_fp4_dequantize(C.byref(self._c), 0, self.shape[0], out.data_ptr(), code,
+                                              _row_stride(out), st))
+        return out
+
+    def __repr__(self):
+        return f"Fp4Matrix({self.shape[0]} x {self.shape[1]}, {self.format}, {self.device})"
+
+
+def _row_stride(t):
+    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else max(1, t.shape[1])
+
+
+def _out(out, shape, dtype, device):
+    import torch
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if not isinstance(out, torch.Tensor) or out.device != device or out.dtype != dtype or tuple(out.shape) != tuple(shape):
+        raise ValueError(f"out must be a {dtype} tensor of shape {tuple(shape)} on {device}")
+    if out.requires_grad:
+        raise ValueError("out must not require a gradient")
+    if out.shape[1] > 1 and out.stride(1) != 1 or out.shape[0] > 1 and out.stride(0) < out.shape[1]:
+        raise ValueError("out must have unit stride along its rows and rows that do not overlap")
+    return out
+
+
+def _pair(a, b):
+    if not isinstance(a, Fp4Matrix) or not isinstance(b, Fp4Matrix):
+        raise TypeError("a and b must be Fp4Matrix")
+    if a.format != b.format or a.shape[1] != b.shape[1] or a.device != b.device:
+        raise ValueError(f"a and b must share format, columns and device: {a} and {b}")
+
+
+def fp4_quantize(x, format="nvfp4"):
+    """x [rows, cols] (CUDA float32, bfloat16 or float16, unit stride along its rows) in 4 bits."""
+    import torch
+    _check_format(format)
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise TypeError("x must be a CUDA tensor")
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError("x must be [rows, cols] with at least one column")
+    code = _dtype_code(x.dtype)
+    rows, cols = x.shape
+    if cols > 1 and x.stride(1) != 1 or rows > 1 and x.stride(0) < cols:
+        raise ValueError("x must have unit stride along its rows and rows that do not overlap")
+    m = Fp4Matrix._empty(rows, cols, format, x.device)
+    with _on(m.device) as st:
+        A.check(_lib().rfx_fp4_quantize(x.data_ptr(), code, _row_stride(x), C.byref(m._c), st))
+    return m
+
+
+def fp4_product(a, b, dtype=None, *, out=None):
+    """a b^T [a.rows, b.rows]: fp32 accumulation on the tensor cores, rounded once to ``dtype``
+    (float32 by default, bfloat16 or float16)."""
+    import torch
+    _pair(a, b)
+    dtype = torch.float32 if dtype is None and out is None else (out.dtype if dtype is None else dtype)
+    code = _dtype_code(dtype)
+    out = _out(out, (a.shape[0], b.shape[0]), dtype, a.device)
+    with _on(a.device) as st:
+        A.check(_lib().rfx_fp4_product(C.byref(a._c), C.byref(b._c), out.data_ptr(), code, _row_stride(out), st))
+    return out
+
+
+def fp4_topk(queries, rows, k, *, self_offset=None):
+    """The k rows with the largest product for every query: (indices int32, values float32)
+    [queries, k], exact value descending, then index ascending; slots without a neighbour hold
+    -1 and -inf.  self_offset: query i is row self_offset + i of ``rows`` and left out for it.
+    k <= 64, at most 256 columns."""
+    import torch
+    _pair(queries, rows)
+    k = int(k)
+    if not 1 <= k <= TOPK_MAX_K:
+        raise ValueError(f"k must be in [1, {TOPK_MAX_K}]")
+    if queries.shape[1] > TOPK_MAX_COLS:
+        raise ValueError(f"fp4_topk takes at most {TOPK_MAX_COLS} columns")
+    off = -1
+    if self_offset is not None:
+        off = int(self_offset)
+        if off < 0 or off + queries.shape[0] > rows.shape[0]:
+            raise ValueError("self_offset must place the queries inside the rows")
+    L = _lib()
+    idx = torch.empty((queries.shape[0], k), dtype=torch.int32, device=queries.device)
+    val = torch.empty((queries.shape[0], k), dtype=torch.float32, device=queries.device)
+    with _on(queries.device) as st:
+        need = C.c_longlong()
+        A.check(L.rfx_fp4_topk_workspace(C.byref(queries._c), C.byref(rows._c), k, C.byref(need)))
+        ws = torch.empty(need.value, dtype=torch.uint8, device=queries.device)
+        A.check(L.rfx_fp4_topk(C.byref(queries._c), C.byref(rows._c), k, off, idx.data_ptr(), val.data_ptr(),
+                               ws.data_ptr(), need.value, st))
+    return idx, val
+
+
+def fp4_status(device=None):
+    """Wait for the device and raise RfxError if a 4-bit product or top-k kernel on it reported a
+    pipeline wait that timed out since the last call."""
+    import torch
+    d = torch.device("cuda", torch.cuda.current_device() if device is None else torch.device(device).index
+                     if not isinstance(device, int) else device)
+    with _on(d):
+        A.check(_lib().rfx_fp4_status())

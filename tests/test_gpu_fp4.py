@@ -1,0 +1,257 @@
+"""Microscaled 4-bit matrices on the device against 64-bit numpy: quantisation and its inverse bit
+for bit, products to the bound of their fp32 accumulation, top-k exactly."""
+import numpy as np
+import pytest
+
+import _fp4_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+FMTS = ["nvfp4", "mxfp4"]
+HALF = {"float32": 2.0 ** -24, "bfloat16": 2.0 ** -8, "float16": 2.0 ** -11}  # half a step, relative
+
+
+def _dev(a):
+    import torch
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def _parts(rng, rows, cols, fmt, spread=4):
+    """Random codes and scales: every code, scales over a few binades, some zero blocks."""
+    nb = -(-cols // ref.BLOCK[fmt])
+    codes = rng.integers(0, 16, (rows, cols)).astype(np.uint8)
+    if fmt == "mxfp4":
+        scales = rng.integers(127 - spread, 127 + spread + 1, (rows, nb)).astype(np.uint8)
+    else:
+        scales = rng.integers(8 * (7 - spread), 8 * (7 + spread) + 1, (rows, nb)).astype(np.uint8)
+        scales[rng.random((rows, nb)) < 0.05] = 0
+    return codes, scales
+
+
+def _matrix(codes, scales, cols, fmt, g=None):
+    import rfx_b200
+    return rfx_b200.Fp4Matrix.from_parts(_dev(ref.pack(codes)), _dev(scales), g, cols=cols, format=fmt)
+
+
+def _same(got, want):
+    got, want = np.asarray(got), np.asarray(want)
+    assert got.shape == want.shape
+    nan = np.isnan(want)
+    assert np.array_equal(np.isnan(got), nan)
+    bad = np.argwhere((got != want) & ~nan)
+    assert len(bad) == 0, (len(bad), bad[:4].tolist(), got[tuple(bad[0])], want[tuple(bad[0])])
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 15), (5, 16), (2, 17), (128, 64), (129, 33), (300, 50), (40, 256),
+                                       (70, 257), (20, 1000), (257, 511), (5, 4097)])
+def test_quantize_matches_the_definition(fmt, rows, cols):
+    import torch
+    import rfx_b200
+    rng = np.random.default_rng(rows * 7919 + cols)
+    x = (rng.normal(size=(rows, cols)) * np.exp(rng.normal(size=(rows, 1)))).astype(np.float32)
+    for dt in (torch.float32, torch.bfloat16, torch.float16):
+        t = torch.from_numpy(x).cuda().to(dt)
+        m = rfx_b200.fp4_quantize(t, format=fmt)
+        codes, scales, g = ref.quantize(t.double().cpu().numpy(), fmt)
+        c, s, gs = m.parts()
+        assert np.array_equal(s.cpu().numpy(), scales)
+        _same(ref.values(ref.unpack(c.cpu().numpy(), cols), scales, g, fmt), ref.values(codes, scales, g, fmt))
+        if fmt == "nvfp4":
+            assert float(gs) == g
+        want = ref.values(codes, scales, g, fmt)
+        for odt in (torch.float32, torch.bfloat16):  # both hold the values exactly
+            _same(m.dequantize(odt).double().cpu().numpy(), want)
+        _same(m.dequantize(torch.float16).cpu().numpy(), want.astype(np.float32).astype(np.float16))
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_quantize_borders(fmt):
+    """Values on, just below and just above every border between two codes and two scales."""
+    import torch
+    import rfx_b200
+    rng = np.random.default_rng(2)
+    mids = (ref.E2M1[1:] + ref.E2M1[:-1]) / 2
+    rows = []
+    for scale in list(ref.E4M3[1::5]) + [2.0 ** -20, 3.0, 1e-3]:
+        for amax in (6.0, 4.5, 5.3125, 6.1875, 3.0):
+            v = np.concatenate([mids, ref.E2M1, [5.9]])
+            base = np.float32(v * scale)
+            up, dn = np.nextafter(base, np.float32(np.inf)), np.nextafter(base, np.float32(-np.inf))
+            for b in (base, up, dn):
+                r = np.zeros(32, np.float32)
+                r[:16] = b * np.where(rng.random(16) < 0.5, -1, 1)
+                r[16:] = b
+                r[0] = r[16] = np.float32(amax * scale)
+                rows.append(r)
+    # a block maximum on the borders between two scales, and beside them
+    edge = (ref.E4M3[1:] + ref.E4M3[:-1]) / 2 * 6
+    for b in (np.float32(edge), np.nextafter(np.float32(edge), np.float32(1e9)), np.nextafter(np.float32(edge), np.float32(0))):
+        for v in b:
+            r = np.zeros(32, np.float32)
+            r[5] = r[21] = v
+            rows.append(r)
+    rows.append(np.full(32, 2688.0, np.float32))  # g = 1
+    x = np.stack(rows)
+    m = rfx_b200.fp4_quantize(torch.from_numpy(x).cuda(), format=fmt)
+    codes, scales, g = ref.quantize(x, fmt)
+    assert np.array_equal(m.parts()[1].cpu().numpy(), scales)
+    _same(m.dequantize().double().cpu().numpy(), ref.values(codes, scales, g, fmt))
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_quantize_extremes(fmt):
+    """Zeros, denormals, the largest floats, infinities and NaN, strided and unaligned rows."""
+    import torch
+    import rfx_b200
+    big = np.float32(3.0e38)
+    x = np.zeros((9, 70), np.float32)
+    x[1, :] = 1e-45
+    x[2, 3] = big
+    x[3, ::2] = -1e-38
+    x[4, 7] = np.inf
+    x[5, 40] = np.nan
+    x[6, :] = np.linspace(-1, 1, 70)
+    x[7, :] = -0.0
+    x[8, 69] = -np.inf
+    for rowset in (range(9), [0, 1, 3], [0], [4, 5], [6, 7]):
+        y = x[list(rowset)]
+        buf = torch.zeros((len(y), 77), device="cuda")
+        buf[:, 3:73] = torch.from_numpy(y)
+        m = rfx_b200.fp4_quantize(buf[:, 3:73], format=fmt)
+        codes, scales, g = ref.quantize(y, fmt)
+        assert np.array_equal(m.parts()[1].cpu().numpy(), scales), rowset
+        with np.errstate(over="ignore"):
+            want = ref.values(codes, scales, g, fmt).astype(np.float32)
+        _same(m.dequantize().cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("rows,cols", [(1, 1), (130, 31), (128, 128), (77, 300), (300, 640)])
+def test_parts_round_trip(fmt, rows, cols):
+    import torch
+    rng = np.random.default_rng(rows + cols)
+    codes, scales = _parts(rng, rows, cols, fmt)
+    g = None if fmt == "mxfp4" else 0.375
+    m = _matrix(codes, scales, cols, fmt, g)
+    c, s, gs = m.parts()
+    assert np.array_equal(ref.unpack(c.cpu().numpy(), cols), codes) and np.array_equal(s.cpu().numpy(), scales)
+    want = ref.values(codes, scales, 1.0 if g is None else g, fmt)
+    _same(m.dequantize().double().cpu().numpy(), want.astype(np.float32))
+    out = torch.full((rows, cols + 5), -7.0, device="cuda")
+    m.dequantize(out=out[:, 2:2 + cols])
+    _same(out[:, 2:2 + cols].cpu().numpy(), want.astype(np.float32))
+    assert (out[:, :2] == -7).all() and (out[:, 2 + cols:] == -7).all()
+    if gs is not None:
+        assert float(gs) == g
+
+
+def _product_check(rng, fmt, m, n, k, dtype="float32", spread=4):
+    import torch
+    import rfx_b200
+    ca, sa = _parts(rng, m, k, fmt, spread)
+    cb, sb = _parts(rng, n, k, fmt, spread)
+    va, vb = ref.values(ca, sa, 1.0, fmt), ref.values(cb, sb, 1.0, fmt)
+    a, b = _matrix(ca, sa, k, fmt), _matrix(cb, sb, k, fmt)
+    buf = torch.full((m, n + 3), -7.0, device="cuda", dtype=getattr(torch, dtype))
+    out = rfx_b200.fp4_product(a, b, out=buf[:, :n])
+    rfx_b200.fp4_status()
+    got = out.double().cpu().numpy()
+    want, size = va @ vb.T, np.abs(va) @ np.abs(vb).T
+    # products are exact; k fp32 additions, each off by at most a unit of the last place (2^-23)
+    # of a partial sum, none of which exceeds `size`; then one rounding to the output type
+    tol = k * 2.0 ** -23 * size
+    tol = tol + HALF[dtype] * (np.abs(want) + tol) + (2.0 ** -25 if dtype == "float16" else 0)
+    bad = np.argwhere(~(np.abs(got - want) <= tol))
+    assert len(bad) == 0, (len(bad), bad[:3].tolist(), got[tuple(bad[0])], want[tuple(bad[0])], tol[tuple(bad[0])])
+    assert (buf[:, n:] == -7).all()
+    print(f"worst error / size: {np.max(np.abs(got - want) / np.maximum(size, 1e-300)):.3g}")
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("m,n,k", [(16, 128, 64), (1, 1, 1), (128, 128, 64), (256, 256, 64), (1, 300, 17), (17, 129, 128),
+                                   (129, 130, 192), (100, 257, 256), (33, 200, 320), (300, 500, 1000), (257, 640, 65),
+                                   (513, 3000, 64), (70, 1000, 4100)])
+def test_product(fmt, m, n, k):
+    _product_check(np.random.default_rng(m + 1000 * n + k), fmt, m, n, k)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_product_half_outputs(fmt, dtype):
+    rng = np.random.default_rng(5)
+    for m, n, k in ((1, 100, 64), (65, 260, 50), (300, 301, 300)):
+        _product_check(rng, fmt, m, n, k, dtype, spread=1)
+
+
+def _topk_check(a, b, va, vb, k, fmt, self_offset=None):
+    import rfx_b200
+    idx, val = rfx_b200.fp4_topk(a, b, k, self_offset=self_offset)
+    rfx_b200.fp4_status()
+    wi, wv = ref.topk(va, vb, k, self_offset, fmt)
+    idx, val = idx.cpu().numpy(), val.cpu().numpy()
+    bad = np.argwhere(idx != wi)
+    assert len(bad) == 0, (len(bad), bad[:4].tolist(), idx[tuple(bad[0])], wi[tuple(bad[0])])
+    assert np.array_equal(val, wv)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("m,n,k,top", [(1, 1, 1, 1), (5, 40, 64, 7), (128, 128, 64, 50), (130, 700, 37, 50), (3, 5000, 64, 64),
+                                       (300, 2000, 200, 10), (64, 3001, 256, 33), (1, 20000, 96, 50)])
+def test_topk(fmt, m, n, k, top):
+    rng = np.random.default_rng(m * 31 + n + k)
+    ca, sa = _parts(rng, m, k, fmt)
+    cb, sb = _parts(rng, n, k, fmt)
+    _topk_check(_matrix(ca, sa, k, fmt), _matrix(cb, sb, k, fmt), ref.values(ca, sa, 1.0, fmt),
+                ref.values(cb, sb, 1.0, fmt), top, fmt)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_topk_ties_and_self(fmt):
+    """Duplicated rows (equal values rank by index), zero rows, negative products, self left out."""
+    rng = np.random.default_rng(8)
+    n, k = 3000, 40
+    c, s = _parts(rng, n, k, fmt, spread=1)
+    c[rng.integers(0, n, 800)] = c[5]
+    s[:] = s[0]
+    c[100:140] = 0
+    v = ref.values(c, s, 1.0, fmt)
+    m = _matrix(c, s, k, fmt)
+    for top in (1, 50, 64):
+        _topk_check(m, m, v, v, top, fmt, self_offset=0)
+    sub = m.rows(256, 700)
+    _topk_check(sub, m, v[256:700], v, 20, fmt, self_offset=256)
+    few = m.rows(0, 30)
+    _topk_check(few, few, v[:30], v[:30], 50, fmt, self_offset=0)  # fewer neighbours than k
+    one = m.rows(0, 1)
+    _topk_check(one, one, v[:1], v[:1], 3, fmt, self_offset=0)     # none at all
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_topk_all_rows_equal(fmt):
+    """Every product equal: the lowest indices win, however much passes the filter."""
+    rng = np.random.default_rng(4)
+    c, s = _parts(rng, 1, 64, fmt, spread=1)
+    c, s = np.repeat(c, 2500, 0), np.repeat(s, 2500, 0)
+    v = ref.values(c, s, 1.0, fmt)
+    m = _matrix(c, s, 64, fmt)
+    _topk_check(m.rows(0, 140), m, v[:140], v, 50, fmt)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_topk_extreme_scales_and_nan(fmt):
+    """Rows whose scale is NaN are nobody's neighbours; the largest and smallest scales."""
+    rng = np.random.default_rng(9)
+    n, k = 900, 64
+    c, s = _parts(rng, n, k, fmt)
+    s[rng.integers(0, n, 30), 0] = 255 if fmt == "mxfp4" else 127
+    if fmt == "mxfp4":
+        s[200:230] = rng.integers(0, 12, (30, s.shape[1]))
+        s[300:310] = rng.integers(180, 200, (10, s.shape[1]))
+    else:
+        s[200:230] = rng.integers(0, 4, (30, s.shape[1]))
+        s[300:310] = 126
+    with np.errstate(all="ignore"):
+        v = ref.values(c, s, 1.0, fmt)
+        m = _matrix(c, s, k, fmt)
+        _topk_check(m, m, v, v, 20, fmt, self_offset=0)
