@@ -55,8 +55,11 @@ __device__ __forceinline__ uint32_t e2m1_mag4(uint32_t w) {
 
 // 0x7F in the bytes whose code (low half of w) has its sign bit set, else 0.
 __device__ __forceinline__ uint32_t e2m1_neg4(uint32_t w) {
-    // a selector of 8 replicates the sign of byte 0 (0xFF), 0 copies it (0x80)
-    return __byte_perm(0x80u, 0u, w & 0x8888u) & 0x7F7F7F7Fu;
+    // a selector of 8 replicates the sign of byte 0 (0xFF), 0 copies it (0x80); __byte_perm drops
+    // the selectors' top bits
+    uint32_t d;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(0x80u), "r"(0u), "r"(w & 0x8888u));
+    return d & 0x7F7F7F7Fu;
 }
 
 // Value of one e2m1 code.
