@@ -16,6 +16,7 @@ LIB_PATH = os.path.join(HERE, "librfx_b200.so")
 RFX_OK = 0
 ERRORS = {-1: "RFX_ERR_ARG", -2: "RFX_ERR_CUDA", -3: "RFX_ERR_OOM", -4: "RFX_ERR_UNSUPPORTED",
           -5: "RFX_ERR_STATE", -6: "RFX_ERR_DEVICE", -7: "RFX_ERR_CANCELLED"}
+FP4_FORMATS = {"mxfp4": 0, "nvfp4": 1}
 TASK_CLASSIFICATION, TASK_REGRESSION, TASK_UNSUPERVISED = 0, 1, 2
 
 _pi = C.POINTER(C.c_int)
@@ -61,6 +62,18 @@ class Stats(C.Structure):
                 ("sketch_bytes", C.c_double)]
 
 
+class Fp4Struct(C.Structure):
+    """rfx_fp4_matrix"""
+    _fields_ = [("format", C.c_int), ("rows", C.c_int), ("cols", C.c_int),
+                ("codes_dev", C.c_void_p), ("scales_dev", C.c_void_p), ("scale_dev", C.c_void_p),
+                ("bounds_dev", C.c_void_p)]
+
+
+class Fp4Layout(C.Structure):
+    _fields_ = [(k, C.c_longlong) for k in ("codes", "scales", "scale", "bounds", "pitch",
+                                            "tile_bytes")]
+
+
 SYMBOLS = (
     "rfx_last_error", "rfx_abi_version", "rfx_device_count", "rfx_cached_bytes", "rfx_empty_cache",
     "rfx_create", "rfx_destroy",
@@ -75,6 +88,9 @@ SYMBOLS = (
     "rfx_leaf_top_k_similar", "rfx_leaf_proximity", "rfx_predict_leaves",
     "rfx_predict_top_k_similar", "rfx_leaf_select_anchors", "rfx_leaf_outlier_scores",
     "rfx_rank_scores_desc", "rfx_predict_outlier_scores",
+    "rfx_fp4_sizes", "rfx_fp4_quantize", "rfx_fp4_dequantize", "rfx_fp4_pack", "rfx_fp4_unpack",
+    "rfx_fp4_product", "rfx_fp4_topk_workspace", "rfx_fp4_topk", "rfx_fp4_status",
+    "rfx_lowrank_pack4", "rfx_lowrank4_factors", "rfx_lowrank4_topk", "rfx_lowrank4_product",
 )
 
 # int (*)(void* user, float* buf_dev, int64_t count): in-place sum over processes
@@ -143,6 +159,19 @@ def load_library(path: str = LIB_PATH):
     L.rfx_lowrank_product.argtypes = [vp, C.c_int, C.c_int, _pf]
     L.rfx_prox_apply.argtypes = [vp, vp, C.c_int, vp, vp]
     L.rfx_lowrank_set_factors.argtypes = [vp, C.POINTER(C.c_int8), _pf, C.c_int, C.c_int]
+    L.rfx_lowrank_pack4.argtypes = [vp, C.c_int]
+    L.rfx_lowrank4_factors.argtypes = [vp, _pf, C.POINTER(C.c_int), C.POINTER(C.c_int)]
+    L.rfx_lowrank4_topk.argtypes = [vp, C.c_int, C.c_int, C.c_int, _pi, _pf]
+    L.rfx_lowrank4_product.argtypes = [vp, C.c_int, C.c_int, _pf]
+    L.rfx_fp4_sizes.argtypes = [C.c_int, C.c_int, C.c_int, C.POINTER(Fp4Layout)]
+    pm, ll = C.POINTER(Fp4Struct), C.c_longlong
+    L.rfx_fp4_quantize.argtypes = [vp, C.c_int, ll, pm, vp]
+    L.rfx_fp4_dequantize.argtypes = [pm, C.c_int, C.c_int, vp, C.c_int, ll, vp]
+    L.rfx_fp4_pack.argtypes = [vp, vp, vp, pm, vp]
+    L.rfx_fp4_unpack.argtypes = [pm, vp, vp, vp]
+    L.rfx_fp4_product.argtypes = [pm, pm, vp, C.c_int, ll, vp]
+    L.rfx_fp4_topk_workspace.argtypes = [pm, pm, C.c_int, C.POINTER(ll)]
+    L.rfx_fp4_topk.argtypes = [pm, pm, C.c_int, ll, vp, vp, vp, ll, vp]
     L.rfx_load_forest.argtypes = [vp, C.POINTER(Forest)]
     L.rfx_impute_round.argtypes = [vp, _pf, _pu8, _pu8, C.c_int, C.c_int, _pi, C.c_int, _pf]
     L.rfx_impute_round_ex.argtypes = [vp, _pf, _pu8, _pu8, C.c_int, C.c_int, _pi, C.c_int,
@@ -174,7 +203,10 @@ def load_library(path: str = LIB_PATH):
                  "rfx_leaf_top_k_similar", "rfx_leaf_proximity", "rfx_predict_leaves",
                  "rfx_predict_top_k_similar", "rfx_leaf_select_anchors",
                  "rfx_leaf_outlier_scores", "rfx_rank_scores_desc",
-                 "rfx_predict_outlier_scores"):
+                 "rfx_predict_outlier_scores", "rfx_fp4_sizes", "rfx_fp4_quantize",
+                 "rfx_fp4_dequantize", "rfx_fp4_pack", "rfx_fp4_unpack", "rfx_fp4_product",
+                 "rfx_fp4_topk_workspace", "rfx_fp4_topk", "rfx_fp4_status", "rfx_lowrank_pack4",
+                 "rfx_lowrank4_factors", "rfx_lowrank4_topk", "rfx_lowrank4_product"):
         getattr(L, name).restype = C.c_int
     _LIB = L
     return L
@@ -510,6 +542,33 @@ class Context:
     def lowrank_product(self, r0: int, r1: int, R: int):
         out = np.zeros((r1 - r0, R), np.float32)
         check(self._lib.rfx_lowrank_product(self.handle, int(r0), int(r1), ptr(out, _pf)))
+        return out
+
+    # ---- low-rank proximity in 4 bits ----
+    def lowrank_pack4(self, format: str):
+        """Quantise the float factors of the last lowrank_build to 'mxfp4' or 'nvfp4'."""
+        if format not in FP4_FORMATS:
+            raise ValueError(f"format must be 'mxfp4' or 'nvfp4', not {format!r}")
+        check(self._lib.rfx_lowrank_pack4(self.handle, FP4_FORMATS[format]))
+
+    def lowrank4_factors(self):
+        """The 4-bit factors' values, float32 [R, rank]."""
+        k, R = C.c_int(), C.c_int()
+        check(self._lib.rfx_lowrank4_factors(self.handle, None, C.byref(k), C.byref(R)))
+        out = np.zeros((R.value, k.value), np.float32)
+        check(self._lib.rfx_lowrank4_factors(self.handle, ptr(out, _pf), None, None))
+        return out
+
+    def lowrank4_topk(self, k: int, r0: int, r1: int):
+        idx = np.zeros((max(r1 - r0, 0), max(k, 0)), np.int32)
+        val = np.zeros((max(r1 - r0, 0), max(k, 0)), np.float32)
+        check(self._lib.rfx_lowrank4_topk(self.handle, int(k), int(r0), int(r1), ptr(idx, _pi),
+                                          ptr(val, _pf)))
+        return idx, val
+
+    def lowrank4_product(self, r0: int, r1: int, R: int):
+        out = np.zeros((max(r1 - r0, 0), R), np.float32)
+        check(self._lib.rfx_lowrank4_product(self.handle, int(r0), int(r1), ptr(out, _pf)))
         return out
 
     def prox_apply(self, X_dev: int, ncols: int, Y_dev: int, nout_dev: int | None = None):

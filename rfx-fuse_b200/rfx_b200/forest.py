@@ -111,9 +111,9 @@ class _Forest:
         self.lowrank_oversample = int(lowrank_oversample)
         self.lowrank_power_iters = int(lowrank_power_iters)
         if self.use_qlora and self.compute_proximity:
-            if self.quant_mode.lower() != "int8":
-                raise NotImplementedError("low-rank proximity is stored as int8 factors: "
-                                          "use quant_mode='int8'")
+            if self.quant_mode.lower() not in ("int8",) + tuple(A.FP4_FORMATS):
+                raise NotImplementedError("low-rank proximity is stored as int8 or 4-bit factors: "
+                                          "use quant_mode='int8', 'nvfp4' or 'mxfp4'")
             if not 1 <= self.rank <= 64:
                 raise NotImplementedError("low-rank proximity rank must be in [1, 64]")
         self.n_bins = min(int(n_bins), 256)
@@ -160,6 +160,11 @@ class _Forest:
 
     def _lowrank_rank(self):
         return self.rank if (self.use_qlora and self.compute_proximity) else 0
+
+    def _lowrank4(self):
+        """The 4-bit format of the low-rank factors, None for int8."""
+        mode = self.quant_mode.lower()
+        return mode if mode in A.FP4_FORMATS else None
 
     def _context(self):
         if self._ctx is None:
@@ -231,6 +236,8 @@ class _Forest:
         if self._lowrank_rank():
             ctx.lowrank_build(self.rank, self.lowrank_oversample, self.lowrank_power_iters,
                               seed=self.iseed)
+            if self._lowrank4():
+                ctx.lowrank_pack4(self._lowrank4())
         self._trees = tr
         self._trees_full = False
         self.acc_ = acc
@@ -346,7 +353,7 @@ class _Forest:
         ctx.prox_dense(0, R, out)
         return out
 
-    # ---- low-rank proximity (use_qlora=True, quant_mode="int8")
+    # ---- low-rank proximity (use_qlora=True, quant_mode="int8", "nvfp4" or "mxfp4")
     def _check_lowrank(self):
         self._check()
         if not self._lowrank_rank():
@@ -356,15 +363,19 @@ class _Forest:
 
     def get_lowrank_factors(self):
         """(A float64 [n, r], B float64 [n, r], r) with proximity ~ A B^T and B = A, the
-        dequantised int8 factors (python/randomforest_py.cpp:2183-2223)."""
+        dequantised int8 or 4-bit factors (python/randomforest_py.cpp:2183-2223)."""
         self._check_lowrank()
-        Af, _, _ = self._context().lowrank_factors()
+        ctx = self._context()
+        Af = ctx.lowrank4_factors() if self._lowrank4() else ctx.lowrank_factors()[0]
         A64 = Af.astype(np.float64)
         return A64, A64.copy(), int(Af.shape[1])
 
     def get_lowrank_quantized(self):
         """(q int8 [n, r], scale float32 [n]): A_i = scale_i * q_i."""
         self._check_lowrank()
+        if self._lowrank4():
+            raise RuntimeError(f"the factors are held as {self._lowrank4()}: "
+                               "get_lowrank_factors() returns their values")
         _, q, s = self._context().lowrank_factors()
         return q, s
 
@@ -378,14 +389,19 @@ class _Forest:
             from .shard import lowrank_topk_sharded  # collective over the fit's ranks
             return lowrank_topk_sharded(self, k, dist)
         row_end = R if row_end is None else int(row_end)
-        return self._context().lowrank_topk(int(k), int(row_begin), row_end)
+        ctx = self._context()
+        topk = ctx.lowrank4_topk if self._lowrank4() else ctx.lowrank_topk
+        return topk(int(k), int(row_begin), row_end)
 
     def get_lowrank_product(self, row_begin=0, row_end=None):
-        """Rows of the reconstructed low-rank proximity (scale_i scale_j q_i . q_j)."""
+        """Rows of the reconstructed low-rank proximity (scale_i scale_j q_i . q_j, or the product
+        of the 4-bit rows)."""
         self._check_lowrank()
         R = self._lowrank_rows()
         row_end = R if row_end is None else int(row_end)
-        return self._context().lowrank_product(int(row_begin), row_end, R)
+        ctx = self._context()
+        product = ctx.lowrank4_product if self._lowrank4() else ctx.lowrank_product
+        return product(int(row_begin), row_end, R)
 
     def _lowrank_rows(self):
         return self.prox_rows if self.prox_rows else self.n_rows_

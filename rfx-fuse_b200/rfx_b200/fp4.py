@@ -20,42 +20,14 @@ import ctypes as C
 
 from . import _abi as A
 
-FORMATS = {"mxfp4": 0, "nvfp4": 1}
+FORMATS = A.FP4_FORMATS
 _BLOCK = {"mxfp4": 32, "nvfp4": 16}
 TOPK_MAX_COLS = 256
 TOPK_MAX_K = 64
 
 
-class _Matrix(C.Structure):
-    _fields_ = [("format", C.c_int), ("rows", C.c_int), ("cols", C.c_int), ("codes_dev", C.c_void_p),
-                ("scales_dev", C.c_void_p), ("scale_dev", C.c_void_p), ("bounds_dev", C.c_void_p)]
-
-
-class _Layout(C.Structure):
-    _fields_ = [(n, C.c_longlong) for n in ("codes", "scales", "scale", "bounds", "pitch", "tile_bytes")]
-
-
-_LIB = None
-
-
-def _lib():
-    global _LIB
-    if _LIB is None:
-        L = A.load_library()
-        vp, i, ll, pm = C.c_void_p, C.c_int, C.c_longlong, C.POINTER(_Matrix)
-        L.rfx_fp4_sizes.argtypes = [i, i, i, C.POINTER(_Layout)]
-        L.rfx_fp4_quantize.argtypes = [vp, i, ll, pm, vp]
-        L.rfx_fp4_dequantize.argtypes = [pm, i, i, vp, i, ll, vp]
-        L.rfx_fp4_pack.argtypes = [vp, vp, vp, pm, vp]
-        L.rfx_fp4_unpack.argtypes = [pm, vp, vp, vp]
-        L.rfx_fp4_product.argtypes = [pm, pm, vp, i, ll, vp]
-        L.rfx_fp4_topk_workspace.argtypes = [pm, pm, i, C.POINTER(ll)]
-        L.rfx_fp4_topk.argtypes = [pm, pm, i, ll, vp, vp, vp, ll, vp]
-        for n in ("sizes", "quantize", "dequantize", "pack", "unpack", "product", "topk_workspace",
-                  "topk", "status"):
-            getattr(L, "rfx_fp4_" + n).restype = C.c_int
-        _LIB = L
-    return _LIB
+_lib = A.load_library
+_Matrix, _Layout = A.Fp4Struct, A.Fp4Layout
 
 
 def _dtype_code(dtype):

@@ -137,6 +137,7 @@ def write(path: str, m: dict) -> None:
 # ---------------------------------------------------------------------------------------
 # Estimators <-> model files
 # ---------------------------------------------------------------------------------------
+# the format's only 4-bit code is nf4's: "mxfp4" and "nvfp4" are written as it (factors are not saved)
 _QUANT = {"fp32": 0, "fp16": 1, "int8": 2, "nf4": 3}
 _LOSS = {"gini": 0, "gini_impurity": 0, "mse": 3, "mean_squared_error": 3, "l2": 3}
 

@@ -171,7 +171,13 @@ def lowrank_topk_sharded(est, k: int, dist):
     order (rfx_lowrank_topk_part; each rank works on its own GPU from the identical factors)
     and gathered: every rank returns the full result.  Collective: every rank must call it."""
     rank, world = dist.get_rank(), dist.get_world_size()
-    rows, idx, val = est._context().lowrank_topk_part(int(k), rank, world)
+    if est._lowrank4():  # 4-bit factors: equal ranges of rows
+        n = est._lowrank_rows()
+        r0, r1 = n * rank // world, n * (rank + 1) // world
+        rows = np.arange(r0, r1)
+        idx, val = est._context().lowrank4_topk(int(k), r0, r1)
+    else:
+        rows, idx, val = est._context().lowrank_topk_part(int(k), rank, world)
     parts = [None] * world
     dist.all_gather_object(parts, (rows, idx, val))
     R = sum(len(p[0]) for p in parts)
@@ -308,6 +314,8 @@ def fit_sharded(est, X, y=None, dist=None, device=None):
 
             ctx.lowrank_build(est.rank, est.lowrank_oversample, est.lowrank_power_iters,
                               seed=est.iseed, nout_dev=t_nout.data_ptr(), reduce=reduce)
+            if est._lowrank4():
+                ctx.lowrank_pack4(est._lowrank4())
             est._sharded_nout = t_nout  # keeps the device counts alive
             est._shard_dist = dist
         torch.cuda.current_stream(dev).synchronize()

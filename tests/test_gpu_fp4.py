@@ -255,3 +255,46 @@ def test_topk_extreme_scales_and_nan(fmt):
         v = ref.values(c, s, 1.0, fmt)
         m = _matrix(c, s, k, fmt)
         _topk_check(m, m, v, v, 20, fmt, self_offset=0)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_estimator_in_4_bits(fmt):
+    """quant_mode: the factors are the float factors quantised; product and top-k follow them; the
+    operators together on the same factors give the same answers."""
+    import rfx_b200
+    from _helpers import synth
+    X, y = synth("multiclass", 700, 10, 5)
+    kw = dict(nsample=700, ntree=30, mdim=10, mtry=3, compute_proximity=True, compute_importance=False,
+              use_qlora=True, rank=24, show_progress=False)
+    est = rfx_b200.RandomForestClassifier(quant_mode=fmt, **kw)
+    est.fit(X, y)
+    A, B, r = est.get_lowrank_factors()
+    assert r == 24 and A.shape == (700, 24) and np.array_equal(A, B)
+    with pytest.raises(RuntimeError, match="held as"):
+        est.get_lowrank_quantized()
+    P = est.get_lowrank_product()
+    tol = 24 * 2.0 ** -23 * (np.abs(A) @ np.abs(A).T) + 2.0 ** -24 * np.abs(A @ A.T)
+    assert (np.abs(P - A @ A.T) <= tol).all()
+    assert np.array_equal(est.get_lowrank_product(301, 450), P[301:450])
+    wi, wv = ref.topk(A, A, 12, 0, fmt)
+    idx, val = est.get_lowrank_topk(12)
+    assert np.array_equal(idx, wi) and np.array_equal(val, wv)
+    idx, val = est.get_lowrank_topk(12, 333, 601)
+    assert np.array_equal(idx, wi[333:601]) and np.array_equal(val, wv[333:601])
+    # int8 factors of the same fit approximate the same floats: 4 bits within their own step
+    e8 = rfx_b200.RandomForestClassifier(quant_mode="int8", **kw)
+    e8.fit(X, y)
+    A8, _, _ = e8.get_lowrank_factors()
+    m = rfx_b200.fp4_quantize(_dev(A.astype(np.float32)), format=fmt)
+    # quantising the quantised values keeps them (their scales divide them exactly)
+    _same(m.dequantize().double().cpu().numpy(), A)
+    _same(rfx_b200.fp4_product(m, m).cpu().numpy(), P)
+    ti, tv = rfx_b200.fp4_topk(m, m, 12, self_offset=0)
+    assert np.array_equal(ti.cpu().numpy(), wi) and np.array_equal(tv.cpu().numpy(), wv)
+    step = np.abs(A8).max(1, keepdims=True) / 127 / 2
+    # a code is off by at most 1 in units of its block's scale (between 4 and 6), the scale is at
+    # most largest / 3 (mxfp4) or (1 + 2^-4) largest / 6 (nvfp4)
+    bs = ref.BLOCK[fmt]
+    for c in range(0, 24, bs):
+        big = np.abs(A8[:, c:c + bs]).max(1, keepdims=True) + step
+        assert (np.abs(A[:, c:c + bs] - A8[:, c:c + bs]) <= big / 3 + step).all()
