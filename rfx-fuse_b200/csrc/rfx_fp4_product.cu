@@ -60,7 +60,7 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
         }
         for (int b = 0; b < p.nacc; ++b) {
             mbar_init(accf(b), 1);
-            mbar_init(acce(b), p.nacc > 1 ? 128 : 256);
+            mbar_init(acce(b), p.nacc > 1 ? 4 : 8);  // one arrival a warp
         }
         *abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -80,84 +80,99 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
     if (warp == 8) {
         if (lane == 0) {
             int step = 0;
+            RingPos st;
             bool ok = true;
             for (int t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
                 const int jt = t % p.njt, i0 = t / p.njt * p.bn;
                 const int rt0 = i0 / kF4Tile;
                 const int rts = min(nrt, p.a.tiles() - rt0);
+                const uint8_t* sb = p.b.scales + (long long)jt * p.b.natoms * kF4Atom;
+                const uint8_t* sa = p.a.scales + (long long)rt0 * p.a.natoms * kF4Atom;
+                int left = p.b.Kp / 64;  // steps to go
                 for (int c = 0; c < p.nchunk; ++c, ++step) {
-                    const int s = step % p.nstage;
-                    if (mbar_wait(empty(s), ((uint32_t)(step / p.nstage) & 1u) ^ 1u, abort) != kWaitOk) {
+                    if (!mbar_wait_fast(empty(st.slot), st.parity ^ 1u, abort)) {
                         if (!*abort) atomicExch(p.err, 1);
                         *abort = 1;
                         ok = false;
                         break;
                     }
-                    const uint32_t st = stage0 + (uint32_t)(s * p.stage_bytes);
-                    const int left = (p.b.Kp - c * 2 * kCB) / 64;
+                    const uint32_t dst = stage0 + (uint32_t)(st.slot * p.stage_bytes), bar = full(st.slot);
                     const int steps = min(left, kCB / 32);
-                    const int atoms = kNv ? steps : (steps + 1) / 2;
-                    const uint32_t sfb = (uint32_t)(atoms * kF4Atom);
-                    mbar_expect_tx(full(s), (uint32_t)((128 + p.bn) * kCB) + sfb * (1 + rts));
-                    tma_load(st, &tmb, c * kCB, jt * 128, full(s));
-                    tma_load(st + off_b, &tma, c * kCB, i0, full(s));
-                    bulk_load(st + off_sb, p.b.scales + ((long long)jt * p.b.natoms + c * kAtoms) * kF4Atom, sfb, full(s));
-                    for (int r = 0; r < rts; ++r)
-                        bulk_load(st + off_sa + r * kAtoms * kF4Atom,
-                                  p.a.scales + ((long long)(rt0 + r) * p.a.natoms + c * kAtoms) * kF4Atom, sfb, full(s));
+                    left -= steps;
+                    const uint32_t sfb = (uint32_t)((kNv ? steps : (steps + 1) / 2) * kF4Atom);
+                    mbar_expect_tx(bar, (uint32_t)((128 + p.bn) * kCB) + sfb * (1 + rts));
+                    tma_load(dst, &tmb, c * kCB, jt * 128, bar);
+                    tma_load(dst + off_b, &tma, c * kCB, i0, bar);
+                    bulk_load(dst + off_sb, sb, sfb, bar);
+                    bulk_load(dst + off_sa, sa, sfb, bar);
+                    if (rts > 1)
+                        bulk_load(dst + off_sa + kAtoms * kF4Atom, sa + (long long)p.a.natoms * kF4Atom, sfb, bar);
+                    sb += kAtoms * kF4Atom;
+                    sa += kAtoms * kF4Atom;
+                    st.next(p.nstage);
                 }
             }
             // drain this thread's copies still in flight
             for (int i = step > p.nstage ? step - p.nstage : 0; i < step; ++i)
-                mbar_wait(full(i % p.nstage), (uint32_t)(i / p.nstage) & 1u, nullptr);
+                mbar_wait<false>(full(i % p.nstage), (uint32_t)(i / p.nstage) & 1u, nullptr);
         }
         __syncwarp();
     } else if (warp == 9) {
         if (lane == 0) {
-            int step = 0, n = 0;
+            RingPos st, ac;
+            int last = -1;
+            uint32_t last_parity = 0;
             bool ok = true;
             const uint32_t sfc = (uint32_t)(4 * kAtoms * (1 + nrt));  // TMEM columns of a stage's scales
-            for (int t = blockIdx.x; ok && t < ntiles; t += gridDim.x, ++n) {
-                const int b = n % p.nacc;
-                if (mbar_wait(acce(b), ((uint32_t)(n / p.nacc) & 1u) ^ 1u, abort) != kWaitOk) {
+            for (int t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
+                if (!mbar_wait_fast(acce(ac.slot), ac.parity ^ 1u, abort)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                const uint32_t d = tmem + (uint32_t)(b * p.acc_cols);
-                for (int c = 0; c < p.nchunk; ++c, ++step) {
-                    const int s = step % p.nstage;
-                    if (mbar_wait(full(s), (uint32_t)(step / p.nstage) & 1u, abort) != kWaitOk) {
+                const uint32_t d = tmem + (uint32_t)(ac.slot * p.acc_cols);
+                int left = p.b.Kp / 64;
+                for (int c = 0; c < p.nchunk; ++c) {
+                    if (!mbar_wait_fast(full(st.slot), st.parity, abort)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t st = stage0 + (uint32_t)(s * p.stage_bytes);
-                    const int left = (p.b.Kp - c * 2 * kCB) / 64;
+                    const uint32_t src = stage0 + (uint32_t)(st.slot * p.stage_bytes);
                     const int steps = min(left, kCB / 32);
+                    left -= steps;
                     const int atoms = kNv ? steps : (steps + 1) / 2;
-                    const uint32_t tsb = tmem + 256u + (uint32_t)s * sfc, tsa = tsb + 4 * kAtoms;
-                    for (int k = 0; k < atoms; ++k) {
-                        f4_copy_atom(tsb + 4 * k, f4_atom_desc(st + off_sb + k * kF4Atom));
-                        for (int r = 0; r < nrt; ++r)
-                            f4_copy_atom(tsa + 4 * (k * nrt + r), f4_atom_desc(st + off_sa + (r * kAtoms + k) * kF4Atom));
+                    const uint32_t tsb = tmem + 256u + (uint32_t)st.slot * sfc, tsa = tsb + 4 * kAtoms;
+                    const uint64_t db = f4_operand_desc<kCB>(src), da = f4_operand_desc<kCB>(src + off_b);
+                    const uint64_t dsb = f4_atom_desc(src + off_sb), dsa = f4_atom_desc(src + off_sa);
+#pragma unroll
+                    for (int k = 0; k < kAtoms; ++k) {
+                        if (k >= atoms) break;
+                        f4_copy_atom(tsb + 4 * k, dsb + k * (kF4Atom >> 4));
+                        f4_copy_atom(tsa + 4 * k * nrt, dsa + k * (kF4Atom >> 4));
+                        if (nrt > 1) f4_copy_atom(tsa + 8 * k + 4, dsa + (kAtoms + k) * (kF4Atom >> 4));
                     }
-                    const uint64_t db = f4_operand_desc<kCB>(st), da = f4_operand_desc<kCB>(st + off_b);
-                    for (int k = 0; k < steps; ++k) {
+#pragma unroll
+                    for (int k = 0; k < kCB / 32; ++k) {
+                        if (k >= steps) break;
                         const int at = kNv ? k : k >> 1;
                         f4_mma<kNv>(d, db + 2 * k, da + 2 * k, f4_idesc<kNv>(p.bn, kNv ? 0 : k & 1),
                                     tsb + 4 * at, tsa + 4 * nrt * at, (c | k) ? 1u : 0u);
                     }
-                    mma_commit(empty(s));
+                    mma_commit(empty(st.slot));
+                    last = st.slot;
+                    last_parity = st.parity;
+                    st.next(p.nstage);
                 }
-                if (ok) mma_commit(accf(b));
+                if (ok) mma_commit(accf(ac.slot));
+                ac.next(p.nacc);
             }
             if (!ok) {
                 if (!*abort) atomicExch(p.err, 2);
                 *abort = 1;
             }
             // the last products must finish before the accumulators are freed
-            if (step > 0) mbar_wait(empty((step - 1) % p.nstage), (uint32_t)((step - 1) / p.nstage) & 1u, nullptr);
+            if (last >= 0) mbar_wait<false>(empty(last), last_parity, nullptr);
         }
         __syncwarp();
     } else {
@@ -188,7 +203,8 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
 #pragma unroll
             for (int c = 0; c < 4; ++c) tmem_pin32(r[c]);
             tc_fence_before();
-            mbar_arrive(acce(b));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acce(b));
             const long long j = (long long)jt * 128 + jl;
             if (j < p.b.rows) {
                 T* o = out + (long long)(i0 + cb) * p.ld + j;

@@ -43,7 +43,6 @@ struct KeysArgs {
     int q0;               // first row tile of a in this batch
     int nq;               // row tiles of a in it
     int ntiles, noct;     // tiles of b, and groups of 8
-    int nstage, stage_bytes;
     uint32_t* keys;       // [rows of the batch][noct][16] pairs of keys
     float* errs;          // [grid] largest finite bound among the tiles of each block
     int* err;
@@ -72,6 +71,13 @@ __device__ __forceinline__ float key_floor(uint32_t key) {
     return __uint_as_float((u & 0x80000000u) ? u & 0x7FFFFFFFu : ~u);
 }
 
+// The ring of b's tiles, two to a stage; TMEM has room for three stages' scales at 128 bytes a row.
+constexpr int kAccs = 3;
+constexpr int keys_stages(int cb) { return cb == 32 ? 8 : 3; }
+constexpr int keys_stage(int nv, int cb) {
+    return (2 * (128 * cb + (cb == 32 ? 1 : nv ? 4 : 2) * kF4Atom) + 1023) / 1024 * 1024;
+}
+
 // A CTA takes the units [u0, u1) of (row tile of a, 8 tiles of b), b fastest.
 //   warps 0-7  quarter warp & 3 of the rows, half warp >> 2 of the columns of every accumulator;
 //   warp 8     one thread loads: the row tile of a into one of two slots, b's tiles into a ring;
@@ -87,6 +93,7 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
     constexpr int kAtoms = kCB == 32 ? 1 : (kNv ? 4 : 2);
     constexpr int kBox = 128 * kCB;
     constexpr int kSlot = kBox + 2048;
+    constexpr int kStages = keys_stages(kCB), kStage = keys_stage(kNv, kCB);  // two tiles of b each
     uint64_t* bars = (uint64_t*)sm;
     // full[16], empty[16], acc_full[3], acc_empty[3], a_full[2], a_empty[2]
     uint32_t* tmem_slot = (uint32_t*)(bars + 42);
@@ -106,13 +113,13 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
     const long long u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < p.nstage; ++s) {
+        for (int s = 0; s < kStages; ++s) {
             mbar_init(full(s), 1);
             mbar_init(empty(s), 1);
         }
-        for (int b = 0; b < 3; ++b) {
+        for (int b = 0; b < kAccs; ++b) {
             mbar_init(accf(b), 1);
-            mbar_init(acce(b), 256);
+            mbar_init(acce(b), 8);  // one arrival a warp
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(afull(b), 1);
@@ -139,32 +146,38 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
         if (lane == 0) {
             const uint32_t sfb = (uint32_t)(atoms * kF4Atom);
             int n = 0, na = 0;
+            RingPos st, sl;
             bool ok = true;
+            int qt = p.q0 + (int)(u0 / p.noct), oct = (int)(u0 % p.noct);
             for (long long u = u0; ok && u < u1; ++u) {
-                const int qt = p.q0 + (int)(u / p.noct), oct = (int)(u % p.noct);
                 if (u == u0 || oct == 0) {
-                    const int sl = na & 1;
-                    if (mbar_wait(aempty(sl), ((uint32_t)(na >> 1) & 1u) ^ 1u, abort) != kWaitOk) {
+                    if (!mbar_wait_fast(aempty(sl.slot), sl.parity ^ 1u, abort)) {
                         ok = false;
                         break;
                     }
-                    const uint32_t st = slot0 + (uint32_t)(sl * kSlot);
-                    mbar_expect_tx(afull(sl), (uint32_t)kBox + sfb);
-                    tma_load(st, &tma, 0, qt * 128, afull(sl));
-                    bulk_load(st + kBox, p.a.scales + (long long)qt * p.a.natoms * kF4Atom, sfb, afull(sl));
+                    const uint32_t dst = slot0 + (uint32_t)(sl.slot * kSlot);
+                    mbar_expect_tx(afull(sl.slot), (uint32_t)kBox + sfb);
+                    tma_load(dst, &tma, 0, qt * 128, afull(sl.slot));
+                    bulk_load(dst + kBox, p.a.scales + (long long)qt * p.a.natoms * kF4Atom, sfb, afull(sl.slot));
+                    sl.next(2);
                     ++na;
                 }
                 const int te = min(p.ntiles, oct * kOct + kOct);
-                for (int t = oct * kOct; t < te; ++t, ++n) {
-                    const int s = n % p.nstage;
-                    if (mbar_wait(empty(s), ((uint32_t)(n / p.nstage) & 1u) ^ 1u, abort) != kWaitOk) {
+                for (int t = oct * kOct; t < te; t += 2, ++n) {
+                    if (!mbar_wait_fast(empty(st.slot), st.parity ^ 1u, abort)) {
                         ok = false;
                         break;
                     }
-                    const uint32_t st = ring0 + (uint32_t)(s * p.stage_bytes);
-                    mbar_expect_tx(full(s), (uint32_t)kBox + sfb);
-                    tma_load(st, &tmb, 0, t * 128, full(s));
-                    bulk_load(st + kBox, p.b.scales + (long long)t * p.b.natoms * kF4Atom, sfb, full(s));
+                    const uint32_t dst = ring0 + (uint32_t)(st.slot * kStage);
+                    const uint32_t sc = t + 1 < te ? 2 * sfb : sfb;  // two tiles' scales follow one another
+                    mbar_expect_tx(full(st.slot), 2u * kBox + sc);
+                    tma_load(dst, &tmb, 0, t * 128, full(st.slot));
+                    bulk_load(dst + 2 * kBox, p.b.scales + (long long)t * p.b.natoms * kF4Atom, sc, full(st.slot));
+                    st.next(kStages);
+                }
+                if (++oct == p.noct) {
+                    oct = 0;
+                    ++qt;
                 }
             }
             if (!ok) {
@@ -172,73 +185,99 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
                 *abort = 1;
             }
             // drain this thread's copies still in flight
-            for (int i = na > 2 ? na - 2 : 0; i < na; ++i) mbar_wait(afull(i & 1), (uint32_t)(i >> 1) & 1u, nullptr);
-            for (int i = n > p.nstage ? n - p.nstage : 0; i < n; ++i)
-                mbar_wait(full(i % p.nstage), (uint32_t)(i / p.nstage) & 1u, nullptr);
+            for (int i = na > 2 ? na - 2 : 0; i < na; ++i) mbar_wait<false>(afull(i & 1), (uint32_t)(i >> 1) & 1u, nullptr);
+            for (int i = n > kStages ? n - kStages : 0; i < n; ++i)
+                mbar_wait<false>(full(i % kStages), (uint32_t)(i / kStages) & 1u, nullptr);
         }
         __syncwarp();
     } else if (warp == 9) {
         if (lane == 0) {
-            int n = 0, na = 0;
+            RingPos st, sl, ac;
+            int last = -1;
+            uint32_t last_parity = 0;
             bool ok = true;
             uint32_t tsa = 0;
             uint64_t da = 0;
+            int oct = (int)(u0 % p.noct);
             for (long long u = u0; ok && u < u1; ++u) {
-                const int oct = (int)(u % p.noct);
                 if (u == u0 || oct == 0) {
-                    const int sl = na & 1;
-                    if (mbar_wait(afull(sl), (uint32_t)(na >> 1) & 1u, abort) != kWaitOk) {
+                    if (!mbar_wait_fast(afull(sl.slot), sl.parity, abort)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t st = slot0 + (uint32_t)(sl * kSlot);
-                    tsa = tmem + 384u + (uint32_t)(16 * sl);
-                    for (int k0 = 0; k0 < atoms; ++k0) f4_copy_atom(tsa + 4 * k0, f4_atom_desc(st + kBox + k0 * kF4Atom));
-                    da = f4_operand_desc<kCB>(st);
-                    ++na;
+                    const uint32_t src = slot0 + (uint32_t)(sl.slot * kSlot);
+                    tsa = tmem + 384u + (uint32_t)(4 * kAtoms * sl.slot);
+                    for (int k0 = 0; k0 < atoms; ++k0) f4_copy_atom(tsa + 4 * k0, f4_atom_desc(src + kBox + k0 * kF4Atom));
+                    da = f4_operand_desc<kCB>(src);
                 }
                 const int te = min(p.ntiles, oct * kOct + kOct);
-                for (int t = oct * kOct; t < te; ++t) {
-                    const int s = n % p.nstage, b = n % 3;
-                    if (mbar_wait(acce(b), ((uint32_t)(n / 3) & 1u) ^ 1u, abort) != kWaitOk ||
-                        mbar_wait(full(s), (uint32_t)(n / p.nstage) & 1u, abort) != kWaitOk) {
+                for (int t = oct * kOct; ok && t < te; t += 2) {
+                    if (!mbar_wait_fast(full(st.slot), st.parity, abort)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t st = ring0 + (uint32_t)(s * p.stage_bytes);
-                    const uint32_t tsb = tmem + 416u + (uint32_t)(s * 4 * kAtoms);
-                    for (int k0 = 0; k0 < atoms; ++k0) f4_copy_atom(tsb + 4 * k0, f4_atom_desc(st + kBox + k0 * kF4Atom));
-                    const uint64_t db = f4_operand_desc<kCB>(st);
-                    for (int k0 = 0; k0 < steps; ++k0) {
-                        const int at = kNv ? k0 : k0 >> 1;
-                        f4_mma<kNv>(tmem + (uint32_t)(128 * b), da + 2 * k0, db + 2 * k0,
-                                    f4_idesc<kNv>(128, kNv ? 0 : k0 & 1), tsa + 4 * at, tsb + 4 * at, k0 ? 1u : 0u);
+                    const uint32_t src = ring0 + (uint32_t)(st.slot * kStage);
+                    const uint32_t tsb = tmem + 384u + (uint32_t)(8 * kAtoms * (1 + st.slot));
+                    const int nt = min(2, te - t);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (h == nt) break;
+                        const uint32_t tsh = tsb + 4 * kAtoms * h;
+                        const uint64_t dsc = f4_atom_desc(src + 2 * kBox + h * atoms * kF4Atom);
+                        const uint64_t db = f4_operand_desc<kCB>(src + h * kBox);
+                        if (kCB == 32) {
+                            f4_copy_atom(tsh, dsc);
+                        } else {
+                            for (int k0 = 0; k0 < atoms; ++k0) f4_copy_atom(tsh + 4 * k0, dsc + k0 * (kF4Atom >> 4));
+                        }
+                        if (!mbar_wait_fast(acce(ac.slot), ac.parity ^ 1u, abort)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t d = tmem + (uint32_t)(128 * ac.slot);
+                        if (kCB == 32) {
+                            f4_mma<kNv>(d, da, db, f4_idesc<kNv>(128, 0), tsa, tsh, 0u);
+                        } else {
+                            for (int k0 = 0; k0 < steps; ++k0) {
+                                const int at = kNv ? k0 : k0 >> 1;
+                                f4_mma<kNv>(d, da + 2 * k0, db + 2 * k0, f4_idesc<kNv>(128, kNv ? 0 : k0 & 1),
+                                            tsa + 4 * at, tsh + 4 * at, k0 ? 1u : 0u);
+                            }
+                        }
+                        mma_commit(accf(ac.slot));
+                        last = ac.slot;
+                        last_parity = ac.parity;
+                        ac.next(kAccs);
                     }
-                    mma_commit(empty(s));
-                    mma_commit(accf(b));
-                    ++n;
+                    if (ok) mma_commit(empty(st.slot));
+                    st.next(kStages);
                 }
-                if (ok && (oct == p.noct - 1 || u == u1 - 1)) mma_commit(aempty((na - 1) & 1));
+                if (++oct == p.noct) oct = 0;
+                if (ok && (oct == 0 || u == u1 - 1)) {
+                    mma_commit(aempty(sl.slot));
+                    sl.next(2);
+                }
             }
             if (!ok) {
                 if (!*abort) atomicExch(p.err, 2);
                 *abort = 1;
             }
             // the last products must finish before the accumulators are freed
-            if (n > 0) mbar_wait(accf((n - 1) % 3), (uint32_t)((n - 1) / 3) & 1u, nullptr);
+            if (last >= 0) mbar_wait<false>(accf(last), last_parity, nullptr);
         }
         __syncwarp();
     } else {
         const int half = warp >> 2, quarter = warp & 3;
-        const uint32_t lane_addr = ((uint32_t)(32 * quarter) << 16) + (uint32_t)(64 * half);
+        const uint32_t lane_addr = tmem + ((uint32_t)(32 * quarter) << 16) + (uint32_t)(64 * half);
         const float kNegInf = -__int_as_float(0x7f800000);
         float worst = 0.0f;  // largest bound of this block's tiles that the filter can use
-        int n = 0;
+        RingPos ac;
         bool ok = true;
+        int qt = p.q0 + (int)(u0 / p.noct), oct = (int)(u0 % p.noct);
         for (long long u = u0; ok && u < u1; ++u) {
-            const int qt = p.q0 + (int)(u / p.noct), oct = (int)(u % p.noct);
             const long long row = (long long)qt * 128 + 32 * quarter + lane;
             const bool any = (long long)qt * 128 + 32 * quarter < p.a.rows;  // of this warp's rows
             const float bq = __ldg(p.a.bounds + qt);
@@ -247,50 +286,61 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
             // a sum of such terms can overflow fp32 and lose its sign: those tiles are looked at
             const uint32_t forced = __ballot_sync(0xFFFFFFFFu, !(bq * bd * kEps < 1e30f));
             if (!((forced >> lane) & 1u)) worst = fmaxf(worst, bq * bd * (kEps * 1.000001f));
+            const int ncols = min(kOct * 128, p.b.rows - oct * kOct * 128) - 64 * half;  // columns that exist
             uint32_t keys[kOct];
+            uint32_t r[2][2][32];
+            // accumulator i is read while the maxima of i - 1 are taken
+            auto fetch = [&](int i) {
+                const bool got = mbar_wait_fast(accf(ac.slot), ac.parity, abort);
+                if (!__all_sync(0xFFFFFFFFu, got)) {
+                    ok = false;
+                    return;
+                }
+                tc_fence_after();
+                if (any) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) tmem_ld32_issue(lane_addr + (uint32_t)(128 * ac.slot + 32 * c), r[i & 1][c]);
+                }
+            };
+            fetch(0);
 #pragma unroll
             for (int i = 0; i < kOct; ++i) {
                 keys[i] = 0;
                 if (i >= nt || !ok) continue;
-                const int b = n % 3;
-                const int w = mbar_wait<false>(accf(b), (uint32_t)(n / 3) & 1u, abort);
-                ++n;
-                if (__any_sync(0xFFFFFFFFu, w != kWaitOk)) {
-                    ok = false;
-                    continue;
-                }
-                tc_fence_after();
-                if (!any) {
+                if (any) {
+                    tmem_wait();
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) tmem_pin32(r[i & 1][c]);
                     tc_fence_before();
-                    mbar_arrive(acce(b));
-                    continue;
                 }
-                uint32_t r[2][32];
-#pragma unroll
-                for (int c = 0; c < 2; ++c) tmem_ld32_issue(tmem + lane_addr + (uint32_t)(128 * b + 32 * c), r[c]);
-                tmem_wait();
-#pragma unroll
-                for (int c = 0; c < 2; ++c) tmem_pin32(r[c]);
-                tc_fence_before();
-                mbar_arrive(acce(b));
-                const int ncol = p.b.rows - (oct * kOct + i) * 128 - 64 * half;  // columns that exist
+                __syncwarp();
+                if (lane == 0) mbar_arrive(acce(ac.slot));
+                ac.next(kAccs);
+                if (i + 1 < nt) fetch(i + 1);
+                if (!any) continue;
+                const int ncol = ncols - 128 * i;
                 uint32_t pair = 0;
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
+                    uint32_t* x = r[i & 1][c];
                     if (ncol < 64) {
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
-                            if (32 * c + e >= ncol) r[c][e] = __float_as_uint(kNegInf);
+                            if (32 * c + e >= ncol) x[e] = __float_as_uint(kNegInf);
                     }
-                    float m0 = __uint_as_float(r[c][0]), m1 = __uint_as_float(r[c][1]);
+                    float m[4];
 #pragma unroll
-                    for (int e = 2; e < 30; e += 4) {
-                        m0 = fmax3(m0, __uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1]));
-                        m1 = fmax3(m1, __uint_as_float(r[c][e + 2]), __uint_as_float(r[c][e + 3]));
+                    for (int e = 0; e < 4; ++e) m[e] = __uint_as_float(x[e]);
+#pragma unroll
+                    for (int e = 4; e < 28; e += 8) {
+#pragma unroll
+                        for (int f = 0; f < 4; ++f)
+                            m[f] = fmax3(m[f], __uint_as_float(x[e + 2 * f]), __uint_as_float(x[e + 2 * f + 1]));
                     }
-                    m0 = fmax3(m0, __uint_as_float(r[c][30]), __uint_as_float(r[c][31]));
-                    m0 = fmaxf(m0, m1);
-                    uint32_t key = m0 == m0 ? key_of(m0) : 0u;  // NaN alone: nobody's neighbours
+                    m[0] = fmax3(m[0], __uint_as_float(x[28]), __uint_as_float(x[29]));
+                    m[1] = fmax3(m[1], __uint_as_float(x[30]), __uint_as_float(x[31]));
+                    const float top = fmaxf(fmax3(m[0], m[1], m[2]), m[3]);
+                    uint32_t key = top == top ? key_of(top) : 0u;  // NaN alone: nobody's neighbours
                     if ((forced >> i) & 1u) key = kAlways;
                     if (ncol <= 32 * c) key = 0;
                     pair |= key << (16 * c);
@@ -302,6 +352,10 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
                     p.keys + ((row - (long long)p.q0 * 128) * p.noct + oct) * (kOctKeys / 2) + 8 * half);
                 o[0] = make_uint4(keys[0], keys[1], keys[2], keys[3]);
                 o[1] = make_uint4(keys[4], keys[5], keys[6], keys[7]);
+            }
+            if (++oct == p.noct) {
+                oct = 0;
+                ++qt;
             }
         }
         if (!ok && lane == 0) {
@@ -544,10 +598,7 @@ TopkPlan topk_plan(const F4& a, const F4& b) {
 
 template <int kNv, int kCB>
 cudaError_t launch_keys(const CUtensorMap& ta, const CUtensorMap& tb, KeysArgs& p, int grid, cudaStream_t st) {
-    constexpr int kAtoms = kCB == 32 ? 1 : (kNv ? 4 : 2);
-    p.stage_bytes = (128 * kCB + kAtoms * kF4Atom + 1023) / 1024 * 1024;
-    p.nstage = kCB == 32 ? 16 : 6;
-    const int smem = 1024 + 1024 + 2 * (128 * kCB + 2048) + p.nstage * p.stage_bytes;
+    const int smem = 1024 + 1024 + 2 * (128 * kCB + 2048) + keys_stages(kCB) * keys_stage(kNv, kCB);
     auto f = k_f4_keys<kNv, kCB>;
     cudaError_t e = cudaFuncSetAttribute((const void*)f, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
@@ -573,7 +624,7 @@ cudaError_t f4_topk(const F4& a, const F4& b, int k, long long self, int* idx, f
     const TopkPlan plan = topk_plan(a, b);
     const int cb = b.Kp == 64 ? 32 : 128;
     CUtensorMap ta, tb;
-    if (!f4_map(&ta, a, 128, cb) || !f4_map(&tb, b, 128, cb)) return cudaErrorInvalidValue;
+    if (!f4_map(&ta, a, 128, cb) || !f4_map(&tb, b, 256, cb)) return cudaErrorInvalidValue;
     KeysArgs p;
     p.a = a;
     p.b = b;

@@ -55,15 +55,40 @@ template <bool kSleep = true>
 __device__ int mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort,
                          unsigned long long* polls = nullptr, volatile int* limit = nullptr,
                          int it = 0) {
-    const unsigned long long t0 = now_ns();
+    unsigned long long t0 = 0;  // read at the 16th poll: most waits end before it
     for (uint32_t spin = 1;; ++spin) {
         if (polls) ++*polls;
         if (mbar_try<kSleep>(bar, parity)) return kWaitOk;
         if (limit && it >= *limit) return kWaitStop;
         if (abort && *abort) return kWaitFail;
-        if ((spin & 15u) == 0 && now_ns() - t0 > kWaitNs) return kWaitFail;
+        if ((spin & 15u) == 0) {
+            const unsigned long long t = now_ns();
+            if (t0 == 0) t0 = t;
+            else if (t - t0 > kWaitNs) return kWaitFail;
+        }
     }
 }
+
+// mbar_wait for the roles that may not lose cycles: one inlined poll, the bounded loop behind it.
+// True when the phase has completed.
+__device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort) {
+    return mbar_wait<false>(bar, parity, abort) == kWaitOk;
+}
+__device__ __forceinline__ bool mbar_wait_fast(uint32_t bar, uint32_t parity, volatile int* abort) {
+    return mbar_try<false>(bar, parity) || mbar_wait_slow(bar, parity, abort);
+}
+
+// A position in a ring of n slots: its slot and the parity of the round.
+struct RingPos {
+    int slot = 0;
+    uint32_t parity = 0;
+    __device__ __forceinline__ void next(int n) {
+        if (++slot == n) {
+            slot = 0;
+            parity ^= 1u;
+        }
+    }
+};
 
 // mbar_wait that also adds the cycles it spent to *cyc.
 template <bool kSleep = true>
