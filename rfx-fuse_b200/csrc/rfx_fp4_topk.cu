@@ -29,7 +29,7 @@ namespace rfx {
 
 namespace {
 
-constexpr int kKThreads = 320;
+constexpr int kKThreads = 576;
 constexpr int kPickThreads = 512;
 constexpr int kOct = 8;                      // tiles of b whose keys a lane keeps before it stores them
 constexpr int kOctKeys = 4 * kOct;           // keys of a row and 8 tiles
@@ -79,9 +79,10 @@ constexpr int keys_stage(int nv, int cb) {
 }
 
 // A CTA takes the units [u0, u1) of (row tile of a, 8 tiles of b), b fastest.
-//   warps 0-7  quarter warp & 3 of the rows, half warp >> 2 of the columns of every accumulator;
-//   warp 8     one thread loads: the row tile of a into one of two slots, b's tiles into a ring;
-//   warp 9     allocates TMEM, one thread copies scales to TMEM and multiplies into three
+//   warps 0-15 quarter warp & 3 of the rows, half warp >> 2 & 1 of the columns, every other tile
+//              (four warps a scheduler: with two, 0.36 instructions a cycle issued);
+//   warp 16    one thread loads: the row tile of a into one of two slots, b's tiles into a ring;
+//   warp 17    allocates TMEM, one thread copies scales to TMEM and multiplies into three
 //              accumulators of 128 columns.
 // Every wait is bounded; on expiry the CTA records it in *err, drains its copies, frees TMEM and
 // returns.
@@ -128,7 +129,7 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
         *abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 9) {
+    if (warp == 17) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                          smem_u32(tmem_slot)),
                      "r"(512)
@@ -142,7 +143,7 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
     const int steps = p.b.Kp / 64;
     const int atoms = kNv ? steps : (steps + 1) / 2;
 
-    if (warp == 8) {
+    if (warp == 16) {
         if (lane == 0) {
             const uint32_t sfb = (uint32_t)(atoms * kF4Atom);
             int n = 0, na = 0;
@@ -190,7 +191,7 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
                 mbar_wait<false>(full(i % kStages), (uint32_t)(i / kStages) & 1u, nullptr);
         }
         __syncwarp();
-    } else if (warp == 9) {
+    } else if (warp == 17) {
         if (lane == 0) {
             RingPos st, sl, ac;
             int last = -1;
@@ -270,59 +271,65 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
         }
         __syncwarp();
     } else {
-        const int half = warp >> 2, quarter = warp & 3;
+        const int quarter = warp & 3, half = (warp >> 2) & 1, par = warp >> 3;
         const uint32_t lane_addr = tmem + ((uint32_t)(32 * quarter) << 16) + (uint32_t)(64 * half);
         const float kNegInf = -__int_as_float(0x7f800000);
         float worst = 0.0f;  // largest bound of this block's tiles that the filter can use
-        RingPos ac;
+        uint32_t n = (uint32_t)par;  // this warp's next tile in the CTA's sequence
         bool ok = true;
         int qt = p.q0 + (int)(u0 / p.noct), oct = (int)(u0 % p.noct);
+        float bd = lane < min(kOct, p.ntiles - oct * kOct) ? __ldg(p.b.bounds + oct * kOct + lane) : 0.0f;
+        float bq = u0 < u1 ? __ldg(p.a.bounds + qt) : 0.0f;
         for (long long u = u0; ok && u < u1; ++u) {
             const long long row = (long long)qt * 128 + 32 * quarter + lane;
             const bool any = (long long)qt * 128 + 32 * quarter < p.a.rows;  // of this warp's rows
-            const float bq = __ldg(p.a.bounds + qt);
             const int nt = min(kOct, p.ntiles - oct * kOct);
-            const float bd = lane < nt ? __ldg(p.b.bounds + oct * kOct + lane) : 0.0f;
             // a sum of such terms can overflow fp32 and lose its sign: those tiles are looked at
             const uint32_t forced = __ballot_sync(0xFFFFFFFFu, !(bq * bd * kEps < 1e30f));
             if (!((forced >> lane) & 1u)) worst = fmaxf(worst, bq * bd * (kEps * 1.000001f));
             const int ncols = min(kOct * 128, p.b.rows - oct * kOct * 128) - 64 * half;  // columns that exist
-            uint32_t keys[kOct];
-            uint32_t r[2][2][32];
-            // accumulator i is read while the maxima of i - 1 are taken
-            auto fetch = [&](int i) {
-                const bool got = mbar_wait_fast(accf(ac.slot), ac.parity, abort);
+            uint32_t* out = p.keys + ((row - (long long)p.q0 * 128) * p.noct + oct) * (kOctKeys / 2) + 8 * half + 4 * par;
+            // the next unit's bounds, under this one's work
+            int oct1 = oct + 1, qt1 = qt;
+            if (oct1 == p.noct) {
+                oct1 = 0;
+                ++qt1;
+            }
+            if (u + 1 < u1) {
+                bd = lane < min(kOct, p.ntiles - oct1 * kOct) ? __ldg(p.b.bounds + oct1 * kOct + lane) : 0.0f;
+                bq = __ldg(p.a.bounds + qt1);
+            }
+            uint32_t keys[kOct / 2];
+#pragma unroll
+            for (int i = 0; i < kOct / 2; ++i) {
+                keys[i] = 0;
+                const int t = 2 * i + par;
+                if (t >= nt || !ok) continue;
+                const uint32_t slot = n % kAccs;
+                const bool got = mbar_wait_fast(accf(slot), (n / kAccs) & 1u, abort);
+                n += 2;
                 if (!__all_sync(0xFFFFFFFFu, got)) {
                     ok = false;
-                    return;
+                    continue;
                 }
-                tc_fence_after();
+                uint32_t r[2][32];
                 if (any) {
+                    tc_fence_after();
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) tmem_ld32_issue(lane_addr + (uint32_t)(128 * ac.slot + 32 * c), r[i & 1][c]);
-                }
-            };
-            fetch(0);
-#pragma unroll
-            for (int i = 0; i < kOct; ++i) {
-                keys[i] = 0;
-                if (i >= nt || !ok) continue;
-                if (any) {
+                    for (int c = 0; c < 2; ++c) tmem_ld32_issue(lane_addr + 128 * slot + 32 * c, r[c]);
                     tmem_wait();
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) tmem_pin32(r[i & 1][c]);
+                    for (int c = 0; c < 2; ++c) tmem_pin32(r[c]);
                     tc_fence_before();
+                    __syncwarp();
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(acce(ac.slot));
-                ac.next(kAccs);
-                if (i + 1 < nt) fetch(i + 1);
+                if (lane == 0) mbar_arrive(acce(slot));
                 if (!any) continue;
-                const int ncol = ncols - 128 * i;
+                const int ncol = ncols - 128 * t;
                 uint32_t pair = 0;
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    uint32_t* x = r[i & 1][c];
+                    uint32_t* x = r[c];
                     if (ncol < 64) {
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
@@ -341,22 +348,16 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
                     m[1] = fmax3(m[1], __uint_as_float(x[30]), __uint_as_float(x[31]));
                     const float top = fmaxf(fmax3(m[0], m[1], m[2]), m[3]);
                     uint32_t key = top == top ? key_of(top) : 0u;  // NaN alone: nobody's neighbours
-                    if ((forced >> i) & 1u) key = kAlways;
+                    if ((forced >> t) & 1u) key = kAlways;
                     if (ncol <= 32 * c) key = 0;
                     pair |= key << (16 * c);
                 }
                 keys[i] = pair;
             }
-            if (ok && row < p.a.rows) {
-                uint4* o = reinterpret_cast<uint4*>(
-                    p.keys + ((row - (long long)p.q0 * 128) * p.noct + oct) * (kOctKeys / 2) + 8 * half);
-                o[0] = make_uint4(keys[0], keys[1], keys[2], keys[3]);
-                o[1] = make_uint4(keys[4], keys[5], keys[6], keys[7]);
-            }
-            if (++oct == p.noct) {
-                oct = 0;
-                ++qt;
-            }
+            if (ok && row < p.a.rows) *reinterpret_cast<uint4*>(out) = make_uint4(keys[0], keys[1], keys[2], keys[3]);
+            n += (uint32_t)nt - 2u * (uint32_t)((nt - par + 1) / 2);  // to its first tile of the next unit
+            oct = oct1;
+            qt = qt1;
         }
         if (!ok && lane == 0) {
             if (!*abort) atomicExch(p.err, 3);
@@ -369,7 +370,7 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == 17) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512)
                      : "memory");
@@ -548,13 +549,13 @@ k_f4_pick(PickArgs p) {
         if (t < nvec) {
             const uint4 x = __ldg(keys + t);
             const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-            // keys 8 t ..: 8 tiles of b, of each 2 halves of 64 columns: [oct][half][tile][2]
-            const int oct = t >> 2, half = (t >> 1) & 1, tile = 4 * (t & 1);
+            // keys 8 t ..: [8 tiles of b][half of 64 columns][parity of the tile][4 tiles][2]
+            const int oct = t >> 2, half = (t >> 1) & 1, par = t & 1;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const uint32_t key = (w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
                 if (key >= bar && key > 0) {
-                    const int chunk = ((oct * kOct + tile + (e >> 1)) * 4) + 2 * half + (e & 1);
+                    const int chunk = (oct * kOct + 2 * (e >> 1) + par) * 4 + 2 * half + (e & 1);
                     list[atomicAdd(&n_list, 1)] = (uint32_t)chunk;
                 }
             }
