@@ -11,8 +11,8 @@
 //   k_f4_keys  products of 128 rows of a with b's tiles of 128 rows (tcgen05, block-scaled); of
 //              every row's 32 neighbouring accumulators only the maximum is kept, as the upper 16
 //              bits of its order-preserving integer (rounded down).
-//   k_f4_pick  a block per row of a.  512 threads take the largest key of every 512th; the k-th
-//              largest of those 512, L, is a lower bound of the k-th largest key: there are k
+//   k_f4_pick  a block per row of a.  The keys form up to 1024 groups; the k-th largest of the
+//              groups' largest keys, L, is a lower bound of the k-th largest key: there are k
 //              columns with accumulators of L or more, so the k-th value is at least L - err, and
 //              a column of the answer has an accumulator of at least L - 2 err.  Only chunks whose
 //              key reaches that (about k of them) are evaluated, all 32 columns exactly, and
@@ -30,12 +30,13 @@ namespace rfx {
 namespace {
 
 constexpr int kKThreads = 576;
-constexpr int kPickThreads = 512;
+constexpr int kPickThreads = 256;
+constexpr int kGroups = 1024;                // groups of keys whose largest ones bound the k-th value
 constexpr int kOct = 8;                      // tiles of b whose keys a lane keeps before it stores them
 constexpr int kOctKeys = 4 * kOct;           // keys of a row and 8 tiles
 constexpr float kEps = 1.0f / 32768.0f;
 constexpr uint32_t kAlways = 0xFFFFu;        // key of a chunk that has to be looked at (no float's)
-constexpr int kList = 8 * kPickThreads + 512; // chunks waiting for their evaluation
+constexpr int kList = 8 * kPickThreads + 256; // chunks waiting for their evaluation
 constexpr int kFound = 1024;                 // values waiting to be ranked
 
 struct KeysArgs {
@@ -53,7 +54,7 @@ struct PickArgs {
     int row0;             // first row of the batch
     int k;
     long long self;       // row of b that is row 0 of a and left out for it (and so on); -1: none
-    int noct;
+    int noct, gshift;     // 2^gshift vectors of 8 keys are a group
     const uint32_t* keys;
     const float* errs;
     int nerrs;
@@ -425,21 +426,28 @@ __device__ double f4_exact(const int* qa, const double* sa, const F4& b, long lo
 }
 
 template <int kNv>
-__global__ void __launch_bounds__(kPickThreads)
+__global__ void __launch_bounds__(kPickThreads, 5)
 k_f4_pick(PickArgs p) {
     __shared__ int qa[kF4TopkK / 4];
     __shared__ double sa[kF4TopkK / 16];
-    __shared__ uint32_t list[kList];
-    __shared__ double fv[kFound];
+    __shared__ double fv[kFound];       // found: values (4 x), columns
     __shared__ int fj[kFound];
-    __shared__ uint32_t tops[kPickThreads];
-    __shared__ int n_list, n_found, n_keep;
-    __shared__ double s_floor;
+    __shared__ uint32_t list[kList];    // chunks to evaluate
+    __shared__ uint32_t tops[kGroups];  // a group's largest key; kVisit: it holds a chunk to look at
+    __shared__ uint16_t glist[kGroups]; // groups to look at
+    __shared__ int n_list, n_found, n_groups;
+    __shared__ uint32_t s_key;
     __shared__ float s_err;
+    constexpr uint32_t kVisit = 0x10000u;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const long long i = (long long)p.row0 + blockIdx.x;
     const int kp = p.self >= 0 ? p.k + 1 : p.k;  // the row itself may be one of the k columns
     const long long self = p.self >= 0 ? p.self + i : -1;
+    const uint4* keys = reinterpret_cast<const uint4*>(p.keys + (long long)blockIdx.x * p.noct * (kOctKeys / 2));
+    const int nvec = p.noct * (kOctKeys / 8);    // 8 keys each
+    const bool single = nvec * 8 <= kGroups;     // a key is a group of its own
+    const int gs = single ? 0 : p.gshift;        // else 2^gs vectors are
+    const int ngroups = single ? nvec * 8 : ((nvec - 1) >> gs) + 1;
 
     // the row, decoded, and its scales
     for (int t = tid; t < p.a.Kp / 4; t += kPickThreads) {
@@ -457,35 +465,77 @@ k_f4_pick(PickArgs p) {
         for (int o = 16; o; o >>= 1) e = fmaxf(e, __shfl_xor_sync(0xFFFFFFFFu, e, o));
         if (lane == 0) {
             s_err = fmaxf(e, 1e-37f);
-            n_list = n_found = n_keep = 0;
+            n_list = n_found = n_groups = 0;
         }
     }
-    // the largest key of every thread's share; L is the kp-th largest of those
-    const uint4* keys = reinterpret_cast<const uint4*>(p.keys + (long long)blockIdx.x * p.noct * (kOctKeys / 2));
-    const int nvec = p.noct * (kOctKeys / 8);  // 8 keys each
-    uint32_t best = 0;
-    for (int t = tid; t < nvec; t += kPickThreads) {
-        const uint4 x = __ldg(keys + t);
+    if (gs > 5) {
+        for (int t = tid; t < ngroups; t += kPickThreads) tops[t] = 0;
+        __syncthreads();
+    }
+    // the largest key of every group
+    for (int t0 = 0; t0 < nvec; t0 += kPickThreads) {
+        const int t = t0 + tid;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (t < nvec) x = __ldg(keys + t);
         const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        if (single) {
+            if (t < nvec) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const uint32_t lo = w[e] & 0xFFFFu, hi = w[e] >> 16;
-            if (lo != kAlways) best = max(best, lo);
-            if (hi != kAlways) best = max(best, hi);
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t key = (w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
+                    tops[8 * t + e] = key == kAlways ? kVisit : key;
+                }
+            }
+            continue;
+        }
+        uint32_t best = 0, visit = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t key = (w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
+            if (key == kAlways) visit = kVisit;
+            else best = max(best, key);
+        }
+        for (int o = 1; o < 32 && o < (1 << gs); o <<= 1) {
+            best = max(best, __shfl_xor_sync(0xFFFFFFFFu, best, o));
+            visit |= __shfl_xor_sync(0xFFFFFFFFu, visit, o);
+        }
+        if (gs <= 5) {
+            if (t < nvec && (t & ((1 << gs) - 1)) == 0) tops[t >> gs] = best | visit;
+        } else if (lane == 0 && t < nvec) {
+            atomicMax(&tops[t >> gs], best);  // visit goes in after the maximum
+            if (visit) atomicOr(&n_groups, 0x40000000);
         }
     }
-    tops[tid] = best;
-    if (tid == 0) s_floor = -__longlong_as_double(0x7ff0000000000000ll);
     __syncthreads();
-    int rank = 0;
-    for (int t = 0; t < kPickThreads; ++t) {
-        const uint32_t o = tops[t];
-        rank += o > best || (o == best && t < tid);
+    // L: the kp-th largest of them, by bisection of its 16 bits (0: there are fewer)
+    if (warp == 0) {
+        uint32_t v[kGroups / 32];
+#pragma unroll
+        for (int e = 0; e < kGroups / 32; ++e) v[e] = lane + 32 * e < ngroups ? tops[lane + 32 * e] & 0xFFFFu : 0u;
+        uint32_t key = 0;
+        for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
+            const uint32_t mid = key | bit;
+            int c = 0;
+#pragma unroll
+            for (int e = 0; e < kGroups / 32; ++e) c += v[e] >= mid;
+            if (__reduce_add_sync(0xFFFFFFFFu, c) >= kp) key = mid;
+        }
+        if (lane == 0) s_key = key;
     }
-    // key 0 holds nothing, or only what no float reaches
-    if (rank == kp - 1 && best > 0) s_floor = (double)key_floor(best) - (double)s_err;
     __syncthreads();
-    double floor_v = s_floor;  // the k-th value is at least this
+    const double err = (double)s_err;
+    const bool everything = (n_groups & 0x40000000) != 0;  // some group of more than 32 vectors is to be looked at
+    // the k-th value is at least this
+    double floor_v = s_key > key_of(-__int_as_float(0x7f800000)) ? (double)key_floor(s_key) - err : -__longlong_as_double(0x7ff0000000000000ll);
+    __syncthreads();
+    if (tid == 0) n_groups = 0;
+    __syncthreads();
+    // an accumulator of the answer is at least floor - err
+    auto bar_of = [&]() { return key_of(__double2float_rd(floor_v - err)); };
+    const uint32_t bar0 = bar_of();
+    for (int t = tid; t < ngroups; t += kPickThreads)
+        if (everything || tops[t] >= max(bar0, 1u)) glist[atomicAdd(&n_groups, 1)] = (uint16_t)t;
+    __syncthreads();
 
     // Ranks what was found, keeps the best k at the front and raises the floor.
     auto rank_found = [&]() {
@@ -516,16 +566,15 @@ k_f4_pick(PickArgs p) {
         if (n_found == p.k) floor_v = fmax(floor_v, 0.25 * fv[p.k - 1]);
         __syncthreads();
     };
-    // Evaluates the chunks of the list; a warp takes a chunk, a lane a column.
+    // Evaluates the chunks of the list, a lane a column, as many at a time as surely have room.
     auto evaluate = [&]() {
         __syncthreads();
         const int n = n_list;
-        for (int c0 = 0; c0 < n; c0 += kPickThreads / 32) {
-            const bool room = n_found <= kFound - kPickThreads;
+        for (int c0 = 0; c0 < n;) {
+            const int room = (kFound - n_found) / 32;
             __syncthreads();  // everyone has read n_found before anyone adds to it
-            if (!room) rank_found();
-            const int c = c0 + warp;
-            if (c < n) {
+            const int c1 = min(n, c0 + room);
+            for (int c = c0 + warp; c < c1; c += kPickThreads / 32) {
                 const long long j = (long long)list[c] * 32 + lane;
                 if (j < p.b.rows && j != self) {
                     const double v = f4_exact<kNv>(qa, sa, p.b, j);
@@ -536,33 +585,40 @@ k_f4_pick(PickArgs p) {
                     }
                 }
             }
+            c0 = c1;
+            if (c0 < n) rank_found();
             __syncthreads();
         }
         if (tid == 0) n_list = 0;
         __syncthreads();
     };
-    // chunks that may hold a column of the answer
-    for (int t0 = 0; t0 < nvec; t0 += kPickThreads) {
-        // an accumulator of the answer is at least floor - err
-        const uint32_t bar = key_of(__double2float_rd(floor_v - (double)s_err));
-        const int t = t0 + tid;
-        if (t < nvec) {
-            const uint4 x = __ldg(keys + t);
-            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-            // keys 8 t ..: [8 tiles of b][half of 64 columns][parity of the tile][4 tiles][2]
-            const int oct = t >> 2, half = (t >> 1) & 1, par = t & 1;
+    // the groups' chunks that may hold a column of the answer
+    const int ng = n_groups;
+    const long long ntask = (long long)ng << gs;  // a vector (a key when single) each
+    for (long long t0 = 0; t0 < ntask; t0 += kPickThreads) {
+        const uint32_t bar = max(bar_of(), 1u);
+        const long long t = t0 + tid;
+        if (t < ntask) {
+            const long long g = glist[t >> gs];
+            const long long vec = single ? g >> 3 : (g << gs) + (t & ((1 << gs) - 1));
+            if (vec < nvec) {
+                const uint4 x = __ldg(keys + vec);
+                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+                // keys 8 vec ..: [8 tiles of b][half of 64 columns][parity of the tile][4 tiles][2]
+                const int oct = (int)(vec >> 2), half = (int)(vec >> 1) & 1, par = (int)vec & 1;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t key = (w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
-                if (key >= bar && key > 0) {
-                    const int chunk = (oct * kOct + 2 * (e >> 1) + par) * 4 + 2 * half + (e & 1);
-                    list[atomicAdd(&n_list, 1)] = (uint32_t)chunk;
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t key = (w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
+                    if (key >= bar && (!single || e == (int)(g & 7))) {
+                        const int chunk = (oct * kOct + 2 * (e >> 1) + par) * 4 + 2 * half + (e & 1);
+                        list[atomicAdd(&n_list, 1)] = (uint32_t)chunk;
+                    }
                 }
             }
         }
         __syncthreads();
         const bool room = n_list <= kList - 8 * kPickThreads;
-        __syncthreads();
+        __syncthreads();  // everyone has read n_list before anyone adds to it
         if (!room) evaluate();
     }
     evaluate();
@@ -640,6 +696,8 @@ cudaError_t f4_topk(const F4& a, const F4& b, int k, long long self, int* idx, f
     q.k = k;
     q.self = self;
     q.noct = plan.noct;
+    q.gshift = 0;
+    while (((plan.noct * (kOctKeys / 8) - 1) >> q.gshift) + 1 > kGroups) ++q.gshift;
     q.keys = p.keys;
     q.errs = p.errs;
     q.idx = idx;
