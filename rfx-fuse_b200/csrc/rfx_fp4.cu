@@ -82,10 +82,11 @@ __global__ void k_f4_amax(const T* __restrict__ x, long long ld, int rows, int c
     if ((threadIdx.x & 31) == 0 && m) atomicMax(out, m);
 }
 
-// Twice the squared norm's share of eight codes: the exact sum of (2 code)^2.
+// Four times the squared norm of eight codes, 4 at least: a norm bound is then never below a
+// scale, so that no product of two scales overflows where the bounds' product does not.
 __device__ __forceinline__ int mag2(uint32_t w) {
     const uint32_t m0 = e2m1_mag4(w), m1 = e2m1_mag4(w >> 16);
-    return (int)__dp4a(m1, m1, __dp4a(m0, m0, 0u));
+    return max(4, (int)__dp4a(m1, m1, __dp4a(m0, m0, 0u)));
 }
 
 // Bound of the tile's row norms from the units' sums of squares n2[row][U] (doubles, so that no

@@ -30,13 +30,12 @@ namespace rfx {
 namespace {
 
 constexpr int kKThreads = 576;
-constexpr int kPickThreads = 256;
 constexpr int kGroups = 1024;                // groups of keys whose largest ones bound the k-th value
 constexpr int kOct = 8;                      // tiles of b whose keys a lane keeps before it stores them
 constexpr int kOctKeys = 4 * kOct;           // keys of a row and 8 tiles
 constexpr float kEps = 1.0f / 32768.0f;
 constexpr uint32_t kAlways = 0xFFFFu;        // key of a chunk that has to be looked at (no float's)
-constexpr int kList = 8 * kPickThreads + 256; // chunks waiting for their evaluation
+constexpr int kList = 8 * 512 + 256;         // chunks waiting for their evaluation
 constexpr int kFound = 1024;                 // values waiting to be ranked
 
 struct KeysArgs {
@@ -45,7 +44,7 @@ struct KeysArgs {
     int nq;               // row tiles of a in it
     int ntiles, noct;     // tiles of b, and groups of 8
     uint32_t* keys;       // [rows of the batch][noct][16] pairs of keys
-    float* errs;          // [grid] largest finite bound among the tiles of each block
+    float* errs;          // [grid] largest err of a block's tiles; negative: some tiles have none
     int* err;
 };
 
@@ -276,6 +275,7 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
         const uint32_t lane_addr = tmem + ((uint32_t)(32 * quarter) << 16) + (uint32_t)(64 * half);
         const float kNegInf = -__int_as_float(0x7f800000);
         float worst = 0.0f;  // largest bound of this block's tiles that the filter can use
+        bool some_forced = false;
         uint32_t n = (uint32_t)par;  // this warp's next tile in the CTA's sequence
         bool ok = true;
         int qt = p.q0 + (int)(u0 / p.noct), oct = (int)(u0 % p.noct);
@@ -287,6 +287,7 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
             const int nt = min(kOct, p.ntiles - oct * kOct);
             // a sum of such terms can overflow fp32 and lose its sign: those tiles are looked at
             const uint32_t forced = __ballot_sync(0xFFFFFFFFu, !(bq * bd * kEps < 1e30f));
+            if (forced) some_forced = true;
             if (!((forced >> lane) & 1u)) worst = fmaxf(worst, bq * bd * (kEps * 1.000001f));
             const int ncols = min(kOct * 128, p.b.rows - oct * kOct * 128) - 64 * half;  // columns that exist
             uint32_t* out = p.keys + ((row - (long long)p.q0 * 128) * p.noct + oct) * (kOctKeys / 2) + 8 * half + 4 * par;
@@ -366,7 +367,7 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
         }
         if (warp == 0) {
             for (int o = 16; o; o >>= 1) worst = fmaxf(worst, __shfl_xor_sync(0xFFFFFFFFu, worst, o));
-            if (lane == 0) p.errs[blockIdx.x] = worst;
+            if (lane == 0) p.errs[blockIdx.x] = some_forced ? -fmaxf(worst, 1e-37f) : worst;
         }
     }
     tc_fence_before();
@@ -389,14 +390,12 @@ __device__ __forceinline__ int dot4(int qa, uint32_t w, int acc) {
     return __dp4a(qa, (int)m, acc) - 2 * __dp4a(qa, (int)(m & e2m1_neg4(w)), 0);
 }
 
-// Four times the exact value of the row (decoded in qa, scales in sa) with row j of b, without
-// the matrix scales; NaN when a scale is.
+// Four times the exact value of the row (decoded in qa, scales in sa) with a row of b (codes cb,
+// first scale sb), without the matrix scales; NaN when a scale is.
 template <int kNv>
-__device__ double f4_exact(const int* qa, const double* sa, const F4& b, long long j) {
-    const uint4* cb = reinterpret_cast<const uint4*>(b.codes + j * b.pitch());
-    const uint8_t* sb = b.scales + f4_scale_at(b, j, 0);
+__device__ __noinline__ double f4_exact(const int* qa, const float* sa, const uint4* cb, const uint8_t* sb, int steps) {
     double v = 0.0;
-    for (int c = 0; c < b.Kp / 64; ++c) {
+    for (int c = 0; c < steps; ++c) {
         uint32_t wb = __ldg(reinterpret_cast<const uint32_t*>(sb + (kNv ? c : c >> 1) * kF4Atom));
         if (!kNv && (c & 1)) wb >>= 16;
 #pragma unroll
@@ -412,74 +411,140 @@ __device__ double f4_exact(const int* qa, const double* sa, const F4& b, long lo
             hi = dot4(q[7], y.w >> 16, hi);
             if (kNv) {
                 // e4m3 times e4m3 times the integer: exact, and so is every sum
-                v += sa[4 * c + 2 * h] * (double)e4m3_value((wb >> (16 * h)) & 0xFFu) * (double)lo;
-                v += sa[4 * c + 2 * h + 1] * (double)e4m3_value((wb >> (16 * h + 8)) & 0xFFu) * (double)hi;
+                v += (double)sa[4 * c + 2 * h] * (double)e4m3_value((wb >> (16 * h)) & 0xFFu) * (double)lo;
+                v += (double)sa[4 * c + 2 * h + 1] * (double)e4m3_value((wb >> (16 * h + 8)) & 0xFFu) * (double)hi;
             } else {
                 const uint32_t eb = (wb >> (8 * h)) & 0xFFu;
                 const double s = eb == 255u ? __longlong_as_double(0x7ff8000000000000ll)
                                             : __longlong_as_double((long long)(eb + 896u) << 52);  // 2^(eb - 127)
-                v += sa[2 * c + h] * s * (double)(lo + hi);
+                v += (double)sa[2 * c + h] * s * (double)(lo + hi);
             }
         }
     }
     return v;
 }
 
+// The same in fp32: within the accumulators' own bound (at most 16 blocks, a few units of 2^-24
+// of the terms' sum), so that the same err covers it.
 template <int kNv>
-__global__ void __launch_bounds__(kPickThreads, 5)
+__device__ __forceinline__ float f4_estimate(const int* qa, const float* sa, const uint4* cb, const uint8_t* sb,
+                                             int steps) {
+    float v = 0.0f;
+    for (int c = 0; c < steps; ++c) {
+        uint32_t wb = __ldg(reinterpret_cast<const uint32_t*>(sb + (kNv ? c : c >> 1) * kF4Atom));
+        const uint4 y2[2] = {__ldg(cb + 2 * c), __ldg(cb + 2 * c + 1)};
+        if (!kNv && (c & 1)) wb >>= 16;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint4 y = y2[h];
+            const int4 q0 = *reinterpret_cast<const int4*>(qa + 16 * c + 8 * h);
+            const int4 q1 = *reinterpret_cast<const int4*>(qa + 16 * c + 8 * h + 4);
+            int lo = 0, hi = 0, nlo = 0, nhi = 0;  // all terms, and those of negative codes
+            const int qs[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
+            const uint32_t ws[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t w = (e & 1) ? ws[e >> 1] >> 16 : ws[e >> 1];
+                const uint32_t m = e2m1_mag4(w);
+                const uint32_t mn = m & e2m1_neg4(w);
+                if (e < 4) {
+                    lo = __dp4a(qs[e], (int)m, lo);
+                    nlo = __dp4a(qs[e], (int)mn, nlo);
+                } else {
+                    hi = __dp4a(qs[e], (int)m, hi);
+                    nhi = __dp4a(qs[e], (int)mn, nhi);
+                }
+            }
+            if (kNv) {
+                v = fmaf(sa[4 * c + 2 * h] * e4m3_value((wb >> (16 * h)) & 0xFFu), (float)(lo - 2 * nlo), v);
+                v = fmaf(sa[4 * c + 2 * h + 1] * e4m3_value((wb >> (16 * h + 8)) & 0xFFu), (float)(hi - 2 * nhi), v);
+            } else {
+                v = fmaf(sa[2 * c + h] * e8m0_value((wb >> (8 * h)) & 0xFFu), (float)(lo + hi - 2 * (nlo + nhi)), v);
+            }
+        }
+    }
+    return v;
+}
+
+// kT threads a row: 256, several rows an SM; 1024 when there are too few rows to fill the GPU.
+template <int kNv, int kT>
+__global__ void __launch_bounds__(kT, kT == 256 ? 4 : 1)
 k_f4_pick(PickArgs p) {
-    __shared__ int qa[kF4TopkK / 4];
-    __shared__ double sa[kF4TopkK / 16];
-    __shared__ double fv[kFound];       // found: values (4 x), columns
+    __shared__ __align__(16) int qa[kF4TopkK / 4];
+    __shared__ float sa[kF4TopkK / 16];
+    __shared__ double fv[kFound];       // found: values (4 x) of the first n_known, columns of all
     __shared__ int fj[kFound];
-    __shared__ uint32_t list[kList];    // chunks to evaluate
+    __shared__ uint32_t list[kList];    // chunks to look at
     __shared__ uint32_t tops[kGroups];  // a group's largest key; kVisit: it holds a chunk to look at
     __shared__ uint16_t glist[kGroups]; // groups to look at
-    __shared__ int n_list, n_found, n_groups;
+    __shared__ int n_list, n_found, n_groups, n_valid;
     __shared__ uint32_t s_key;
     __shared__ float s_err;
+    __shared__ int s_forced;
     constexpr uint32_t kVisit = 0x10000u;
+    const double kNegInf = -__longlong_as_double(0x7ff0000000000000ll);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const long long i = (long long)p.row0 + blockIdx.x;
     const int kp = p.self >= 0 ? p.k + 1 : p.k;  // the row itself may be one of the k columns
     const long long self = p.self >= 0 ? p.self + i : -1;
     const uint4* keys = reinterpret_cast<const uint4*>(p.keys + (long long)blockIdx.x * p.noct * (kOctKeys / 2));
     const int nvec = p.noct * (kOctKeys / 8);    // 8 keys each
+    const uint8_t* b_codes = p.b.codes;
+    const uint8_t* b_scales = p.b.scales;
+    const int pitch = p.b.pitch(), tile_bytes = p.b.natoms * kF4Atom, steps = p.b.Kp / 64;
+    auto codes_of = [=](int j) { return reinterpret_cast<const uint4*>(b_codes + (long long)j * pitch); };
+    auto scales_of = [=](int j) {
+        return b_scales + (long long)(j >> 7) * tile_bytes + (j & 31) * 16 + ((j >> 5) & 3) * 4;
+    };
     const bool single = nvec * 8 <= kGroups;     // a key is a group of its own
     const int gs = single ? 0 : p.gshift;        // else 2^gs vectors are
     const int ngroups = single ? nvec * 8 : ((nvec - 1) >> gs) + 1;
 
     // the row, decoded, and its scales
-    for (int t = tid; t < p.a.Kp / 4; t += kPickThreads) {
+    for (int t = tid; t < p.a.Kp / 4; t += kT) {
         const uint32_t w = *reinterpret_cast<const uint16_t*>(p.a.codes + i * p.a.pitch() + 2 * t);
         int d = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) d |= ((int)(2.0f * e2m1_value((w >> (4 * e)) & 15u)) & 0xFF) << (8 * e);
         qa[t] = d;
     }
-    for (int t = tid; t < p.a.Kp / (kNv ? 16 : 32); t += kPickThreads)
-        sa[t] = (double)f4_scale_value(kNv, p.a.scales[f4_scale_at(p.a, i, t)]);
-    if (warp == 0) {
+    for (int t = tid; t < p.a.Kp / (kNv ? 16 : 32); t += kT)
+        sa[t] = f4_scale_value(kNv, p.a.scales[f4_scale_at(p.a, i, t)]);
+    if (warp == kT / 32 - 1) {
         float e = 0.0f;
-        for (int t = lane; t < p.nerrs; t += 32) e = fmaxf(e, __ldg(p.errs + t));
+        bool f = false;
+        for (int t = lane; t < p.nerrs; t += 32) {
+            const float x = __ldg(p.errs + t);
+            f |= x < 0.0f;
+            e = fmaxf(e, fabsf(x));
+        }
         for (int o = 16; o; o >>= 1) e = fmaxf(e, __shfl_xor_sync(0xFFFFFFFFu, e, o));
+        f = __any_sync(0xFFFFFFFFu, f);
         if (lane == 0) {
             s_err = fmaxf(e, 1e-37f);
+            s_forced = f;
             n_list = n_found = n_groups = 0;
         }
     }
-    if (gs > 5) {
-        for (int t = tid; t < ngroups; t += kPickThreads) tops[t] = 0;
-        __syncthreads();
-    }
+    for (int t = tid; t < ngroups; t += kT) tops[t] = 0;
+    __syncthreads();
+    const bool forced = s_forced != 0;  // some chunks have to be looked at whatever their keys
     // the largest key of every group
-    for (int t0 = 0; t0 < nvec; t0 += kPickThreads) {
+#pragma unroll 4
+    for (int t0 = 0; t0 < nvec; t0 += kT) {
         const int t = t0 + tid;
         uint4 x = make_uint4(0, 0, 0, 0);
         if (t < nvec) x = __ldg(keys + t);
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        uint32_t visit = 0;
+        if (forced) {
+            const uint32_t a0 = __vcmpeq2(x.x, 0xFFFFFFFFu), a1 = __vcmpeq2(x.y, 0xFFFFFFFFu);
+            const uint32_t a2 = __vcmpeq2(x.z, 0xFFFFFFFFu), a3 = __vcmpeq2(x.w, 0xFFFFFFFFu);
+            if (a0 | a1 | a2 | a3) visit = kVisit;
+            if (!single) x = make_uint4(x.x & ~a0, x.y & ~a1, x.z & ~a2, x.w & ~a3);
+        }
         if (single) {
             if (t < nvec) {
+                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const uint32_t key = (w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
@@ -488,22 +553,18 @@ k_f4_pick(PickArgs p) {
             }
             continue;
         }
-        uint32_t best = 0, visit = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const uint32_t key = (w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
-            if (key == kAlways) visit = kVisit;
-            else best = max(best, key);
-        }
+        const uint32_t m = __vmaxu2(__vmaxu2(x.x, x.y), __vmaxu2(x.z, x.w));
+        uint32_t best = max(m & 0xFFFFu, m >> 16) | visit;  // the flag is above every key
         for (int o = 1; o < 32 && o < (1 << gs); o <<= 1) {
-            best = max(best, __shfl_xor_sync(0xFFFFFFFFu, best, o));
-            visit |= __shfl_xor_sync(0xFFFFFFFFu, visit, o);
+            const uint32_t other = __shfl_xor_sync(0xFFFFFFFFu, best, o);
+            best = max(best & 0xFFFFu, other & 0xFFFFu) | ((best | other) & kVisit);
         }
-        if (gs <= 5) {
-            if (t < nvec && (t & ((1 << gs) - 1)) == 0) tops[t >> gs] = best | visit;
-        } else if (lane == 0 && t < nvec) {
-            atomicMax(&tops[t >> gs], best);  // visit goes in after the maximum
-            if (visit) atomicOr(&n_groups, 0x40000000);
+        if (t < nvec && (t & ((1 << min(gs, 5)) - 1)) == 0) {
+            if (gs <= 5) {
+                tops[t >> gs] = best;
+            } else {  // a flag hides the maximum: lower, so still a bound
+                atomicMax(&tops[t >> gs], best & kVisit ? kVisit : best);
+            }
         }
     }
     __syncthreads();
@@ -524,65 +585,72 @@ k_f4_pick(PickArgs p) {
     }
     __syncthreads();
     const double err = (double)s_err;
-    const bool everything = (n_groups & 0x40000000) != 0;  // some group of more than 32 vectors is to be looked at
     // the k-th value is at least this
-    double floor_v = s_key > key_of(-__int_as_float(0x7f800000)) ? (double)key_floor(s_key) - err : -__longlong_as_double(0x7ff0000000000000ll);
-    __syncthreads();
-    if (tid == 0) n_groups = 0;
-    __syncthreads();
-    // an accumulator of the answer is at least floor - err
-    auto bar_of = [&]() { return key_of(__double2float_rd(floor_v - err)); };
-    const uint32_t bar0 = bar_of();
-    for (int t = tid; t < ngroups; t += kPickThreads)
-        if (everything || tops[t] >= max(bar0, 1u)) glist[atomicAdd(&n_groups, 1)] = (uint16_t)t;
+    double floor_v = s_key > key_of(-__int_as_float(0x7f800000)) ? (double)key_floor(s_key) - err : kNegInf;
+    // an accumulator, or an estimate, of the answer is at least floor - err
+    auto bar_of = [&]() { return max(key_of(__double2float_rd(floor_v - err)), 1u); };
+    {
+        const uint32_t bar = bar_of();
+        for (int t = tid; t < ngroups; t += kT)
+            if (tops[t] >= bar) glist[atomicAdd(&n_groups, 1)] = (uint16_t)t;
+    }
     __syncthreads();
 
-    // Ranks what was found, keeps the best k at the front and raises the floor.
+    // Evaluates what was found exactly, ranks it, keeps the best k at the front and raises the floor.
+    int n_known = 0;
     auto rank_found = [&]() {
         __syncthreads();
         const int n = n_found;
-        double v[kFound / kPickThreads];
-        int j[kFound / kPickThreads], r[kFound / kPickThreads];
+        if (tid == 0) n_valid = 0;
+        for (int t = n_known + tid; t < n; t += kT) {
+            const double x = f4_exact<kNv>(qa, sa, codes_of(fj[t]), scales_of(fj[t]), steps);
+            const bool in = x * 0.25 >= floor_v;  // false for NaN
+            fv[t] = in ? x : kNegInf;
+            if (!in) fj[t] = 0x7FFFFFFF;
+        }
+        __syncthreads();
+        constexpr int kE = (kFound + kT - 1) / kT;
+        double v[kE];
+        int j[kE], r[kE];
 #pragma unroll
-        for (int e = 0; e < kFound / kPickThreads; ++e) {
-            const int t = tid + e * kPickThreads;
+        for (int e = 0; e < kE; ++e) {
+            const int t = tid + e * kT;
             r[e] = kFound;
-            if (t >= n) continue;
+            if (t >= n || fj[t] == 0x7FFFFFFF) continue;
             v[e] = fv[t];
             j[e] = fj[t];
             int c = 0;
             for (int o = 0; o < n; ++o) c += f4_better(fv[o], fj[o], v[e], j[e]);
             r[e] = c;
+            if (c < p.k) atomicAdd(&n_valid, 1);
         }
         __syncthreads();
 #pragma unroll
-        for (int e = 0; e < kFound / kPickThreads; ++e)
+        for (int e = 0; e < kE; ++e)
             if (r[e] < p.k) {
                 fv[r[e]] = v[e];
                 fj[r[e]] = j[e];
             }
-        if (tid == 0) n_found = min(n, p.k);
+        if (tid == 0) n_found = n_valid;
         __syncthreads();
-        if (n_found == p.k) floor_v = fmax(floor_v, 0.25 * fv[p.k - 1]);
+        n_known = n_found;
+        if (n_known == p.k) floor_v = fmax(floor_v, 0.25 * fv[p.k - 1]);
         __syncthreads();
     };
-    // Evaluates the chunks of the list, a lane a column, as many at a time as surely have room.
-    auto evaluate = [&]() {
+    // Looks at the chunks of the list, a lane a column, as many at a time as surely have room.
+    auto look = [&]() {
         __syncthreads();
         const int n = n_list;
         for (int c0 = 0; c0 < n;) {
             const int room = (kFound - n_found) / 32;
             __syncthreads();  // everyone has read n_found before anyone adds to it
             const int c1 = min(n, c0 + room);
-            for (int c = c0 + warp; c < c1; c += kPickThreads / 32) {
+            const float least = 4.0f * __double2float_rd(floor_v - err);
+            for (int c = c0 + warp; c < c1; c += kT / 32) {
                 const long long j = (long long)list[c] * 32 + lane;
                 if (j < p.b.rows && j != self) {
-                    const double v = f4_exact<kNv>(qa, sa, p.b, j);
-                    if (v * 0.25 >= floor_v) {  // false for NaN
-                        const int at = atomicAdd(&n_found, 1);
-                        fv[at] = v;
-                        fj[at] = (int)j;
-                    }
+                    // without a bound on the terms fp32 could overflow: rank_found decides
+                    if (forced || f4_estimate<kNv>(qa, sa, codes_of((int)j), scales_of((int)j), steps) >= least) fj[atomicAdd(&n_found, 1)] = (int)j;
                 }
             }
             c0 = c1;
@@ -594,11 +662,12 @@ k_f4_pick(PickArgs p) {
     };
     // the groups' chunks that may hold a column of the answer
     const int ng = n_groups;
+    constexpr int kScan = kT < 512 ? kT : 512;    // vectors a round
     const long long ntask = (long long)ng << gs;  // a vector (a key when single) each
-    for (long long t0 = 0; t0 < ntask; t0 += kPickThreads) {
-        const uint32_t bar = max(bar_of(), 1u);
+    for (long long t0 = 0; t0 < ntask; t0 += kScan) {
+        const uint32_t bar = bar_of();
         const long long t = t0 + tid;
-        if (t < ntask) {
+        if (tid < kScan && t < ntask) {
             const long long g = glist[t >> gs];
             const long long vec = single ? g >> 3 : (g << gs) + (t & ((1 << gs) - 1));
             if (vec < nvec) {
@@ -617,15 +686,15 @@ k_f4_pick(PickArgs p) {
             }
         }
         __syncthreads();
-        const bool room = n_list <= kList - 8 * kPickThreads;
+        const bool room = n_list <= kList - 8 * kScan;
         __syncthreads();  // everyone has read n_list before anyone adds to it
-        if (!room) evaluate();
+        if (!room) look();
     }
-    evaluate();
+    look();
     rank_found();
     const double g = (double)__ldg(p.a.gs) * (double)__ldg(p.b.gs);
-    for (int s = tid; s < p.k; s += kPickThreads) {
-        const bool in = s < n_found;
+    for (int s = tid; s < p.k; s += kT) {
+        const bool in = s < n_known;
         p.idx[i * p.k + s] = in ? fj[s] : -1;
         p.val[i * p.k + s] = in ? (float)(fv[s] * 0.25 * g) : -__int_as_float(0x7f800000);
     }
@@ -713,8 +782,13 @@ cudaError_t f4_topk(const F4& a, const F4& b, int k, long long self, int* idx, f
         if (e != cudaSuccess) return e;
         q.row0 = (int)r0;
         q.nerrs = grid;
-        if (b.nv) k_f4_pick<1><<<rows, kPickThreads, 0, st>>>(q);
-        else k_f4_pick<0><<<rows, kPickThreads, 0, st>>>(q);
+        if (rows <= 2 * sms) {
+            if (b.nv) k_f4_pick<1, 1024><<<rows, 1024, 0, st>>>(q);
+            else k_f4_pick<0, 1024><<<rows, 1024, 0, st>>>(q);
+        } else {
+            if (b.nv) k_f4_pick<1, 256><<<rows, 256, 0, st>>>(q);
+            else k_f4_pick<0, 256><<<rows, 256, 0, st>>>(q);
+        }
         *launches += 2;
         if ((e = cudaGetLastError()) != cudaSuccess) return e;
     }
