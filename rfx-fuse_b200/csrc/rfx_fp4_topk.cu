@@ -11,7 +11,7 @@
 //   k_f4_keys  products of 128 rows of a with b's tiles of 128 rows (tcgen05, block-scaled); of
 //              every row's 32 neighbouring accumulators only the maximum is kept, as the upper 16
 //              bits of its order-preserving integer (rounded down).
-//   k_f4_pick  a block per row of a.  The keys form up to 1024 groups; the k-th largest of the
+//   k_f4_pick  a block per row of a.  The keys form as many groups as threads at most; the k-th largest of the
 //              groups' largest keys, L, is a lower bound of the k-th largest key: there are k
 //              columns with accumulators of L or more, so the k-th value is at least L - err, and
 //              a column of the answer has an accumulator of at least L - 2 err.  Only chunks whose
@@ -30,7 +30,6 @@ namespace rfx {
 namespace {
 
 constexpr int kKThreads = 576;
-constexpr int kGroups = 1024;                // groups of keys whose largest ones bound the k-th value
 constexpr int kOct = 8;                      // tiles of b whose keys a lane keeps before it stores them
 constexpr int kOctKeys = 4 * kOct;           // keys of a row and 8 tiles
 constexpr float kEps = 1.0f / 32768.0f;
@@ -53,7 +52,8 @@ struct PickArgs {
     int row0;             // first row of the batch
     int k;
     long long self;       // row of b that is row 0 of a and left out for it (and so on); -1: none
-    int noct, gshift;     // 2^gshift vectors of 8 keys are a group
+    int noct;
+    int h;                // 2^h keys are a group; at most kT groups
     const uint32_t* keys;
     const float* errs;
     int nerrs;
@@ -475,10 +475,9 @@ k_f4_pick(PickArgs p) {
     __shared__ double fv[kFound];       // found: values (4 x) of the first n_known, columns of all
     __shared__ int fj[kFound];
     __shared__ uint32_t list[kList];    // chunks to look at
-    __shared__ uint32_t tops[kGroups];  // a group's largest key; kVisit: it holds a chunk to look at
-    __shared__ uint16_t glist[kGroups]; // groups to look at
+    __shared__ uint32_t tops[kT];       // a group's largest key; kVisit: it holds a chunk to look at
+    __shared__ uint16_t glist[kT];      // groups to look at
     __shared__ int n_list, n_found, n_groups, n_valid;
-    __shared__ uint32_t s_key;
     __shared__ float s_err;
     __shared__ int s_forced;
     constexpr uint32_t kVisit = 0x10000u;
@@ -496,10 +495,60 @@ k_f4_pick(PickArgs p) {
     auto scales_of = [=](int j) {
         return b_scales + (long long)(j >> 7) * tile_bytes + (j & 31) * 16 + ((j >> 5) & 3) * 4;
     };
-    const bool single = nvec * 8 <= kGroups;     // a key is a group of its own
-    const int gs = single ? 0 : p.gshift;        // else 2^gs vectors are
-    const int ngroups = single ? nvec * 8 : ((nvec - 1) >> gs) + 1;
+    const int h = p.h, gs = max(h - 3, 0);       // groups of 2^h keys: of 2^gs vectors, or parts of one
+    const int ngroups = ((nvec * 8 - 1) >> h) + 1;
 
+    if (gs > 5) {
+        tops[tid] = 0;
+        __syncthreads();
+    }
+    // the largest key of every group
+#pragma unroll 4
+    for (int t0 = 0; t0 < nvec; t0 += kT) {
+        const int t = t0 + tid;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (t < nvec) x = __ldg(keys + t);
+        // chunks that have to be looked at whatever their keys
+        const uint32_t a0 = __vcmpeq2(x.x, 0xFFFFFFFFu), a1 = __vcmpeq2(x.y, 0xFFFFFFFFu);
+        const uint32_t a2 = __vcmpeq2(x.z, 0xFFFFFFFFu), a3 = __vcmpeq2(x.w, 0xFFFFFFFFu);
+        if (h >= 3) {
+            const uint32_t m = __vmaxu2(__vmaxu2(x.x & ~a0, x.y & ~a1), __vmaxu2(x.z & ~a2, x.w & ~a3));
+            uint32_t best = max(m & 0xFFFFu, m >> 16) | ((a0 | a1 | a2 | a3) ? kVisit : 0u);
+            for (int o = 1; o < 32 && o < (1 << gs); o <<= 1) {
+                const uint32_t other = __shfl_xor_sync(0xFFFFFFFFu, best, o);
+                best = max(best & 0xFFFFu, other & 0xFFFFu) | ((best | other) & kVisit);
+            }
+            if (t < nvec && (t & ((1 << min(gs, 5)) - 1)) == 0) {
+                // (a flag above the maximum hides it: lower, so still a bound)
+                if (gs <= 5) tops[t >> gs] = best;
+                else atomicMax(&tops[t >> gs], best & kVisit ? kVisit : best);
+            }
+        } else if (t < nvec) {
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            uint32_t key[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                key[e] = (w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
+                if (key[e] == kAlways) key[e] = kVisit;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (h == 0) {
+                    tops[8 * t + e] = key[e];
+                } else if (h == 1 && (e & 1) == 0) {
+                    tops[4 * t + e / 2] = (max(key[e] & 0xFFFFu, key[e + 1] & 0xFFFFu)) | ((key[e] | key[e + 1]) & kVisit);
+                } else if (h == 2 && (e & 3) == 0) {
+                    uint32_t m = 0, f = 0;
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) {
+                        m = max(m, key[(e & 4) + d] & 0xFFFFu);
+                        f |= key[(e & 4) + d] & kVisit;
+                    }
+                    tops[2 * t + e / 4] = m | f;
+                }
+            }
+        }
+    }
     // the row, decoded, and its scales
     for (int t = tid; t < p.a.Kp / 4; t += kT) {
         const uint32_t w = *reinterpret_cast<const uint16_t*>(p.a.codes + i * p.a.pitch() + 2 * t);
@@ -526,74 +575,19 @@ k_f4_pick(PickArgs p) {
             n_list = n_found = n_groups = 0;
         }
     }
-    for (int t = tid; t < ngroups; t += kT) tops[t] = 0;
     __syncthreads();
-    const bool forced = s_forced != 0;  // some chunks have to be looked at whatever their keys
-    // the largest key of every group
-#pragma unroll 4
-    for (int t0 = 0; t0 < nvec; t0 += kT) {
-        const int t = t0 + tid;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (t < nvec) x = __ldg(keys + t);
-        uint32_t visit = 0;
-        if (forced) {
-            const uint32_t a0 = __vcmpeq2(x.x, 0xFFFFFFFFu), a1 = __vcmpeq2(x.y, 0xFFFFFFFFu);
-            const uint32_t a2 = __vcmpeq2(x.z, 0xFFFFFFFFu), a3 = __vcmpeq2(x.w, 0xFFFFFFFFu);
-            if (a0 | a1 | a2 | a3) visit = kVisit;
-            if (!single) x = make_uint4(x.x & ~a0, x.y & ~a1, x.z & ~a2, x.w & ~a3);
-        }
-        if (single) {
-            if (t < nvec) {
-                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const uint32_t key = (w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
-                    tops[8 * t + e] = key == kAlways ? kVisit : key;
-                }
-            }
-            continue;
-        }
-        const uint32_t m = __vmaxu2(__vmaxu2(x.x, x.y), __vmaxu2(x.z, x.w));
-        uint32_t best = max(m & 0xFFFFu, m >> 16) | visit;  // the flag is above every key
-        for (int o = 1; o < 32 && o < (1 << gs); o <<= 1) {
-            const uint32_t other = __shfl_xor_sync(0xFFFFFFFFu, best, o);
-            best = max(best & 0xFFFFu, other & 0xFFFFu) | ((best | other) & kVisit);
-        }
-        if (t < nvec && (t & ((1 << min(gs, 5)) - 1)) == 0) {
-            if (gs <= 5) {
-                tops[t >> gs] = best;
-            } else {  // a flag hides the maximum: lower, so still a bound
-                atomicMax(&tops[t >> gs], best & kVisit ? kVisit : best);
-            }
-        }
-    }
-    __syncthreads();
-    // L: the kp-th largest of them, by bisection of its 16 bits (0: there are fewer)
-    if (warp == 0) {
-        uint32_t v[kGroups / 32];
-#pragma unroll
-        for (int e = 0; e < kGroups / 32; ++e) v[e] = lane + 32 * e < ngroups ? tops[lane + 32 * e] & 0xFFFFu : 0u;
-        uint32_t key = 0;
-        for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
-            const uint32_t mid = key | bit;
-            int c = 0;
-#pragma unroll
-            for (int e = 0; e < kGroups / 32; ++e) c += v[e] >= mid;
-            if (__reduce_add_sync(0xFFFFFFFFu, c) >= kp) key = mid;
-        }
-        if (lane == 0) s_key = key;
-    }
-    __syncthreads();
+    const bool forced = s_forced != 0;
+    // L: the kp-th largest of the groups' keys, by bisection of its 16 bits (0: there are fewer)
+    const uint32_t mytop = tid < ngroups ? tops[tid] : 0u;
+    uint32_t s_key = 0;
+    for (uint32_t bit = 0x8000u; bit; bit >>= 1)
+        if (__syncthreads_count((mytop & 0xFFFFu) >= (s_key | bit)) >= kp) s_key |= bit;
     const double err = (double)s_err;
     // the k-th value is at least this
     double floor_v = s_key > key_of(-__int_as_float(0x7f800000)) ? (double)key_floor(s_key) - err : kNegInf;
     // an accumulator, or an estimate, of the answer is at least floor - err
     auto bar_of = [&]() { return max(key_of(__double2float_rd(floor_v - err)), 1u); };
-    {
-        const uint32_t bar = bar_of();
-        for (int t = tid; t < ngroups; t += kT)
-            if (tops[t] >= bar) glist[atomicAdd(&n_groups, 1)] = (uint16_t)t;
-    }
+    if (mytop >= bar_of()) glist[atomicAdd(&n_groups, 1)] = (uint16_t)tid;
     __syncthreads();
 
     // Evaluates what was found exactly, ranks it, keeps the best k at the front and raises the floor.
@@ -663,13 +657,13 @@ k_f4_pick(PickArgs p) {
     // the groups' chunks that may hold a column of the answer
     const int ng = n_groups;
     constexpr int kScan = kT < 512 ? kT : 512;    // vectors a round
-    const long long ntask = (long long)ng << gs;  // a vector (a key when single) each
+    const long long ntask = (long long)ng << gs;  // a vector each
     for (long long t0 = 0; t0 < ntask; t0 += kScan) {
         const uint32_t bar = bar_of();
         const long long t = t0 + tid;
         if (tid < kScan && t < ntask) {
             const long long g = glist[t >> gs];
-            const long long vec = single ? g >> 3 : (g << gs) + (t & ((1 << gs) - 1));
+            const long long vec = h < 3 ? (g << h) >> 3 : (g << gs) + (t & ((1 << gs) - 1));
             if (vec < nvec) {
                 const uint4 x = __ldg(keys + vec);
                 const uint32_t w[4] = {x.x, x.y, x.z, x.w};
@@ -678,7 +672,7 @@ k_f4_pick(PickArgs p) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const uint32_t key = (w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
-                    if (key >= bar && (!single || e == (int)(g & 7))) {
+                    if (key >= bar && (h >= 3 || (int)((8 * vec + e) >> h) == (int)g)) {
                         const int chunk = (oct * kOct + 2 * (e >> 1) + par) * 4 + 2 * half + (e & 1);
                         list[atomicAdd(&n_list, 1)] = (uint32_t)chunk;
                     }
@@ -707,7 +701,8 @@ __global__ void k_f4_topk_none(long long n, int* idx, float* val) {
     }
 }
 
-// Rows of a whose keys are made before they are read: about 48 MB of keys, whole tiles.
+// Rows of a whose keys are made before they are read.
+constexpr long long kKeyMB = 256;
 struct TopkPlan {
     int noct, rows;
     long long key_bytes;
@@ -716,7 +711,7 @@ TopkPlan topk_plan(const F4& a, const F4& b) {
     TopkPlan t;
     t.noct = (b.tiles() + kOct - 1) / kOct;
     const long long row = (long long)t.noct * kOctKeys * 2;
-    const long long tiles = std::max(1ll, (48ll << 20) / (row * 128));
+    const long long tiles = std::max(1ll, (kKeyMB << 20) / (row * 128));
     t.rows = (int)std::min<long long>(a.rows, tiles * 128);
     t.key_bytes = (row * t.rows + 255) / 256 * 256;
     return t;
@@ -765,8 +760,6 @@ cudaError_t f4_topk(const F4& a, const F4& b, int k, long long self, int* idx, f
     q.k = k;
     q.self = self;
     q.noct = plan.noct;
-    q.gshift = 0;
-    while (((plan.noct * (kOctKeys / 8) - 1) >> q.gshift) + 1 > kGroups) ++q.gshift;
     q.keys = p.keys;
     q.errs = p.errs;
     q.idx = idx;
@@ -782,7 +775,10 @@ cudaError_t f4_topk(const F4& a, const F4& b, int k, long long self, int* idx, f
         if (e != cudaSuccess) return e;
         q.row0 = (int)r0;
         q.nerrs = grid;
-        if (rows <= 2 * sms) {
+        const int threads = rows <= 2 * sms ? 1024 : 256;
+        q.h = 0;
+        while (((plan.noct * kOctKeys - 1) >> q.h) + 1 > threads) ++q.h;
+        if (threads == 1024) {
             if (b.nv) k_f4_pick<1, 1024><<<rows, 1024, 0, st>>>(q);
             else k_f4_pick<0, 1024><<<rows, 1024, 0, st>>>(q);
         } else {
