@@ -34,7 +34,9 @@ constexpr int kOct = 8;                      // tiles of b whose keys a lane kee
 constexpr int kOctKeys = 4 * kOct;           // keys of a row and 8 tiles
 constexpr float kEps = 1.0f / 32768.0f;
 constexpr uint32_t kAlways = 0xFFFFu;        // key of a chunk that has to be looked at (no float's)
-constexpr int kList = 8 * 512 + 256;         // chunks waiting for their evaluation
+constexpr int kScan = 256;                   // units a round turns into chunks
+constexpr int kList = 8 * kScan + 256;       // chunks waiting for their evaluation
+constexpr int kUnits = 4096;                 // units of keys: a key, or every 4096th vector of 8
 constexpr int kFound = 1024;                 // values waiting to be ranked
 
 struct KeysArgs {
@@ -53,7 +55,6 @@ struct PickArgs {
     int k;
     long long self;       // row of b that is row 0 of a and left out for it (and so on); -1: none
     int noct;
-    int h;                // 2^h keys are a group; at most kT groups
     const uint32_t* keys;
     const float* errs;
     int nerrs;
@@ -424,43 +425,36 @@ __device__ __noinline__ double f4_exact(const int* qa, const float* sa, const ui
     return v;
 }
 
-// The same in fp32: within the accumulators' own bound (at most 16 blocks, a few units of 2^-24
-// of the terms' sum), so that the same err covers it.
+// 64 columns of the same in fp32, added to v: within the accumulators' own bound (at most 16 blocks,
+// a few units of 2^-24 of the terms' sum), so that the same err covers it.
 template <int kNv>
-__device__ __forceinline__ float f4_estimate(const int* qa, const float* sa, const uint4* cb, const uint8_t* sb,
-                                             int steps) {
-    float v = 0.0f;
-    for (int c = 0; c < steps; ++c) {
-        uint32_t wb = __ldg(reinterpret_cast<const uint32_t*>(sb + (kNv ? c : c >> 1) * kF4Atom));
-        const uint4 y2[2] = {__ldg(cb + 2 * c), __ldg(cb + 2 * c + 1)};
-        if (!kNv && (c & 1)) wb >>= 16;
+__device__ __forceinline__ float f4_estimate64(const int* qa, const float* sa, uint4 y0, uint4 y1, uint32_t wb, float v) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint4 y = y2[h];
-            const int4 q0 = *reinterpret_cast<const int4*>(qa + 16 * c + 8 * h);
-            const int4 q1 = *reinterpret_cast<const int4*>(qa + 16 * c + 8 * h + 4);
-            int lo = 0, hi = 0, nlo = 0, nhi = 0;  // all terms, and those of negative codes
-            const int qs[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
-            const uint32_t ws[4] = {y.x, y.y, y.z, y.w};
+    for (int h = 0; h < 2; ++h) {
+        const uint4 y = h ? y1 : y0;
+        const int4 q0 = *reinterpret_cast<const int4*>(qa + 8 * h);
+        const int4 q1 = *reinterpret_cast<const int4*>(qa + 8 * h + 4);
+        int lo = 0, hi = 0, nlo = 0, nhi = 0;  // all terms, and those of negative codes
+        const int qs[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
+        const uint32_t ws[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t w = (e & 1) ? ws[e >> 1] >> 16 : ws[e >> 1];
-                const uint32_t m = e2m1_mag4(w);
-                const uint32_t mn = m & e2m1_neg4(w);
-                if (e < 4) {
-                    lo = __dp4a(qs[e], (int)m, lo);
-                    nlo = __dp4a(qs[e], (int)mn, nlo);
-                } else {
-                    hi = __dp4a(qs[e], (int)m, hi);
-                    nhi = __dp4a(qs[e], (int)mn, nhi);
-                }
-            }
-            if (kNv) {
-                v = fmaf(sa[4 * c + 2 * h] * e4m3_value((wb >> (16 * h)) & 0xFFu), (float)(lo - 2 * nlo), v);
-                v = fmaf(sa[4 * c + 2 * h + 1] * e4m3_value((wb >> (16 * h + 8)) & 0xFFu), (float)(hi - 2 * nhi), v);
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t w = (e & 1) ? ws[e >> 1] >> 16 : ws[e >> 1];
+            const uint32_t m = e2m1_mag4(w);
+            const uint32_t mn = m & e2m1_neg4(w);
+            if (e < 4) {
+                lo = __dp4a(qs[e], (int)m, lo);
+                nlo = __dp4a(qs[e], (int)mn, nlo);
             } else {
-                v = fmaf(sa[2 * c + h] * e8m0_value((wb >> (8 * h)) & 0xFFu), (float)(lo + hi - 2 * (nlo + nhi)), v);
+                hi = __dp4a(qs[e], (int)m, hi);
+                nhi = __dp4a(qs[e], (int)mn, nhi);
             }
+        }
+        if (kNv) {
+            v = fmaf(sa[2 * h] * e4m3_value((wb >> (16 * h)) & 0xFFu), (float)(lo - 2 * nlo), v);
+            v = fmaf(sa[2 * h + 1] * e4m3_value((wb >> (16 * h + 8)) & 0xFFu), (float)(hi - 2 * nhi), v);
+        } else {
+            v = fmaf(sa[h] * e8m0_value((wb >> (8 * h)) & 0xFFu), (float)(lo + hi - 2 * (nlo + nhi)), v);
         }
     }
     return v;
@@ -475,17 +469,16 @@ k_f4_pick(PickArgs p) {
     __shared__ double fv[kFound];       // found: values (4 x) of the first n_known, columns of all
     __shared__ int fj[kFound];
     __shared__ uint32_t list[kList];    // chunks to look at
-    __shared__ uint32_t tops[kT];       // a group's largest key; kVisit: it holds a chunk to look at
-    __shared__ uint16_t glist[kT];      // groups to look at
-    __shared__ int n_list, n_found, n_groups, n_valid;
+    __shared__ __align__(16) uint16_t tops[kUnits];  // a unit's largest key
+    __shared__ uint16_t ulist[kUnits];  // units to look at
+    __shared__ int n_list, n_found, n_units, n_valid;
     __shared__ float s_err;
     __shared__ int s_forced;
-    constexpr uint32_t kVisit = 0x10000u;
     const double kNegInf = -__longlong_as_double(0x7ff0000000000000ll);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const long long i = (long long)p.row0 + blockIdx.x;
     const int kp = p.self >= 0 ? p.k + 1 : p.k;  // the row itself may be one of the k columns
-    const long long self = p.self >= 0 ? p.self + i : -1;
+    const int self = p.self >= 0 ? (int)(p.self + i) : -1;
     const uint4* keys = reinterpret_cast<const uint4*>(p.keys + (long long)blockIdx.x * p.noct * (kOctKeys / 2));
     const int nvec = p.noct * (kOctKeys / 8);    // 8 keys each
     const uint8_t* b_codes = p.b.codes;
@@ -495,57 +488,26 @@ k_f4_pick(PickArgs p) {
     auto scales_of = [=](int j) {
         return b_scales + (long long)(j >> 7) * tile_bytes + (j & 31) * 16 + ((j >> 5) & 3) * 4;
     };
-    const int h = p.h, gs = max(h - 3, 0);       // groups of 2^h keys: of 2^gs vectors, or parts of one
-    const int ngroups = ((nvec * 8 - 1) >> h) + 1;
+    const bool small = nvec * 8 <= kUnits;       // a unit is a key
+    const int nunits = small ? nvec * 8 : min(nvec, kUnits);
 
-    if (gs > 5) {
-        tops[tid] = 0;
-        __syncthreads();
-    }
-    // the largest key of every group
-#pragma unroll 4
-    for (int t0 = 0; t0 < nvec; t0 += kT) {
-        const int t = t0 + tid;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (t < nvec) x = __ldg(keys + t);
-        // chunks that have to be looked at whatever their keys
-        const uint32_t a0 = __vcmpeq2(x.x, 0xFFFFFFFFu), a1 = __vcmpeq2(x.y, 0xFFFFFFFFu);
-        const uint32_t a2 = __vcmpeq2(x.z, 0xFFFFFFFFu), a3 = __vcmpeq2(x.w, 0xFFFFFFFFu);
-        if (h >= 3) {
-            const uint32_t m = __vmaxu2(__vmaxu2(x.x & ~a0, x.y & ~a1), __vmaxu2(x.z & ~a2, x.w & ~a3));
-            uint32_t best = max(m & 0xFFFFu, m >> 16) | ((a0 | a1 | a2 | a3) ? kVisit : 0u);
-            for (int o = 1; o < 32 && o < (1 << gs); o <<= 1) {
-                const uint32_t other = __shfl_xor_sync(0xFFFFFFFFu, best, o);
-                best = max(best & 0xFFFFu, other & 0xFFFFu) | ((best | other) & kVisit);
-            }
-            if (t < nvec && (t & ((1 << min(gs, 5)) - 1)) == 0) {
-                // (a flag above the maximum hides it: lower, so still a bound)
-                if (gs <= 5) tops[t >> gs] = best;
-                else atomicMax(&tops[t >> gs], best & kVisit ? kVisit : best);
-            }
-        } else if (t < nvec) {
-            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-            uint32_t key[8];
+    // the largest key of every unit, four vectors in flight; thread t owns the units t, t + kT, ...
+    for (int t0 = tid; t0 < nvec; t0 += 4 * kT) {
+        uint4 x[4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                key[e] = (w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
-                if (key[e] == kAlways) key[e] = kVisit;
-            }
+        for (int e = 0; e < 4; ++e)
+            x[e] = t0 + e * kT < nvec ? __ldg(keys + t0 + e * kT) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if (h == 0) {
-                    tops[8 * t + e] = key[e];
-                } else if (h == 1 && (e & 1) == 0) {
-                    tops[4 * t + e / 2] = (max(key[e] & 0xFFFFu, key[e + 1] & 0xFFFFu)) | ((key[e] | key[e + 1]) & kVisit);
-                } else if (h == 2 && (e & 3) == 0) {
-                    uint32_t m = 0, f = 0;
-#pragma unroll
-                    for (int d = 0; d < 4; ++d) {
-                        m = max(m, key[(e & 4) + d] & 0xFFFFu);
-                        f |= key[(e & 4) + d] & kVisit;
-                    }
-                    tops[2 * t + e / 4] = m | f;
-                }
+        for (int e = 0; e < 4; ++e) {
+            const int t = t0 + e * kT;
+            if (t >= nvec) continue;
+            if (small) {
+                reinterpret_cast<uint4*>(tops)[t] = x[e];
+            } else {
+                const uint32_t m = __vmaxu2(__vmaxu2(x[e].x, x[e].y), __vmaxu2(x[e].z, x[e].w));
+                uint32_t best = max(m & 0xFFFFu, m >> 16);
+                if (t >= kUnits) best = max(best, (uint32_t)tops[t % kUnits]);
+                tops[t % kUnits] = (uint16_t)best;
             }
         }
     }
@@ -572,22 +534,31 @@ k_f4_pick(PickArgs p) {
         if (lane == 0) {
             s_err = fmaxf(e, 1e-37f);
             s_forced = f;
-            n_list = n_found = n_groups = 0;
+            n_list = n_found = n_units = 0;
         }
     }
     __syncthreads();
     const bool forced = s_forced != 0;
-    // L: the kp-th largest of the groups' keys, by bisection of its 16 bits (0: there are fewer)
-    const uint32_t mytop = tid < ngroups ? tops[tid] : 0u;
+    // a thread's units are a group: L is the kp-th largest of the groups' largest keys, by
+    // bisection of its 16 bits (0: there are fewer)
+    uint32_t top = 0;
+    for (int t = tid; t < nunits; t += kT) {
+        const uint32_t key = tops[t];
+        if (key != kAlways) top = max(top, key);
+    }
     uint32_t s_key = 0;
     for (uint32_t bit = 0x8000u; bit; bit >>= 1)
-        if (__syncthreads_count((mytop & 0xFFFFu) >= (s_key | bit)) >= kp) s_key |= bit;
+        if (__syncthreads_count(top >= (s_key | bit)) >= kp) s_key |= bit;
     const double err = (double)s_err;
     // the k-th value is at least this
     double floor_v = s_key > key_of(-__int_as_float(0x7f800000)) ? (double)key_floor(s_key) - err : kNegInf;
     // an accumulator, or an estimate, of the answer is at least floor - err
     auto bar_of = [&]() { return max(key_of(__double2float_rd(floor_v - err)), 1u); };
-    if (mytop >= bar_of()) glist[atomicAdd(&n_groups, 1)] = (uint16_t)tid;
+    {
+        const uint32_t bar = bar_of();
+        for (int t = tid; t < nunits; t += kT)
+            if (tops[t] >= bar) ulist[atomicAdd(&n_units, 1)] = (uint16_t)t;
+    }
     __syncthreads();
 
     // Evaluates what was found exactly, ranks it, keeps the best k at the front and raises the floor.
@@ -640,12 +611,30 @@ k_f4_pick(PickArgs p) {
             __syncthreads();  // everyone has read n_found before anyone adds to it
             const int c1 = min(n, c0 + room);
             const float least = 4.0f * __double2float_rd(floor_v - err);
+            // the next chunk's first 64 columns are loaded under this one's arithmetic
+            uint4 y0, y1;
+            uint32_t sc;
+            auto fetch = [&](int c) {
+                const int j = min((int)list[c] * 32 + lane, p.b.rows - 1);
+                y0 = __ldg(codes_of(j));
+                y1 = __ldg(codes_of(j) + 1);
+                sc = __ldg(reinterpret_cast<const uint32_t*>(scales_of(j)));
+            };
+            if (c0 + warp < c1) fetch(c0 + warp);
             for (int c = c0 + warp; c < c1; c += kT / 32) {
-                const long long j = (long long)list[c] * 32 + lane;
-                if (j < p.b.rows && j != self) {
-                    // without a bound on the terms fp32 could overflow: rank_found decides
-                    if (forced || f4_estimate<kNv>(qa, sa, codes_of((int)j), scales_of((int)j), steps) >= least) fj[atomicAdd(&n_found, 1)] = (int)j;
+                const int j = (int)list[c] * 32 + lane;
+                const uint4 z0 = y0, z1 = y1;
+                const uint32_t zs = sc;
+                if (c + kT / 32 < c1) fetch(c + kT / 32);
+                float v = f4_estimate64<kNv>(qa, sa, z0, z1, zs, 0.0f);
+                for (int st = 1; st < steps; ++st) {
+                    const int jc = min(j, p.b.rows - 1);
+                    const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(scales_of(jc) + (kNv ? st : st >> 1) * kF4Atom));
+                    v = f4_estimate64<kNv>(qa + 16 * st, sa + (kNv ? 4 : 2) * st, __ldg(codes_of(jc) + 2 * st),
+                                           __ldg(codes_of(jc) + 2 * st + 1), !kNv && (st & 1) ? w >> 16 : w, v);
                 }
+                // without a bound on the terms fp32 could overflow: rank_found decides
+                if (j < p.b.rows && j != self && (forced || v >= least)) fj[atomicAdd(&n_found, 1)] = j;
             }
             c0 = c1;
             if (c0 < n) rank_found();
@@ -654,28 +643,29 @@ k_f4_pick(PickArgs p) {
         if (tid == 0) n_list = 0;
         __syncthreads();
     };
-    // the groups' chunks that may hold a column of the answer
-    const int ng = n_groups;
-    constexpr int kScan = kT < 512 ? kT : 512;    // vectors a round
-    const long long ntask = (long long)ng << gs;  // a vector each
-    for (long long t0 = 0; t0 < ntask; t0 += kScan) {
+    // the units' chunks that may hold a column of the answer
+    const int per = small ? 1 : (nvec + kUnits - 1) / kUnits;  // vectors of a unit
+    const int ntask = n_units * per;
+    for (int t0 = 0; t0 < ntask; t0 += kScan) {
         const uint32_t bar = bar_of();
-        const long long t = t0 + tid;
+        const int t = t0 + tid;
         if (tid < kScan && t < ntask) {
-            const long long g = glist[t >> gs];
-            const long long vec = h < 3 ? (g << h) >> 3 : (g << gs) + (t & ((1 << gs) - 1));
+            const int unit = ulist[t / per];
+            const int vec = small ? unit >> 3 : unit + t % per * kUnits;
             if (vec < nvec) {
-                const uint4 x = __ldg(keys + vec);
-                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
                 // keys 8 vec ..: [8 tiles of b][half of 64 columns][parity of the tile][4 tiles][2]
-                const int oct = (int)(vec >> 2), half = (int)(vec >> 1) & 1, par = (int)vec & 1;
+                const int oct = vec >> 2, half = (vec >> 1) & 1, par = vec & 1;
+                const int chunk0 = (oct * kOct + par) * 4 + 2 * half;
+                if (small) {
+                    const int e = unit & 7;
+                    if (tops[unit] >= bar) list[atomicAdd(&n_list, 1)] = (uint32_t)(chunk0 + 8 * (e >> 1) + (e & 1));
+                } else {
+                    const uint4 x = __ldg(keys + vec);
+                    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const uint32_t key = (w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
-                    if (key >= bar && (h >= 3 || (int)((8 * vec + e) >> h) == (int)g)) {
-                        const int chunk = (oct * kOct + 2 * (e >> 1) + par) * 4 + 2 * half + (e & 1);
-                        list[atomicAdd(&n_list, 1)] = (uint32_t)chunk;
-                    }
+                    for (int e = 0; e < 8; ++e)
+                        if (((w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu) >= bar)
+                            list[atomicAdd(&n_list, 1)] = (uint32_t)(chunk0 + 8 * (e >> 1) + (e & 1));
                 }
             }
         }
@@ -776,8 +766,6 @@ cudaError_t f4_topk(const F4& a, const F4& b, int k, long long self, int* idx, f
         q.row0 = (int)r0;
         q.nerrs = grid;
         const int threads = rows <= 2 * sms ? 1024 : 256;
-        q.h = 0;
-        while (((plan.noct * kOctKeys - 1) >> q.h) + 1 > threads) ++q.h;
         if (threads == 1024) {
             if (b.nv) k_f4_pick<1, 1024><<<rows, 1024, 0, st>>>(q);
             else k_f4_pick<0, 1024><<<rows, 1024, 0, st>>>(q);
