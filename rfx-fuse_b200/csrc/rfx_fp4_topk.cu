@@ -29,9 +29,9 @@ namespace rfx {
 
 namespace {
 
-constexpr int kKThreads = 576;
-constexpr int kOct = 8;                      // tiles of b whose keys a lane keeps before it stores them
-constexpr int kOctKeys = 4 * kOct;           // keys of a row and 8 tiles
+constexpr int kKThreads = 448;
+constexpr int kSpan = 6;                     // tiles of b in a unit of work: two for each of three groups of warps
+constexpr int kSpanKeys = 4 * kSpan;         // keys of a row and a span
 constexpr float kEps = 1.0f / 32768.0f;
 constexpr uint32_t kAlways = 0xFFFFu;        // key of a chunk that has to be looked at (no float's)
 constexpr int kScan = 256;                   // units a round turns into chunks
@@ -43,8 +43,8 @@ struct KeysArgs {
     F4 a, b;
     int q0;               // first row tile of a in this batch
     int nq;               // row tiles of a in it
-    int ntiles, noct;     // tiles of b, and groups of 8
-    uint32_t* keys;       // [rows of the batch][noct][16] pairs of keys
+    int ntiles, nspan;     // tiles of b, and spans of them
+    uint32_t* keys;       // [rows of the batch][nspan][12] pairs of keys
     float* errs;          // [grid] largest err of a block's tiles; negative: some tiles have none
     int* err;
 };
@@ -54,7 +54,7 @@ struct PickArgs {
     int row0;             // first row of the batch
     int k;
     long long self;       // row of b that is row 0 of a and left out for it (and so on); -1: none
-    int noct;
+    int nspan;
     const uint32_t* keys;
     const float* errs;
     int nerrs;
@@ -79,11 +79,10 @@ constexpr int keys_stage(int nv, int cb) {
     return (2 * (128 * cb + (cb == 32 ? 1 : nv ? 4 : 2) * kF4Atom) + 1023) / 1024 * 1024;
 }
 
-// A CTA takes the units [u0, u1) of (row tile of a, 8 tiles of b), b fastest.
-//   warps 0-15 quarter warp & 3 of the rows, half warp >> 2 & 1 of the columns, every other tile
-//              (four warps a scheduler: with two, 0.36 instructions a cycle issued);
-//   warp 16    one thread loads: the row tile of a into one of two slots, b's tiles into a ring;
-//   warp 17    allocates TMEM, one thread copies scales to TMEM and multiplies into three
+// A CTA takes the units [u0, u1) of (row tile of a, span of b), b fastest.
+//   warps 0-11 quarter warp & 3 of the rows, every third tile, always of the same accumulator;
+//   warp 12    one thread loads: the row tile of a into one of two slots, b's tiles into a ring;
+//   warp 13    allocates TMEM, one thread copies scales to TMEM and multiplies into three
 //              accumulators of 128 columns.
 // Every wait is bounded; on expiry the CTA records it in *err, drains its copies, frees TMEM and
 // returns.
@@ -111,7 +110,7 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
     const uint32_t ring0 = slot0 + 2 * kSlot;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long long units = (long long)p.nq * p.noct;
+    const long long units = (long long)p.nq * p.nspan;
     const long long u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
 
     if (threadIdx.x == 0) {
@@ -121,7 +120,7 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
         }
         for (int b = 0; b < kAccs; ++b) {
             mbar_init(accf(b), 1);
-            mbar_init(acce(b), 8);  // one arrival a warp
+            mbar_init(acce(b), 4);  // one arrival a warp
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(afull(b), 1);
@@ -130,7 +129,7 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
         *abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 17) {
+    if (warp == 13) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                          smem_u32(tmem_slot)),
                      "r"(512)
@@ -144,15 +143,15 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
     const int steps = p.b.Kp / 64;
     const int atoms = kNv ? steps : (steps + 1) / 2;
 
-    if (warp == 16) {
+    if (warp == 12) {
         if (lane == 0) {
             const uint32_t sfb = (uint32_t)(atoms * kF4Atom);
             int n = 0, na = 0;
             RingPos st, sl;
             bool ok = true;
-            int qt = p.q0 + (int)(u0 / p.noct), oct = (int)(u0 % p.noct);
+            int qt = p.q0 + (int)(u0 / p.nspan), span = (int)(u0 % p.nspan);
             for (long long u = u0; ok && u < u1; ++u) {
-                if (u == u0 || oct == 0) {
+                if (u == u0 || span == 0) {
                     if (!mbar_wait_fast(aempty(sl.slot), sl.parity ^ 1u, abort)) {
                         ok = false;
                         break;
@@ -164,8 +163,8 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
                     sl.next(2);
                     ++na;
                 }
-                const int te = min(p.ntiles, oct * kOct + kOct);
-                for (int t = oct * kOct; t < te; t += 2, ++n) {
+                const int te = min(p.ntiles, span * kSpan + kSpan);
+                for (int t = span * kSpan; t < te; t += 2, ++n) {
                     if (!mbar_wait_fast(empty(st.slot), st.parity ^ 1u, abort)) {
                         ok = false;
                         break;
@@ -177,8 +176,8 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
                     bulk_load(dst + 2 * kBox, p.b.scales + (long long)t * p.b.natoms * kF4Atom, sc, full(st.slot));
                     st.next(kStages);
                 }
-                if (++oct == p.noct) {
-                    oct = 0;
+                if (++span == p.nspan) {
+                    span = 0;
                     ++qt;
                 }
             }
@@ -192,17 +191,17 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
                 mbar_wait<false>(full(i % kStages), (uint32_t)(i / kStages) & 1u, nullptr);
         }
         __syncwarp();
-    } else if (warp == 17) {
+    } else if (warp == 13) {
         if (lane == 0) {
-            RingPos st, sl, ac;
+            RingPos st, sl;
+            uint32_t uses = 0;  // a parity bit for every accumulator
             int last = -1;
-            uint32_t last_parity = 0;
             bool ok = true;
             uint32_t tsa = 0;
             uint64_t da = 0;
-            int oct = (int)(u0 % p.noct);
+            int span = (int)(u0 % p.nspan);
             for (long long u = u0; ok && u < u1; ++u) {
-                if (u == u0 || oct == 0) {
+                if (u == u0 || span == 0) {
                     if (!mbar_wait_fast(afull(sl.slot), sl.parity, abort)) {
                         ok = false;
                         break;
@@ -213,8 +212,8 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
                     for (int k0 = 0; k0 < atoms; ++k0) f4_copy_atom(tsa + 4 * k0, f4_atom_desc(src + kBox + k0 * kF4Atom));
                     da = f4_operand_desc<kCB>(src);
                 }
-                const int te = min(p.ntiles, oct * kOct + kOct);
-                for (int t = oct * kOct; ok && t < te; t += 2) {
+                const int te = min(p.ntiles, span * kSpan + kSpan);
+                for (int t = span * kSpan; ok && t < te; t += 2) {
                     if (!mbar_wait_fast(full(st.slot), st.parity, abort)) {
                         ok = false;
                         break;
@@ -234,12 +233,13 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
                         } else {
                             for (int k0 = 0; k0 < atoms; ++k0) f4_copy_atom(tsh + 4 * k0, dsc + k0 * (kF4Atom >> 4));
                         }
-                        if (!mbar_wait_fast(acce(ac.slot), ac.parity ^ 1u, abort)) {
+                        const int ac = (t + h - span * kSpan) % kAccs;
+                        if (!mbar_wait_fast(acce(ac), ((uses >> ac) & 1u) ^ 1u, abort)) {
                             ok = false;
                             break;
                         }
                         tc_fence_after();
-                        const uint32_t d = tmem + (uint32_t)(128 * ac.slot);
+                        const uint32_t d = tmem + (uint32_t)(128 * ac);
                         if (kCB == 32) {
                             f4_mma<kNv>(d, da, db, f4_idesc<kNv>(128, 0), tsa, tsh, 0u);
                         } else {
@@ -249,16 +249,15 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
                                             tsa + 4 * at, tsh + 4 * at, k0 ? 1u : 0u);
                             }
                         }
-                        mma_commit(accf(ac.slot));
-                        last = ac.slot;
-                        last_parity = ac.parity;
-                        ac.next(kAccs);
+                        mma_commit(accf(ac));
+                        last = ac;
+                        uses ^= 1u << ac;
                     }
                     if (ok) mma_commit(empty(st.slot));
                     st.next(kStages);
                 }
-                if (++oct == p.noct) oct = 0;
-                if (ok && (oct == 0 || u == u1 - 1)) {
+                if (++span == p.nspan) span = 0;
+                if (ok && (span == 0 || u == u1 - 1)) {
                     mma_commit(aempty(sl.slot));
                     sl.next(2);
                 }
@@ -268,98 +267,100 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
                 *abort = 1;
             }
             // the last products must finish before the accumulators are freed
-            if (last >= 0) mbar_wait<false>(accf(last), last_parity, nullptr);
+            if (last >= 0) mbar_wait<false>(accf(last), ((uses >> last) & 1u) ^ 1u, nullptr);
         }
         __syncwarp();
     } else {
-        const int quarter = warp & 3, half = (warp >> 2) & 1, par = warp >> 3;
-        const uint32_t lane_addr = tmem + ((uint32_t)(32 * quarter) << 16) + (uint32_t)(64 * half);
+        const int quarter = warp & 3, phase = warp >> 2;
+        const uint32_t lane_addr = tmem + ((uint32_t)(32 * quarter) << 16) + (uint32_t)(128 * phase);
         const float kNegInf = -__int_as_float(0x7f800000);
         float worst = 0.0f;  // largest bound of this block's tiles that the filter can use
         bool some_forced = false;
-        uint32_t n = (uint32_t)par;  // this warp's next tile in the CTA's sequence
+        uint32_t parity = 0;
         bool ok = true;
-        int qt = p.q0 + (int)(u0 / p.noct), oct = (int)(u0 % p.noct);
-        float bd = lane < min(kOct, p.ntiles - oct * kOct) ? __ldg(p.b.bounds + oct * kOct + lane) : 0.0f;
+        int qt = p.q0 + (int)(u0 / p.nspan), span = (int)(u0 % p.nspan);
+        float bd = lane < min(kSpan, p.ntiles - span * kSpan) ? __ldg(p.b.bounds + span * kSpan + lane) : 0.0f;
         float bq = u0 < u1 ? __ldg(p.a.bounds + qt) : 0.0f;
         for (long long u = u0; ok && u < u1; ++u) {
             const long long row = (long long)qt * 128 + 32 * quarter + lane;
             const bool any = (long long)qt * 128 + 32 * quarter < p.a.rows;  // of this warp's rows
-            const int nt = min(kOct, p.ntiles - oct * kOct);
+            const int nt = min(kSpan, p.ntiles - span * kSpan);
             // a sum of such terms can overflow fp32 and lose its sign: those tiles are looked at
             const uint32_t forced = __ballot_sync(0xFFFFFFFFu, !(bq * bd * kEps < 1e30f));
             if (forced) some_forced = true;
             if (!((forced >> lane) & 1u)) worst = fmaxf(worst, bq * bd * (kEps * 1.000001f));
-            const int ncols = min(kOct * 128, p.b.rows - oct * kOct * 128) - 64 * half;  // columns that exist
-            uint32_t* out = p.keys + ((row - (long long)p.q0 * 128) * p.noct + oct) * (kOctKeys / 2) + 8 * half + 4 * par;
+            const int ncols = min(kSpan * 128, p.b.rows - span * kSpan * 128);  // columns that exist
+            const bool plain = forced == 0 && ncols == kSpan * 128;
+            uint32_t* out = p.keys + ((row - (long long)p.q0 * 128) * p.nspan + span) * (kSpanKeys / 2) + 4 * phase;
             // the next unit's bounds, under this one's work
-            int oct1 = oct + 1, qt1 = qt;
-            if (oct1 == p.noct) {
-                oct1 = 0;
+            int span1 = span + 1, qt1 = qt;
+            if (span1 == p.nspan) {
+                span1 = 0;
                 ++qt1;
             }
             if (u + 1 < u1) {
-                bd = lane < min(kOct, p.ntiles - oct1 * kOct) ? __ldg(p.b.bounds + oct1 * kOct + lane) : 0.0f;
+                bd = lane < min(kSpan, p.ntiles - span1 * kSpan) ? __ldg(p.b.bounds + span1 * kSpan + lane) : 0.0f;
                 bq = __ldg(p.a.bounds + qt1);
             }
-            uint32_t keys[kOct / 2];
+            uint32_t keys[4] = {0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < kOct / 2; ++i) {
-                keys[i] = 0;
-                const int t = 2 * i + par;
+            for (int i = 0; i < kSpan / kAccs; ++i) {
+                const int t = kAccs * i + phase;
                 if (t >= nt || !ok) continue;
-                const uint32_t slot = n % kAccs;
-                const bool got = mbar_wait_fast(accf(slot), (n / kAccs) & 1u, abort);
-                n += 2;
+                const bool got = mbar_wait_fast(accf(phase), parity, abort);
+                parity ^= 1u;
                 if (!__all_sync(0xFFFFFFFFu, got)) {
                     ok = false;
                     continue;
                 }
-                uint32_t r[2][32];
                 if (any) {
+                    // 32 columns are read while the maximum of the 32 before is taken
+                    uint32_t r[2][32];
                     tc_fence_after();
+                    tmem_ld32_issue(lane_addr, r[0]);
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) tmem_ld32_issue(lane_addr + 128 * slot + 32 * c, r[c]);
-                    tmem_wait();
+                    for (int c = 0; c < 4; ++c) {
+                        tmem_wait();
+                        tmem_pin32(r[c & 1]);
+                        if (c < 3) {
+                            tmem_ld32_issue(lane_addr + 32 * (c + 1), r[(c + 1) & 1]);
+                        } else {
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(acce(phase));
+                        }
+                        uint32_t* x = r[c & 1];
+                        const int ncol = ncols - 128 * t - 32 * c;
+                        if (!plain && ncol < 32) {
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) tmem_pin32(r[c]);
-                    tc_fence_before();
-                    __syncwarp();
-                }
-                if (lane == 0) mbar_arrive(acce(slot));
-                if (!any) continue;
-                const int ncol = ncols - 128 * t;
-                uint32_t pair = 0;
+                            for (int e = 0; e < 32; ++e)
+                                if (e >= ncol) x[e] = __float_as_uint(kNegInf);
+                        }
+                        float m[4];
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t* x = r[c];
-                    if (ncol < 64) {
+                        for (int e = 0; e < 4; ++e) m[e] = __uint_as_float(x[e]);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (32 * c + e >= ncol) x[e] = __float_as_uint(kNegInf);
+                        for (int e = 4; e < 28; e += 8) {
+#pragma unroll
+                            for (int f = 0; f < 4; ++f)
+                                m[f] = fmax3(m[f], __uint_as_float(x[e + 2 * f]), __uint_as_float(x[e + 2 * f + 1]));
+                        }
+                        m[0] = fmax3(m[0], __uint_as_float(x[28]), __uint_as_float(x[29]));
+                        m[1] = fmax3(m[1], __uint_as_float(x[30]), __uint_as_float(x[31]));
+                        const float top = fmaxf(fmax3(m[0], m[1], m[2]), m[3]);
+                        uint32_t key = top == top ? key_of(top) : 0u;  // NaN alone: nobody's neighbours
+                        if (!plain) {
+                            if ((forced >> t) & 1u) key = kAlways;
+                            if (ncol <= 0) key = 0;
+                        }
+                        keys[2 * i + (c >> 1)] |= key << (16 * (c & 1));
                     }
-                    float m[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) m[e] = __uint_as_float(x[e]);
-#pragma unroll
-                    for (int e = 4; e < 28; e += 8) {
-#pragma unroll
-                        for (int f = 0; f < 4; ++f)
-                            m[f] = fmax3(m[f], __uint_as_float(x[e + 2 * f]), __uint_as_float(x[e + 2 * f + 1]));
-                    }
-                    m[0] = fmax3(m[0], __uint_as_float(x[28]), __uint_as_float(x[29]));
-                    m[1] = fmax3(m[1], __uint_as_float(x[30]), __uint_as_float(x[31]));
-                    const float top = fmaxf(fmax3(m[0], m[1], m[2]), m[3]);
-                    uint32_t key = top == top ? key_of(top) : 0u;  // NaN alone: nobody's neighbours
-                    if ((forced >> t) & 1u) key = kAlways;
-                    if (ncol <= 32 * c) key = 0;
-                    pair |= key << (16 * c);
+                } else if (lane == 0) {
+                    mbar_arrive(acce(phase));
                 }
-                keys[i] = pair;
             }
             if (ok && row < p.a.rows) *reinterpret_cast<uint4*>(out) = make_uint4(keys[0], keys[1], keys[2], keys[3]);
-            n += (uint32_t)nt - 2u * (uint32_t)((nt - par + 1) / 2);  // to its first tile of the next unit
-            oct = oct1;
+            span = span1;
             qt = qt1;
         }
         if (!ok && lane == 0) {
@@ -373,7 +374,7 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 17) {
+    if (warp == 13) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512)
                      : "memory");
@@ -479,8 +480,8 @@ k_f4_pick(PickArgs p) {
     const long long i = (long long)p.row0 + blockIdx.x;
     const int kp = p.self >= 0 ? p.k + 1 : p.k;  // the row itself may be one of the k columns
     const int self = p.self >= 0 ? (int)(p.self + i) : -1;
-    const uint4* keys = reinterpret_cast<const uint4*>(p.keys + (long long)blockIdx.x * p.noct * (kOctKeys / 2));
-    const int nvec = p.noct * (kOctKeys / 8);    // 8 keys each
+    const uint4* keys = reinterpret_cast<const uint4*>(p.keys + (long long)blockIdx.x * p.nspan * (kSpanKeys / 2));
+    const int nvec = p.nspan * (kSpanKeys / 8);    // 8 keys each
     const uint8_t* b_codes = p.b.codes;
     const uint8_t* b_scales = p.b.scales;
     const int pitch = p.b.pitch(), tile_bytes = p.b.natoms * kF4Atom, steps = p.b.Kp / 64;
@@ -653,19 +654,18 @@ k_f4_pick(PickArgs p) {
             const int unit = ulist[t / per];
             const int vec = small ? unit >> 3 : unit + t % per * kUnits;
             if (vec < nvec) {
-                // keys 8 vec ..: [8 tiles of b][half of 64 columns][parity of the tile][4 tiles][2]
-                const int oct = vec >> 2, half = (vec >> 1) & 1, par = vec & 1;
-                const int chunk0 = (oct * kOct + par) * 4 + 2 * half;
+                // keys 8 vec ..: [span][tile % 3][tile / 3][4 chunks of the tile]
+                const int chunk0 = (vec / kAccs * kSpan + vec % kAccs) * 4;
                 if (small) {
                     const int e = unit & 7;
-                    if (tops[unit] >= bar) list[atomicAdd(&n_list, 1)] = (uint32_t)(chunk0 + 8 * (e >> 1) + (e & 1));
+                    if (tops[unit] >= bar) list[atomicAdd(&n_list, 1)] = (uint32_t)(chunk0 + 4 * kAccs * (e >> 2) + (e & 3));
                 } else {
                     const uint4 x = __ldg(keys + vec);
                     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
                         if (((w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu) >= bar)
-                            list[atomicAdd(&n_list, 1)] = (uint32_t)(chunk0 + 8 * (e >> 1) + (e & 1));
+                            list[atomicAdd(&n_list, 1)] = (uint32_t)(chunk0 + 4 * kAccs * (e >> 2) + (e & 3));
                 }
             }
         }
@@ -694,13 +694,13 @@ __global__ void k_f4_topk_none(long long n, int* idx, float* val) {
 // Rows of a whose keys are made before they are read.
 constexpr long long kKeyMB = 256;
 struct TopkPlan {
-    int noct, rows;
+    int nspan, rows;
     long long key_bytes;
 };
 TopkPlan topk_plan(const F4& a, const F4& b) {
     TopkPlan t;
-    t.noct = (b.tiles() + kOct - 1) / kOct;
-    const long long row = (long long)t.noct * kOctKeys * 2;
+    t.nspan = (b.tiles() + kSpan - 1) / kSpan;
+    const long long row = (long long)t.nspan * kSpanKeys * 2;
     const long long tiles = std::max(1ll, (kKeyMB << 20) / (row * 128));
     t.rows = (int)std::min<long long>(a.rows, tiles * 128);
     t.key_bytes = (row * t.rows + 255) / 256 * 256;
@@ -740,7 +740,7 @@ cudaError_t f4_topk(const F4& a, const F4& b, int k, long long self, int* idx, f
     p.a = a;
     p.b = b;
     p.ntiles = b.tiles();
-    p.noct = plan.noct;
+    p.nspan = plan.nspan;
     p.keys = (uint32_t*)ws;
     p.errs = (float*)((uint8_t*)ws + plan.key_bytes);
     p.err = err;
@@ -749,7 +749,7 @@ cudaError_t f4_topk(const F4& a, const F4& b, int k, long long self, int* idx, f
     q.b = b;
     q.k = k;
     q.self = self;
-    q.noct = plan.noct;
+    q.nspan = plan.nspan;
     q.keys = p.keys;
     q.errs = p.errs;
     q.idx = idx;
@@ -758,7 +758,7 @@ cudaError_t f4_topk(const F4& a, const F4& b, int k, long long self, int* idx, f
         const int rows = (int)std::min<long long>(plan.rows, a.rows - r0);
         p.q0 = (int)(r0 / 128);
         p.nq = (rows + 127) / 128;
-        const int grid = (int)std::min<long long>((long long)p.nq * p.noct, sms);
+        const int grid = (int)std::min<long long>((long long)p.nq * p.nspan, sms);
         cudaError_t e;
         if (cb == 32) e = b.nv ? launch_keys<1, 32>(ta, tb, p, grid, st) : launch_keys<0, 32>(ta, tb, p, grid, st);
         else e = b.nv ? launch_keys<1, 128>(ta, tb, p, grid, st) : launch_keys<0, 128>(ta, tb, p, grid, st);
