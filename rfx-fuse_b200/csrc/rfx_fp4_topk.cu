@@ -316,6 +316,7 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
                 if (any) {
                     // 32 columns are read while the maximum of the 32 before is taken
                     uint32_t r[2][32];
+                    float top[4];
                     tc_fence_after();
                     tmem_ld32_issue(lane_addr, r[0]);
 #pragma unroll
@@ -330,8 +331,8 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
                             if (lane == 0) mbar_arrive(acce(phase));
                         }
                         uint32_t* x = r[c & 1];
-                        const int ncol = ncols - 128 * t - 32 * c;
-                        if (!plain && ncol < 32) {
+                        if (!plain) {
+                            const int ncol = ncols - 128 * t - 32 * c;
 #pragma unroll
                             for (int e = 0; e < 32; ++e)
                                 if (e >= ncol) x[e] = __float_as_uint(kNegInf);
@@ -347,13 +348,23 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
                         }
                         m[0] = fmax3(m[0], __uint_as_float(x[28]), __uint_as_float(x[29]));
                         m[1] = fmax3(m[1], __uint_as_float(x[30]), __uint_as_float(x[31]));
-                        const float top = fmaxf(fmax3(m[0], m[1], m[2]), m[3]);
-                        uint32_t key = top == top ? key_of(top) : 0u;  // NaN alone: nobody's neighbours
+                        // NaN alone becomes -inf: nobody's neighbours
+                        top[c] = fmax3(fmax3(m[0], m[1], m[2]), m[3], kNegInf);
+                    }
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        // key_of both: the upper halves, all bits flipped under a sign, else the sign
+                        uint32_t pair = __byte_perm(__float_as_uint(top[2 * c]), __float_as_uint(top[2 * c + 1]), 0x7632);
+                        uint32_t neg;
+                        asm("prmt.b32 %0, %1, %2, %3;" : "=r"(neg) : "r"(pair), "r"(0u), "r"(0xBB99u));
+                        pair ^= neg | 0x80008000u;
                         if (!plain) {
-                            if ((forced >> t) & 1u) key = kAlways;
-                            if (ncol <= 0) key = 0;
+                            const int ncol = ncols - 128 * t - 64 * c;
+                            if ((forced >> t) & 1u) pair = kAlways << 16 | kAlways;
+                            if (ncol <= 32) pair &= 0xFFFFu;
+                            if (ncol <= 0) pair = 0;
                         }
-                        keys[2 * i + (c >> 1)] |= key << (16 * (c & 1));
+                        keys[2 * i + c] = pair;
                     }
                 } else if (lane == 0) {
                     mbar_arrive(acce(phase));
