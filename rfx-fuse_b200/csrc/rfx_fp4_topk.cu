@@ -109,9 +109,10 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
     const uint32_t slot0 = bar0 + 1024u;
     const uint32_t ring0 = slot0 + 2 * kSlot;
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const long long units = (long long)p.nq * p.nspan;
-    const long long u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
+    const long long u0 = units * blockIdx.x / gridDim.x;
+    const int nu = (int)(units * (blockIdx.x + 1) / gridDim.x - u0);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
@@ -139,110 +140,101 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
     const int steps = p.b.Kp / 64;
     const int atoms = kNv ? steps : (steps + 1) / 2;
 
     if (warp == 12) {
-        if (lane == 0) {
-            const uint32_t sfb = (uint32_t)(atoms * kF4Atom);
-            int n = 0, na = 0;
-            RingPos st, sl;
-            bool ok = true;
-            int qt = p.q0 + (int)(u0 / p.nspan), span = (int)(u0 % p.nspan);
-            for (long long u = u0; ok && u < u1; ++u) {
-                if (u == u0 || span == 0) {
-                    if (!mbar_wait_fast(aempty(sl.slot), sl.parity ^ 1u, abort)) {
-                        ok = false;
-                        break;
-                    }
+        const uint32_t sfb = (uint32_t)(atoms * kF4Atom);
+        int n = 0, na = 0;
+        RingPos st, sl;
+        bool ok = true;
+        int qt = p.q0 + (int)(u0 / p.nspan), span = (int)(u0 % p.nspan);
+        for (int u = 0; ok && u < nu; ++u) {
+            if (u == 0 || span == 0) {
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(aempty(sl.slot), sl.parity ^ 1u, abort));
+                if (!ok) break;
+                if (elect_one()) {
                     const uint32_t dst = slot0 + (uint32_t)(sl.slot * kSlot);
                     mbar_expect_tx(afull(sl.slot), (uint32_t)kBox + sfb);
                     tma_load(dst, &tma, 0, qt * 128, afull(sl.slot));
                     bulk_load(dst + kBox, p.a.scales + (long long)qt * p.a.natoms * kF4Atom, sfb, afull(sl.slot));
-                    sl.next(2);
-                    ++na;
                 }
-                const int te = min(p.ntiles, span * kSpan + kSpan);
-                for (int t = span * kSpan; t < te; t += 2, ++n) {
-                    if (!mbar_wait_fast(empty(st.slot), st.parity ^ 1u, abort)) {
-                        ok = false;
-                        break;
-                    }
+                sl.next(2);
+                ++na;
+            }
+            const int te = min(p.ntiles, span * kSpan + kSpan);
+            for (int t = span * kSpan; t < te; t += 2, ++n) {
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(empty(st.slot), st.parity ^ 1u, abort));
+                if (!ok) break;
+                if (elect_one()) {
                     const uint32_t dst = ring0 + (uint32_t)(st.slot * kStage);
                     const uint32_t sc = t + 1 < te ? 2 * sfb : sfb;  // two tiles' scales follow one another
                     mbar_expect_tx(full(st.slot), 2u * kBox + sc);
                     tma_load(dst, &tmb, 0, t * 128, full(st.slot));
                     bulk_load(dst + 2 * kBox, p.b.scales + (long long)t * p.b.natoms * kF4Atom, sc, full(st.slot));
-                    st.next(kStages);
                 }
-                if (++span == p.nspan) {
-                    span = 0;
-                    ++qt;
-                }
+                st.next(kStages);
             }
-            if (!ok) {
-                if (!*abort) atomicExch(p.err, 1);
-                *abort = 1;
+            if (++span == p.nspan) {
+                span = 0;
+                ++qt;
             }
-            // drain this thread's copies still in flight
-            for (int i = na > 2 ? na - 2 : 0; i < na; ++i) mbar_wait<false>(afull(i & 1), (uint32_t)(i >> 1) & 1u, nullptr);
-            for (int i = n > kStages ? n - kStages : 0; i < n; ++i)
-                mbar_wait<false>(full(i % kStages), (uint32_t)(i / kStages) & 1u, nullptr);
         }
+        if (!ok && lane == 0) {
+            if (!*abort) atomicExch(p.err, 1);
+            *abort = 1;
+        }
+        // drain this warp's copies still in flight
+        for (int i = na > 2 ? na - 2 : 0; i < na; ++i) mbar_wait<false>(afull(i & 1), (uint32_t)(i >> 1) & 1u, nullptr);
+        for (int i = n > kStages ? n - kStages : 0; i < n; ++i)
+            mbar_wait<false>(full(i % kStages), (uint32_t)(i / kStages) & 1u, nullptr);
         __syncwarp();
     } else if (warp == 13) {
-        if (lane == 0) {
-            RingPos st, sl;
-            uint32_t uses = 0;  // a parity bit for every accumulator
-            int last = -1;
-            bool ok = true;
-            uint32_t tsa = 0;
-            uint64_t da = 0;
-            int span = (int)(u0 % p.nspan);
-            for (long long u = u0; ok && u < u1; ++u) {
-                if (u == u0 || span == 0) {
-                    if (!mbar_wait_fast(afull(sl.slot), sl.parity, abort)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint32_t src = slot0 + (uint32_t)(sl.slot * kSlot);
-                    tsa = tmem + 384u + (uint32_t)(4 * kAtoms * sl.slot);
+        RingPos st, sl;
+        uint32_t uses = 0;  // a parity bit for every accumulator
+        int last = -1;
+        bool ok = true;
+        uint32_t tsa = 0;
+        uint64_t da = 0;
+        int span = (int)(u0 % p.nspan);
+        for (int u = 0; ok && u < nu; ++u) {
+            if (u == 0 || span == 0) {
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(afull(sl.slot), sl.parity, abort));
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t src = slot0 + (uint32_t)(sl.slot * kSlot);
+                tsa = tmem + 384u + (uint32_t)(4 * kAtoms * sl.slot);
+                if (elect_one())
                     for (int k0 = 0; k0 < atoms; ++k0) f4_copy_atom(tsa + 4 * k0, f4_atom_desc(src + kBox + k0 * kF4Atom));
-                    da = f4_operand_desc<kCB>(src);
-                }
-                const int te = min(p.ntiles, span * kSpan + kSpan);
-                for (int t = span * kSpan; ok && t < te; t += 2) {
-                    if (!mbar_wait_fast(full(st.slot), st.parity, abort)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint32_t src = ring0 + (uint32_t)(st.slot * kStage);
-                    const uint32_t tsb = tmem + 384u + (uint32_t)(8 * kAtoms * (1 + st.slot));
-                    const int nt = min(2, te - t);
+                da = f4_operand_desc<kCB>(src);
+            }
+            const int nt = min(kSpan, p.ntiles - span * kSpan);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (h == nt) break;
-                        const uint32_t tsh = tsb + 4 * kAtoms * h;
-                        const uint64_t dsc = f4_atom_desc(src + 2 * kBox + h * atoms * kF4Atom);
-                        const uint64_t db = f4_operand_desc<kCB>(src + h * kBox);
+            for (int t = 0; t < kSpan; t += 2) {
+                if (t >= nt || !ok) break;
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(full(st.slot), st.parity, abort));
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t src = ring0 + (uint32_t)(st.slot * kStage);
+                const uint32_t tsb = tmem + 384u + (uint32_t)(8 * kAtoms * (1 + st.slot));
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (t + h >= nt) break;
+                    const int ac = (t + h) % kAccs;
+                    const uint32_t tsh = tsb + 4 * kAtoms * h;
+                    const uint64_t dsc = f4_atom_desc(src + 2 * kBox + h * atoms * kF4Atom);
+                    const uint64_t db = f4_operand_desc<kCB>(src + h * kBox);
+                    ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(acce(ac), ((uses >> ac) & 1u) ^ 1u, abort));
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t d = tmem + (uint32_t)(128 * ac);
+                    if (elect_one()) {
                         if (kCB == 32) {
                             f4_copy_atom(tsh, dsc);
-                        } else {
-                            for (int k0 = 0; k0 < atoms; ++k0) f4_copy_atom(tsh + 4 * k0, dsc + k0 * (kF4Atom >> 4));
-                        }
-                        const int ac = (t + h - span * kSpan) % kAccs;
-                        if (!mbar_wait_fast(acce(ac), ((uses >> ac) & 1u) ^ 1u, abort)) {
-                            ok = false;
-                            break;
-                        }
-                        tc_fence_after();
-                        const uint32_t d = tmem + (uint32_t)(128 * ac);
-                        if (kCB == 32) {
                             f4_mma<kNv>(d, da, db, f4_idesc<kNv>(128, 0), tsa, tsh, 0u);
                         } else {
+                            for (int k0 = 0; k0 < atoms; ++k0) f4_copy_atom(tsh + 4 * k0, dsc + k0 * (kF4Atom >> 4));
                             for (int k0 = 0; k0 < steps; ++k0) {
                                 const int at = kNv ? k0 : k0 >> 1;
                                 f4_mma<kNv>(d, da + 2 * k0, db + 2 * k0, f4_idesc<kNv>(128, kNv ? 0 : k0 & 1),
@@ -250,25 +242,25 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
                             }
                         }
                         mma_commit(accf(ac));
-                        last = ac;
-                        uses ^= 1u << ac;
+                        if (h == 1 || t + 1 >= nt) mma_commit(empty(st.slot));
                     }
-                    if (ok) mma_commit(empty(st.slot));
-                    st.next(kStages);
+                    last = ac;
+                    uses ^= 1u << ac;
                 }
-                if (++span == p.nspan) span = 0;
-                if (ok && (span == 0 || u == u1 - 1)) {
-                    mma_commit(aempty(sl.slot));
-                    sl.next(2);
-                }
+                st.next(kStages);
             }
-            if (!ok) {
-                if (!*abort) atomicExch(p.err, 2);
-                *abort = 1;
+            if (++span == p.nspan) span = 0;
+            if (ok && (span == 0 || u == nu - 1)) {
+                if (elect_one()) mma_commit(aempty(sl.slot));
+                sl.next(2);
             }
-            // the last products must finish before the accumulators are freed
-            if (last >= 0) mbar_wait<false>(accf(last), ((uses >> last) & 1u) ^ 1u, nullptr);
         }
+        if (!ok && lane == 0) {
+            if (!*abort) atomicExch(p.err, 2);
+            *abort = 1;
+        }
+        // the last products must finish before the accumulators are freed
+        if (last >= 0) mbar_wait<false>(accf(last), ((uses >> last) & 1u) ^ 1u, nullptr);
         __syncwarp();
     } else {
         const int quarter = warp & 3, phase = warp >> 2;
@@ -280,8 +272,8 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
         bool ok = true;
         int qt = p.q0 + (int)(u0 / p.nspan), span = (int)(u0 % p.nspan);
         float bd = lane < min(kSpan, p.ntiles - span * kSpan) ? __ldg(p.b.bounds + span * kSpan + lane) : 0.0f;
-        float bq = u0 < u1 ? __ldg(p.a.bounds + qt) : 0.0f;
-        for (long long u = u0; ok && u < u1; ++u) {
+        float bq = nu > 0 ? __ldg(p.a.bounds + qt) : 0.0f;
+        for (int u = 0; ok && u < nu; ++u) {
             const long long row = (long long)qt * 128 + 32 * quarter + lane;
             const bool any = (long long)qt * 128 + 32 * quarter < p.a.rows;  // of this warp's rows
             const int nt = min(kSpan, p.ntiles - span * kSpan);
@@ -298,7 +290,7 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
                 span1 = 0;
                 ++qt1;
             }
-            if (u + 1 < u1) {
+            if (u + 1 < nu) {
                 bd = lane < min(kSpan, p.ntiles - span1 * kSpan) ? __ldg(p.b.bounds + span1 * kSpan + lane) : 0.0f;
                 bq = __ldg(p.a.bounds + qt1);
             }

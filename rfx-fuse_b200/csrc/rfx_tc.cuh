@@ -78,6 +78,19 @@ __device__ __forceinline__ bool mbar_wait_fast(uint32_t bar, uint32_t parity, vo
     return mbar_try<false>(bar, parity) || mbar_wait_slow(bar, parity, abort);
 }
 
+// True in one lane of a converged warp.  The single-issuer roles run their loops in the whole warp
+// and issue under this predicate: addresses and descriptors then stay in uniform registers, which
+// the TMA and tcgen05 instructions take (a loop inside one lane moves each of them there first).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xFFFFFFFF;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(p));
+    return p != 0;
+}
+
 // A position in a ring of n slots: its slot and the parity of the round.
 struct RingPos {
     int slot = 0;
