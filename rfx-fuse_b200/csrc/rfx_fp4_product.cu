@@ -11,9 +11,9 @@
 //              accumulators form a ring and the two groups of four warps take alternate tiles;
 //              with more, both take the one accumulator, half the columns each, and release it as
 //              soon as it is in registers, so the next tile's products run under the stores;
-//   warp 8     one thread loads code rows by TMA and scale atoms by bulk copies into a ring of
+//   warp 8     loads code rows by TMA and scale atoms by bulk copies into a ring of
 //              chunks of 256 columns (64 when the matrix has no more);
-//   warp 9     allocates TMEM; one thread copies the chunk's atoms to TMEM (its columns belong to
+//   warp 9     allocates TMEM; copies the chunk's atoms to TMEM (its columns belong to
 //              the ring stage, so a stage's "empty" barrier also frees them) and multiplies.
 // Every wait is bounded; on expiry the CTA records it in *err, drains its copies, frees TMEM and
 // returns.
@@ -51,7 +51,7 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
     const uint32_t off_sb = off_b + (uint32_t)((p.bn * kCB + 1023) / 1024 * 1024);  // scales of b, then of a
     const uint32_t off_sa = off_sb + kAtoms * kF4Atom;
     const int ntiles = p.njt * p.nit;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.nstage; ++s) {
@@ -75,30 +75,26 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
 
     if (warp == 8) {
-        if (lane == 0) {
-            int step = 0;
-            RingPos st;
-            bool ok = true;
-            for (int t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
-                const int jt = t % p.njt, i0 = t / p.njt * p.bn;
-                const int rt0 = i0 / kF4Tile;
-                const int rts = min(nrt, p.a.tiles() - rt0);
-                const uint8_t* sb = p.b.scales + (long long)jt * p.b.natoms * kF4Atom;
-                const uint8_t* sa = p.a.scales + (long long)rt0 * p.a.natoms * kF4Atom;
-                int left = p.b.Kp / 64;  // steps to go
-                for (int c = 0; c < p.nchunk; ++c, ++step) {
-                    if (!mbar_wait_fast(empty(st.slot), st.parity ^ 1u, abort)) {
-                        if (!*abort) atomicExch(p.err, 1);
-                        *abort = 1;
-                        ok = false;
-                        break;
-                    }
+        int step = 0;
+        RingPos st;
+        bool ok = true;
+        for (int t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
+            const int jt = t % p.njt, i0 = t / p.njt * p.bn;
+            const int rt0 = i0 / kF4Tile;
+            const int rts = min(nrt, p.a.tiles() - rt0);
+            const uint8_t* sb = p.b.scales + (long long)jt * p.b.natoms * kF4Atom;
+            const uint8_t* sa = p.a.scales + (long long)rt0 * p.a.natoms * kF4Atom;
+            int left = p.b.Kp / 64;  // steps to go
+            for (int c = 0; c < p.nchunk; ++c, ++step) {
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(empty(st.slot), st.parity ^ 1u, abort));
+                if (!ok) break;
+                const int steps = min(left, kCB / 32);
+                left -= steps;
+                if (elect_one()) {
                     const uint32_t dst = stage0 + (uint32_t)(st.slot * p.stage_bytes), bar = full(st.slot);
-                    const int steps = min(left, kCB / 32);
-                    left -= steps;
                     const uint32_t sfb = (uint32_t)((kNv ? steps : (steps + 1) / 2) * kF4Atom);
                     mbar_expect_tx(bar, (uint32_t)((128 + p.bn) * kCB) + sfb * (1 + rts));
                     tma_load(dst, &tmb, c * kCB, jt * 128, bar);
@@ -107,44 +103,44 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
                     bulk_load(dst + off_sa, sa, sfb, bar);
                     if (rts > 1)
                         bulk_load(dst + off_sa + kAtoms * kF4Atom, sa + (long long)p.a.natoms * kF4Atom, sfb, bar);
-                    sb += kAtoms * kF4Atom;
-                    sa += kAtoms * kF4Atom;
-                    st.next(p.nstage);
                 }
+                sb += kAtoms * kF4Atom;
+                sa += kAtoms * kF4Atom;
+                st.next(p.nstage);
             }
-            // drain this thread's copies still in flight
-            for (int i = step > p.nstage ? step - p.nstage : 0; i < step; ++i)
-                mbar_wait<false>(full(i % p.nstage), (uint32_t)(i / p.nstage) & 1u, nullptr);
         }
+        if (!ok && lane == 0) {
+            if (!*abort) atomicExch(p.err, 1);
+            *abort = 1;
+        }
+        // drain this warp's copies still in flight
+        for (int i = step > p.nstage ? step - p.nstage : 0; i < step; ++i)
+            mbar_wait<false>(full(i % p.nstage), (uint32_t)(i / p.nstage) & 1u, nullptr);
         __syncwarp();
     } else if (warp == 9) {
-        if (lane == 0) {
-            RingPos st, ac;
-            int last = -1;
-            uint32_t last_parity = 0;
-            bool ok = true;
-            const uint32_t sfc = (uint32_t)(4 * kAtoms * (1 + nrt));  // TMEM columns of a stage's scales
-            for (int t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
-                if (!mbar_wait_fast(acce(ac.slot), ac.parity ^ 1u, abort)) {
-                    ok = false;
-                    break;
-                }
+        RingPos st, ac;
+        int last = -1;
+        uint32_t last_parity = 0;
+        bool ok = true;
+        const uint32_t sfc = (uint32_t)(4 * kAtoms * (1 + nrt));  // TMEM columns of a stage's scales
+        for (int t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(acce(ac.slot), ac.parity ^ 1u, abort));
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t d = tmem + (uint32_t)(ac.slot * p.acc_cols);
+            int left = p.b.Kp / 64;
+            for (int c = 0; c < p.nchunk; ++c) {
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(full(st.slot), st.parity, abort));
+                if (!ok) break;
                 tc_fence_after();
-                const uint32_t d = tmem + (uint32_t)(ac.slot * p.acc_cols);
-                int left = p.b.Kp / 64;
-                for (int c = 0; c < p.nchunk; ++c) {
-                    if (!mbar_wait_fast(full(st.slot), st.parity, abort)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint32_t src = stage0 + (uint32_t)(st.slot * p.stage_bytes);
-                    const int steps = min(left, kCB / 32);
-                    left -= steps;
-                    const int atoms = kNv ? steps : (steps + 1) / 2;
-                    const uint32_t tsb = tmem + 256u + (uint32_t)st.slot * sfc, tsa = tsb + 4 * kAtoms;
-                    const uint64_t db = f4_operand_desc<kCB>(src), da = f4_operand_desc<kCB>(src + off_b);
-                    const uint64_t dsb = f4_atom_desc(src + off_sb), dsa = f4_atom_desc(src + off_sa);
+                const uint32_t src = stage0 + (uint32_t)(st.slot * p.stage_bytes);
+                const int steps = min(left, kCB / 32);
+                left -= steps;
+                const int atoms = kNv ? steps : (steps + 1) / 2;
+                const uint32_t tsb = tmem + 256u + (uint32_t)st.slot * sfc, tsa = tsb + 4 * kAtoms;
+                const uint64_t db = f4_operand_desc<kCB>(src), da = f4_operand_desc<kCB>(src + off_b);
+                const uint64_t dsb = f4_atom_desc(src + off_sb), dsa = f4_atom_desc(src + off_sa);
+                if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < kAtoms; ++k) {
                         if (k >= atoms) break;
@@ -160,20 +156,20 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
                                     tsb + 4 * at, tsa + 4 * nrt * at, (c | k) ? 1u : 0u);
                     }
                     mma_commit(empty(st.slot));
-                    last = st.slot;
-                    last_parity = st.parity;
-                    st.next(p.nstage);
+                    if (c == p.nchunk - 1) mma_commit(accf(ac.slot));
                 }
-                if (ok) mma_commit(accf(ac.slot));
-                ac.next(p.nacc);
+                last = st.slot;
+                last_parity = st.parity;
+                st.next(p.nstage);
             }
-            if (!ok) {
-                if (!*abort) atomicExch(p.err, 2);
-                *abort = 1;
-            }
-            // the last products must finish before the accumulators are freed
-            if (last >= 0) mbar_wait<false>(empty(last), last_parity, nullptr);
+            ac.next(p.nacc);
         }
+        if (!ok && lane == 0) {
+            if (!*abort) atomicExch(p.err, 2);
+            *abort = 1;
+        }
+        // the last products must finish before the accumulators are freed
+        if (last >= 0) mbar_wait<false>(empty(last), last_parity, nullptr);
         __syncwarp();
     } else {
         const int group = warp >> 2;

@@ -81,8 +81,8 @@ constexpr int keys_stage(int nv, int cb) {
 
 // A CTA takes the units [u0, u1) of (row tile of a, span of b), b fastest.
 //   warps 0-11 quarter warp & 3 of the rows, every third tile, always of the same accumulator;
-//   warp 12    one thread loads: the row tile of a into one of two slots, b's tiles into a ring;
-//   warp 13    allocates TMEM, one thread copies scales to TMEM and multiplies into three
+//   warp 12    loads the row tile of a into one of two slots, b's tiles into a ring;
+//   warp 13    allocates TMEM, copies scales to TMEM and multiplies into three
 //              accumulators of 128 columns.
 // Every wait is bounded; on expiry the CTA records it in *err, drains its copies, frees TMEM and
 // returns.
