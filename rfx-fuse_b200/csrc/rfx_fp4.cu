@@ -18,7 +18,19 @@ namespace rfx {
 namespace {
 
 constexpr int kQThreads = 256;
-constexpr int kQChunk = 512;  // columns of a block of the grid, for matrices wider than kF4TopkK
+constexpr int kQChunk = 256;  // columns of a block of the grid
+
+// Division of n < 2^31 by a constant as a multiplication and a shift (Granlund and Montgomery,
+// Division by invariant integers using multiplication, PLDI 1994).
+struct FastDiv {
+    uint32_t m, s, d;
+    explicit FastDiv(uint32_t div) : d(div) {
+        s = 0;
+        while ((1ull << s) < div) ++s;
+        m = (uint32_t)((((1ull << s) - div) << 32) / div + 1);
+    }
+    __device__ __forceinline__ uint32_t quo(uint32_t n) const { return (__umulhi(m, n) + n) >> s; }
+};
 
 // The matrix scale for the largest finite |x| (its bits).
 __device__ __forceinline__ float nv_matrix_scale(uint32_t bits) {
@@ -31,49 +43,38 @@ __device__ __forceinline__ float nv_matrix_scale(uint32_t bits) {
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
-// Columns [c, c + 8) of a row of `cols` into v, zeros from cols on.
+// Elements of a 16-byte load.
+template <class T> constexpr int kVecOf = 16 / (int)sizeof(T);
+
+// Columns [c, c + kVecOf) of a row of `cols` into v, zeros from cols on.
 template <class T, bool kVec>
-__device__ __forceinline__ void load8(const T* row, int c, int cols, float* v) {
-    if (kVec && c + 8 <= cols) {
-        if (sizeof(T) == 4) {
-            const float4 a = __ldg(reinterpret_cast<const float4*>(row + c));
-            const float4 b = __ldg(reinterpret_cast<const float4*>(row + c) + 1);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else {
-            const uint4 a = __ldg(reinterpret_cast<const uint4*>(row + c));
-            T t[8];
-            *reinterpret_cast<uint4*>(t) = a;
+__device__ __forceinline__ void load_vec(const T* row, int c, int cols, float* v) {
+    if (kVec && c + kVecOf<T> <= cols) {
+        const uint4 a = __ldg(reinterpret_cast<const uint4*>(row + c));
+        T t[kVecOf<T>];
+        memcpy(t, &a, 16);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(t[i]);
-        }
+        for (int i = 0; i < kVecOf<T>; ++i) v[i] = to_f32<T>(t[i]);
         return;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? to_f32<T>(row[c + i]) : 0.0f;
+    for (int i = 0; i < kVecOf<T>; ++i) v[i] = c + i < cols ? to_f32<T>(row[c + i]) : 0.0f;
 }
 
-// Largest finite |x|, by integer maximum (the order of the atomics does not matter).
+// Largest finite |x|, by integer maximum (the order of the atomics does not matter).  Rows
+// [0, rows) of U vectors each, rows * U < 2^31.
 template <class T, bool kVec>
-__global__ void k_f4_amax(const T* __restrict__ x, long long ld, int rows, int cols, uint32_t* out) {
-    const int U = (cols + 7) / 8;
-    const long long total = (long long)rows * U;
-    const long long step = (long long)gridDim.x * blockDim.x;
+__global__ void k_f4_amax(const T* __restrict__ x, long long ld, int rows, int cols, FastDiv U, uint32_t* out) {
+    const uint32_t total = (uint32_t)rows * U.d;
+    const uint32_t step = gridDim.x * blockDim.x;
     uint32_t m = 0;
-    for (long long t = (long long)blockIdx.x * blockDim.x + threadIdx.x; t < total; t += step) {
-        long long r;
-        int u;
-        if (total < (1ll << 31)) {
-            r = (uint32_t)t / (uint32_t)U;
-            u = (int)((uint32_t)t % (uint32_t)U);
-        } else {
-            r = t / U;
-            u = (int)(t % U);
-        }
-        float v[8];
-        load8<T, kVec>(x + r * ld, 8 * u, cols, v);
+#pragma unroll 4
+    for (uint32_t t = blockIdx.x * blockDim.x + threadIdx.x; t < total; t += step) {
+        const uint32_t r = U.quo(t);
+        float v[kVecOf<T>];
+        load_vec<T, kVec>(x + (long long)r * ld, (int)(t - r * U.d) * kVecOf<T>, cols, v);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < kVecOf<T>; ++i) {
             const uint32_t b = abs_bits(v[i]);
             if (b < 0x7F800000u) m = max(m, b);
         }
@@ -89,42 +90,47 @@ __device__ __forceinline__ int mag2(uint32_t w) {
     return max(4, (int)__dp4a(m1, m1, __dp4a(m0, m0, 0u)));
 }
 
-// Bound of the tile's row norms from the units' sums of squares n2[row][U] (doubles, so that no
-// scale's square underflows); rows with a NaN scale are left out, they are nobody's neighbour.
-__device__ void tile_bound(const double* n2, int U, int rows, float* out) {
-    __shared__ double worst[4];
-    double m = 0.0;
+// Scale in a norm's bound: not below 2^-60, so that no square underflows (a bound may be larger
+// than the norm, and infinite where a square overflows).
+__device__ __forceinline__ float bound_scale(float s) { return s < 8.673617379884035e-19f ? 8.673617379884035e-19f : s; }
+
+// Bound of the tile's row norms from the units' sums of (2 x)^2, n2[unit][row] (padded to 129
+// rows); rows with a NaN scale are left out, they are nobody's neighbour.
+__device__ void tile_bound(const float* n2, int U, int rows, float* out) {
+    __shared__ float worst[4];
+    float m = 0.0f;
     if (threadIdx.x < kF4Tile) {
         if ((int)threadIdx.x < rows) {
-            double s = 0.0;
-            for (int u = 0; u < U; ++u) s += n2[threadIdx.x * U + u];
-            m = s >= 0.0 ? s : 0.0;
+            float s = 0.0f;
+            for (int u = 0; u < U; ++u) s += n2[u * 129 + threadIdx.x];
+            m = s >= 0.0f ? s : 0.0f;
         }
-        for (int o = 16; o; o >>= 1) m = fmax(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
         if ((threadIdx.x & 31) == 0) worst[threadIdx.x >> 5] = m;
     }
     __syncthreads();
     if (threadIdx.x == 0) {
-        m = fmax(fmax(worst[0], worst[1]), fmax(worst[2], worst[3]));
-        *out = __double2float_ru(sqrt(m) * 0.5 * 1.000001);
+        m = fmaxf(fmaxf(worst[0], worst[1]), fmaxf(worst[2], worst[3]));
+        *out = sqrtf(m) * 0.50001f;  // at most 64 additions, each off by 2^-24
     }
 }
 
-// One block: 128 rows x up to kQChunk columns (all of them when the matrix has at most
-// kF4TopkK).  A lane holds 8 columns; a block of columns is 2 or 4 neighbouring lanes.  Codes
-// leave as 4 bytes a lane, scales through shared memory in the atoms' order.  kSelf: the grid is
-// this block alone, which then finds the matrix scale itself (one launch for small matrices).
-// Tiles run from the last to the first: k_f4_amax has just read the last ones into L2.
+// One block: 128 rows x up to kQChunk columns.  A lane holds one 16-byte vector; a block of columns
+// is 2 to 8 neighbouring lanes.  Codes leave as 2 or 4 bytes a lane, scales through shared memory
+// in the atoms' order.  kSelf: the grid is this block alone, which then finds the matrix scale
+// itself (one launch for small matrices).  Tiles run from the last to the first: k_f4_amax has
+// just read the last ones into L2.
 template <class T, bool kVec, int kNv, bool kSelf>
 __global__ void __launch_bounds__(kQThreads)
-k_f4_quantize(const T* __restrict__ x, long long ld, F4 m) {
+k_f4_quantize(const T* __restrict__ x, long long ld, F4 m, FastDiv Ud) {
+    constexpr int kV = kVecOf<T>;
     __shared__ uint32_t sf[kQChunk / 64 * kF4Atom / 4];
     __shared__ uint32_t s_amax;
-    extern __shared__ double n2[];
+    extern __shared__ float n2[];
     const int tile = gridDim.x - 1 - blockIdx.x;
     const int c0 = blockIdx.y * kQChunk;
     const int kc = min(kQChunk, m.Kp - c0);  // columns of this block (multiple of 64)
-    const int U = kc / 8;
+    const int U = kc / kV;                   // vectors of a row; Ud divides by it but in the last chunk
     const int r0 = tile * kF4Tile;
     const int nr = min(kF4Tile, m.rows - r0);
     const bool bounds = m.Kp <= kF4TopkK;
@@ -132,16 +138,18 @@ k_f4_quantize(const T* __restrict__ x, long long ld, F4 m) {
     for (int i = threadIdx.x; i < atoms * (kF4Atom / 4); i += kQThreads) sf[i] = 0;
     if (kSelf && threadIdx.x == 0) s_amax = 0;
     __syncthreads();
+    const bool whole = U == (int)Ud.d;
+    const T* src = x + (long long)r0 * ld;
     float g = 1.0f;
     if (kNv) {
         uint32_t amax = 0;
         if (kSelf) {
             for (int t = threadIdx.x; t < nr * U; t += kQThreads) {
                 const int q = t / U, u = t - q * U;
-                float v[8];
-                load8<T, kVec>(x + (long long)(r0 + q) * ld, c0 + 8 * u, m.cols, v);
+                float v[kV];
+                load_vec<T, kVec>(src + (long long)q * ld, c0 + kV * u, m.cols, v);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < kV; ++i) {
                     const uint32_t b = abs_bits(v[i]);
                     if (b < 0x7F800000u) amax = max(amax, b);
                 }
@@ -156,22 +164,25 @@ k_f4_quantize(const T* __restrict__ x, long long ld, F4 m) {
     }
     if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) m.gs[0] = g;
     const float inv_g = 1.0f / g;
-    constexpr int kLanes = kNv ? 2 : 4;  // lanes of a block of columns
-    // U is a multiple of 8, so a block of columns never straddles a warp's end; every lane of a
-    // warp makes the same number of rounds
+    constexpr int kLanes = (kNv ? 16 : 32) / kV;  // lanes of a block of columns
+    constexpr int kCodes = kV / 2;                // bytes of codes of a lane
+    uint8_t* dst = m.codes + (long long)r0 * m.pitch() + c0 / 2;
+    // U is a multiple of 8, so a block of columns never straddles a warp's end, and every lane of
+    // a warp makes the same number of rounds
+#pragma unroll 2
     for (int t = threadIdx.x; t < kF4Tile * U; t += kQThreads) {
-        const int q = t / U, u = t - q * U;
+        const int q = whole ? (int)Ud.quo((uint32_t)t) : t / U, u = t - q * U;
         const bool live = q < nr;
-        float v[8];
+        float v[kV];
         if (live) {
-            load8<T, kVec>(x + (long long)(r0 + q) * ld, c0 + 8 * u, m.cols, v);
+            load_vec<T, kVec>(src + (long long)q * ld, c0 + kV * u, m.cols, v);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+            for (int i = 0; i < kV; ++i) v[i] = 0.0f;
         }
         uint32_t amax = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) amax = max(amax, abs_bits(v[i]));
+        for (int i = 0; i < kV; ++i) amax = max(amax, abs_bits(v[i]));
 #pragma unroll
         for (int o = 1; o < kLanes; o <<= 1) amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
         uint32_t byte;
@@ -183,7 +194,7 @@ k_f4_quantize(const T* __restrict__ x, long long ld, F4 m) {
             // Research and Development 34(1), 1990)
             const float r = s > 0.0f ? 1.0f / s : 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < kV; ++i) {
                 const float xs = v[i] * inv_g;
                 const float y = xs * r;
                 v[i] = fmaf(fmaf(-y, s, xs), r, y);
@@ -196,9 +207,11 @@ k_f4_quantize(const T* __restrict__ x, long long ld, F4 m) {
             s = e8m0_value(byte);
             const float r = __int_as_float((127 - e) << 23);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] *= r;
+            for (int i = 0; i < kV; ++i) v[i] *= r;
         }
-        uint32_t w = cvt_e2m1x8(v);
+        uint32_t w;
+        if constexpr (kV == 8) w = cvt_e2m1x8(v);
+        else w = cvt_e2m1x4(v);
         if (kNv && s == 0.0f) w = 0;
         if (amax >= 0x7F800000u) {
             byte = kNv ? 0x7Fu : 0xFFu;
@@ -206,67 +219,93 @@ k_f4_quantize(const T* __restrict__ x, long long ld, F4 m) {
             s = __int_as_float(0x7fc00000);
         }
         if (live) {
-            reinterpret_cast<uint32_t*>(m.codes + (long long)(r0 + q) * m.pitch() + c0 / 2)[u] = w;
-            if (u % kLanes == 0 && c0 + 8 * u < m.cols) {
+            uint8_t* o = dst + (long long)q * m.pitch() + u * kCodes;
+            if (kV == 8) *reinterpret_cast<uint32_t*>(o) = w;
+            else *reinterpret_cast<uint16_t*>(o) = (uint16_t)w;
+            if (u % kLanes == 0 && c0 + kV * u < m.cols) {
                 const int blk = u / kLanes;
                 reinterpret_cast<uint8_t*>(sf)[blk / 4 * kF4Atom + (q % 32) * 16 + q / 32 * 4 + blk % 4] = (uint8_t)byte;
             }
-            if (bounds) n2[q * U + u] = (double)mag2(w) * ((double)s * (double)s);
+            if (bounds) {
+                const float b = bound_scale(s);
+                n2[u * 129 + q] = (float)mag2(w) * (b * b);
+            }
         }
     }
     __syncthreads();
-    uint32_t* dst = reinterpret_cast<uint32_t*>(m.scales + ((long long)tile * m.natoms + c0 / (kNv ? 64 : 128)) * kF4Atom);
-    for (int i = threadIdx.x; i < atoms * (kF4Atom / 4); i += kQThreads) dst[i] = sf[i];
+    uint32_t* out = reinterpret_cast<uint32_t*>(m.scales + ((long long)tile * m.natoms + c0 / (kNv ? 64 : 128)) * kF4Atom);
+    for (int i = threadIdx.x; i < atoms * (kF4Atom / 4); i += kQThreads) out[i] = sf[i];
     if (bounds) tile_bound(n2, U, nr, m.bounds + tile);
 }
 
-// Values of rows [r0, r1): a thread per element, so that any leading dimension stores coalesced.
-template <class T>
-__global__ void k_f4_dequantize_any(F4 m, int r0, long long n, T* __restrict__ out, long long ld) {
-    const long long step = (long long)gridDim.x * blockDim.x;
+// Values of rows [r0, r1) to a contiguous, 16-byte aligned output: a thread per 16 bytes of it.
+// kWhole: they all lie in one row (cols a multiple of their number), and so in one block.
+template <class T, int kNv, bool kWhole>
+__global__ void k_f4_dequantize_flat(F4 m, int r0, uint32_t n, FastDiv cols, T* __restrict__ out) {
+    constexpr int kV = kVecOf<T>;
+    constexpr int sh = kNv ? 4 : 5;
+    const uint32_t step = gridDim.x * blockDim.x;
     const float g = __ldg(m.gs);
-    const int sh = m.nv ? 4 : 5;
-    for (long long t = (long long)blockIdx.x * blockDim.x + threadIdx.x; t < n; t += step) {
-        long long r;
-        int c;
-        if (n < (1ll << 31)) {
-            r = (uint32_t)t / (uint32_t)m.cols;
-            c = (int)((uint32_t)t - (uint32_t)r * (uint32_t)m.cols);
+    const uint32_t nvec = (n + kV - 1) / kV;
+#pragma unroll 4
+    for (uint32_t t = blockIdx.x * blockDim.x + threadIdx.x; t < nvec; t += step) {
+        const uint32_t at = t * kV;
+        uint32_t r = cols.quo(at);
+        int c = (int)(at - r * cols.d);
+        T v[kV];
+        if (kWhole) {
+            const long long row = (long long)r0 + r;
+            const uint8_t* codes = m.codes + row * m.pitch() + c / 2;
+            const uint32_t w = kV == 8 ? __ldg(reinterpret_cast<const uint32_t*>(codes))
+                                       : (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(codes));
+            const float s = f4_scale_value(kNv, __ldg(m.scales + f4_scale_at(m, row, c >> sh)));
+            float f[kV];
+            e2m1_values<kV>(w, f);
+#pragma unroll
+            for (int i = 0; i < kV; ++i) v[i] = from_f32<T>(f[i] * s * g);
         } else {
-            r = t / m.cols;
-            c = (int)(t - r * m.cols);
+            float s = 0.0f;
+            uint32_t b = 0;
+#pragma unroll
+            for (int i = 0; i < kV; ++i) {
+                if (at + i < n) {
+                    const long long row = (long long)r0 + r;
+                    if (i == 0 || (c & 1) == 0) b = __ldg(m.codes + row * m.pitch() + c / 2);
+                    if (i == 0 || (c & ((1 << sh) - 1)) == 0)
+                        s = f4_scale_value(kNv, __ldg(m.scales + f4_scale_at(m, row, c >> sh)));
+                    v[i] = from_f32<T>(e2m1_value((c & 1) ? b >> 4 : b & 15u) * s * g);
+                    if (++c == (int)cols.d) {
+                        c = 0;
+                        ++r;
+                    }
+                }
+            }
         }
-        const uint32_t b = __ldg(m.codes + (r0 + r) * m.pitch() + c / 2);
-        const float s = f4_scale_value(m.nv, __ldg(m.scales + f4_scale_at(m, r0 + r, c >> sh)));
-        out[r * ld + c] = from_f32<T>(e2m1_value((c & 1) ? b >> 4 : b & 15u) * s * g);
+        if (kWhole || at + kV <= n) {
+            uint4 o;
+            memcpy(&o, v, 16);
+            *reinterpret_cast<uint4*>(out + at) = o;
+        } else {
+#pragma unroll
+            for (int i = 0; i < kV; ++i)
+                if (at + i < n) out[at + i] = v[i];
+        }
     }
 }
 
-// The same for rows whose 8-column pieces are all whole and 16-byte aligned.
+// The same for any leading dimension and alignment: a thread per element.
 template <class T>
-__global__ void k_f4_dequantize_vec(F4 m, int r0, long long n, T* __restrict__ out, long long ld) {
-    const int U = m.cols / 8;
-    const long long step = (long long)gridDim.x * blockDim.x;
+__global__ void k_f4_dequantize_any(F4 m, int r0, uint32_t n, FastDiv cols, T* __restrict__ out, long long ld) {
+    const uint32_t step = gridDim.x * blockDim.x;
     const float g = __ldg(m.gs);
-    const int sh = m.nv ? 1 : 2;
-    for (long long t = (long long)blockIdx.x * blockDim.x + threadIdx.x; t < n; t += step) {
-        long long r;
-        int u;
-        if (n < (1ll << 31)) {
-            r = (uint32_t)t / (uint32_t)U;
-            u = (int)((uint32_t)t - (uint32_t)r * (uint32_t)U);
-        } else {
-            r = t / U;
-            u = (int)(t - r * U);
-        }
-        const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(m.codes + (r0 + r) * m.pitch()) + u);
-        const float s = f4_scale_value(m.nv, __ldg(m.scales + f4_scale_at(m, r0 + r, u >> sh)));
-        T v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = from_f32<T>(e2m1_value((w >> (4 * i)) & 15u) * s * g);
-        uint4* o = reinterpret_cast<uint4*>(out + r * ld + 8 * u);
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) o[i] = reinterpret_cast<const uint4*>(v)[i];
+    const int sh = m.nv ? 4 : 5;
+    for (uint32_t t = blockIdx.x * blockDim.x + threadIdx.x; t < n; t += step) {
+        const uint32_t r = cols.quo(t);
+        const int c = (int)(t - r * cols.d);
+        const long long row = (long long)r0 + r;
+        const uint32_t b = __ldg(m.codes + row * m.pitch() + c / 2);
+        const float s = f4_scale_value(m.nv, __ldg(m.scales + f4_scale_at(m, row, c >> sh)));
+        out[r * ld + c] = from_f32<T>(e2m1_value((c & 1) ? b >> 4 : b & 15u) * s * g);
     }
 }
 
@@ -275,7 +314,7 @@ __global__ void k_f4_dequantize_vec(F4 m, int r0, long long n, T* __restrict__ o
 __global__ void __launch_bounds__(kQThreads)
 k_f4_pack(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, const float* g, F4 m) {
     __shared__ uint32_t sf[kQChunk / 64 * kF4Atom / 4];
-    extern __shared__ double n2[];
+    extern __shared__ float n2[];
     const int tile = blockIdx.x;
     const int c0 = blockIdx.y * kQChunk;
     const int kc = min(kQChunk, m.Kp - c0);
@@ -308,8 +347,8 @@ k_f4_pack(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
         if ((u & ((1 << sh) - 1)) == 0)
             reinterpret_cast<uint8_t*>(sf)[blk / 4 * kF4Atom + (q % 32) * 16 + q / 32 * 4 + blk % 4] = (uint8_t)byte;
         if (bounds) {
-            const double s = (double)f4_scale_value(m.nv, byte);
-            n2[q * U + u] = (double)mag2(w) * (s * s);
+            const float s = bound_scale(f4_scale_value(m.nv, byte));
+            n2[u * 129 + q] = (float)mag2(w) * (s * s);
         }
     }
     __syncthreads();
@@ -332,25 +371,36 @@ __global__ void k_f4_unpack(F4 m, uint8_t* __restrict__ codes, uint8_t* __restri
     }
 }
 
+size_t bound_smem(const F4& m, int width) {
+    return m.Kp <= kF4TopkK ? (size_t)(m.Kp / width) * 129 * sizeof(float) : 0;
+}
+
 template <class T, bool kVec>
 cudaError_t quantize_t(const T* x, long long ld, const F4& m, int sms, cudaStream_t st, int* launches) {
     const dim3 grid((unsigned)m.tiles(), (unsigned)((m.Kp + kQChunk - 1) / kQChunk));
-    const size_t smem = m.Kp <= kF4TopkK ? (size_t)kF4Tile * (m.Kp / 8) * sizeof(double) : 0;
+    const size_t smem = bound_smem(m, kVecOf<T>);
     const bool self = grid.x == 1 && grid.y == 1;
+    const FastDiv U((uint32_t)(std::min(m.Kp, kQChunk) / kVecOf<T>));
     if (!m.nv) {
-        k_f4_quantize<T, kVec, 0, false><<<grid, kQThreads, smem, st>>>(x, ld, m);
+        k_f4_quantize<T, kVec, 0, false><<<grid, kQThreads, smem, st>>>(x, ld, m, U);
         *launches += 1;
     } else if (self) {
-        k_f4_quantize<T, kVec, 1, true><<<grid, kQThreads, smem, st>>>(x, ld, m);
+        k_f4_quantize<T, kVec, 1, true><<<grid, kQThreads, smem, st>>>(x, ld, m, U);
         *launches += 1;
     } else {
         cudaError_t e = cudaMemsetAsync(m.gs + 1, 0, 4, st);
         if (e != cudaSuccess) return e;
-        const long long units = (long long)m.rows * ((m.cols + 7) / 8);
-        const int blocks = (int)std::min<long long>((units + 255) / 256, (long long)sms * 8);
-        k_f4_amax<T, kVec><<<blocks, 256, 0, st>>>(x, ld, m.rows, m.cols, reinterpret_cast<uint32_t*>(m.gs) + 1);
-        k_f4_quantize<T, kVec, 1, false><<<grid, kQThreads, smem, st>>>(x, ld, m);
-        *launches += 2;
+        const FastDiv vecs((uint32_t)((m.cols + kVecOf<T> - 1) / kVecOf<T>));
+        const int most = (int)std::min<long long>(m.rows, (1ll << 30) / vecs.d);  // rows of a launch
+        for (int r0 = 0; r0 < m.rows; r0 += std::min(most, m.rows - r0)) {
+            const int rows = std::min(most, m.rows - r0);
+            const int blocks = (int)std::min<long long>(((long long)rows * vecs.d + 255) / 256, (long long)sms * 8);
+            k_f4_amax<T, kVec><<<blocks, 256, 0, st>>>(x + (long long)r0 * ld, ld, rows, m.cols, vecs,
+                                                      reinterpret_cast<uint32_t*>(m.gs) + 1);
+            *launches += 1;
+        }
+        k_f4_quantize<T, kVec, 1, false><<<grid, kQThreads, smem, st>>>(x, ld, m, U);
+        *launches += 1;
     }
     return cudaGetLastError();
 }
@@ -363,12 +413,25 @@ cudaError_t quantize_d(const void* x, long long ld, const F4& m, int sms, cudaSt
 }
 
 template <class T>
-cudaError_t dequantize_d(const F4& m, int r0, int r1, void* out, long long ld, cudaStream_t st) {
-    const bool vec = m.cols % 8 == 0 && ((uintptr_t)out & 15) == 0 && (ld * (long long)sizeof(T)) % 16 == 0;
-    const long long n = (long long)(r1 - r0) * (vec ? m.cols / 8 : m.cols);
-    const int blocks = (int)std::min<long long>((n + 255) / 256, 1ll << 20);
-    if (vec) k_f4_dequantize_vec<T><<<blocks, 256, 0, st>>>(m, r0, n, (T*)out, ld);
-    else k_f4_dequantize_any<T><<<blocks, 256, 0, st>>>(m, r0, n, (T*)out, ld);
+cudaError_t dequantize_d(const F4& m, int r0, int r1, T* out, long long ld, int sms, cudaStream_t st) {
+    constexpr int kV = kVecOf<T>;
+    const FastDiv cols((uint32_t)m.cols);
+    // 2^30 elements a launch at most, and whole vectors of a contiguous output
+    const int most = (int)std::max<long long>(kV, std::min<long long>(r1 - r0, (1ll << 30) / m.cols) / kV * kV);
+    for (int r = r0; r < r1; r += std::min(most, r1 - r)) {
+        const int rows = std::min(most, r1 - r);
+        const uint32_t n = (uint32_t)rows * (uint32_t)m.cols;
+        T* o = out + (long long)(r - r0) * ld;
+        const bool flat = ((uintptr_t)o & 15) == 0 && (ld == m.cols || rows == 1);
+        const bool whole = m.cols % kV == 0;
+        const uint32_t threads = flat ? (n + kV - 1) / kV : n;
+        const int blocks = (int)std::min<uint32_t>((threads + 255) / 256, (uint32_t)sms * 32);
+        if (!flat) k_f4_dequantize_any<T><<<blocks, 256, 0, st>>>(m, r, n, cols, o, ld);
+        else if (m.nv && whole) k_f4_dequantize_flat<T, 1, true><<<blocks, 256, 0, st>>>(m, r, n, cols, o);
+        else if (m.nv) k_f4_dequantize_flat<T, 1, false><<<blocks, 256, 0, st>>>(m, r, n, cols, o);
+        else if (whole) k_f4_dequantize_flat<T, 0, true><<<blocks, 256, 0, st>>>(m, r, n, cols, o);
+        else k_f4_dequantize_flat<T, 0, false><<<blocks, 256, 0, st>>>(m, r, n, cols, o);
+    }
     return cudaGetLastError();
 }
 
@@ -381,15 +444,15 @@ cudaError_t f4_quantize(const void* x, int dtype, long long ld, const F4& m, int
     return quantize_d<__half>(x, ld, m, sms, st, launches);
 }
 
-cudaError_t f4_dequantize(const F4& m, int r0, int r1, void* out, int dtype, long long ld, cudaStream_t st) {
-    if (dtype == RFX_F32) return dequantize_d<float>(m, r0, r1, out, ld, st);
-    if (dtype == RFX_BF16) return dequantize_d<__nv_bfloat16>(m, r0, r1, out, ld, st);
-    return dequantize_d<__half>(m, r0, r1, out, ld, st);
+cudaError_t f4_dequantize(const F4& m, int r0, int r1, void* out, int dtype, long long ld, int sms, cudaStream_t st) {
+    if (dtype == RFX_F32) return dequantize_d<float>(m, r0, r1, (float*)out, ld, sms, st);
+    if (dtype == RFX_BF16) return dequantize_d<__nv_bfloat16>(m, r0, r1, (__nv_bfloat16*)out, ld, sms, st);
+    return dequantize_d<__half>(m, r0, r1, (__half*)out, ld, sms, st);
 }
 
 cudaError_t f4_pack(const uint8_t* codes, const uint8_t* scales, const float* g, const F4& m, cudaStream_t st) {
     const dim3 grid((unsigned)m.tiles(), (unsigned)((m.Kp + kQChunk - 1) / kQChunk));
-    const size_t smem = m.Kp <= kF4TopkK ? (size_t)kF4Tile * (m.Kp / 8) * sizeof(double) : 0;
+    const size_t smem = bound_smem(m, 8);
     k_f4_pack<<<grid, kQThreads, smem, st>>>(codes, scales, g, m);
     return cudaGetLastError();
 }

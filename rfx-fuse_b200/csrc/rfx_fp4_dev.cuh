@@ -48,6 +48,18 @@ __device__ __forceinline__ uint32_t cvt_e2m1x8(const float* v) {
     return d;
 }
 
+// The same for four floats, in the lower half of a word.
+__device__ __forceinline__ uint32_t cvt_e2m1x4(const float* v) {
+    uint32_t d;
+    asm("{\n\t.reg .b8 b0, b1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+        "mov.b32 %0, {b0, b1, b0, b1};\n\t}\n"
+        : "=r"(d)
+        : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]));
+    return d & 0xFFFFu;
+}
+
 // Twice the magnitudes (0, 1, 2, 3, 4, 6, 8, 12) of the four codes in the low half of w, as bytes.
 __device__ __forceinline__ uint32_t e2m1_mag4(uint32_t w) {
     return __byte_perm(0x03020100u, 0x0C080604u, w & 0x7777u);
@@ -60,6 +72,22 @@ __device__ __forceinline__ uint32_t e2m1_neg4(uint32_t w) {
     uint32_t d;
     asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(0x80u), "r"(0u), "r"(w & 0x8888u));
     return d & 0x7F7F7F7Fu;
+}
+
+// The values of kN (4 or 8) codes in a word, through the upper bytes of their fp16 forms.
+template <int kN>
+__device__ __forceinline__ void e2m1_values(uint32_t w, float* v) {
+#pragma unroll
+    for (int q = 0; q < kN / 4; ++q) {
+        const uint32_t x = w >> (16 * q);
+        const uint32_t hi = __byte_perm(0x3E3C3800u, 0x46444240u, x & 0x7777u) | ((e2m1_neg4(x) & 0x01010101u) << 7);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const uint32_t pair = __byte_perm(hi, 0u, e ? 0x3424u : 0x1404u);
+            v[4 * q + 2 * e] = __half2float(__ushort_as_half((unsigned short)(pair & 0xFFFFu)));
+            v[4 * q + 2 * e + 1] = __half2float(__ushort_as_half((unsigned short)(pair >> 16)));
+        }
+    }
 }
 
 // Value of one e2m1 code.
