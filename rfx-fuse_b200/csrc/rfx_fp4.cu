@@ -43,22 +43,25 @@ __device__ __forceinline__ float nv_matrix_scale(uint32_t bits) {
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
-// Elements of a 16-byte load.
+// Elements of a 16-byte vector.
 template <class T> constexpr int kVecOf = 16 / (int)sizeof(T);
 
-// Columns [c, c + kVecOf) of a row of `cols` into v, zeros from cols on.
-template <class T, bool kVec>
-__device__ __forceinline__ void load_vec(const T* row, int c, int cols, float* v) {
-    if (kVec && c + kVecOf<T> <= cols) {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(row + c));
-        T t[kVecOf<T>];
-        memcpy(t, &a, 16);
+// Columns [c, c + kN) of a row of `cols` into v, zeros from cols on.
+template <class T, bool kVec, int kN>
+__device__ __forceinline__ void load_cols(const T* row, int c, int cols, float* v) {
+    if (kVec && c + kN <= cols) {
 #pragma unroll
-        for (int i = 0; i < kVecOf<T>; ++i) v[i] = to_f32<T>(t[i]);
+        for (int h = 0; h < kN; h += kVecOf<T>) {
+            const uint4 a = __ldg(reinterpret_cast<const uint4*>(row + c + h));
+            T t[kVecOf<T>];
+            memcpy(t, &a, 16);
+#pragma unroll
+            for (int i = 0; i < kVecOf<T>; ++i) v[h + i] = to_f32<T>(t[i]);
+        }
         return;
     }
 #pragma unroll
-    for (int i = 0; i < kVecOf<T>; ++i) v[i] = c + i < cols ? to_f32<T>(row[c + i]) : 0.0f;
+    for (int i = 0; i < kN; ++i) v[i] = c + i < cols ? to_f32<T>(row[c + i]) : 0.0f;
 }
 
 // Largest finite |x|, by integer maximum (the order of the atomics does not matter).  Rows
@@ -72,7 +75,7 @@ __global__ void k_f4_amax(const T* __restrict__ x, long long ld, int rows, int c
     for (uint32_t t = blockIdx.x * blockDim.x + threadIdx.x; t < total; t += step) {
         const uint32_t r = U.quo(t);
         float v[kVecOf<T>];
-        load_vec<T, kVec>(x + (long long)r * ld, (int)(t - r * U.d) * kVecOf<T>, cols, v);
+        load_cols<T, kVec, kVecOf<T>>(x + (long long)r * ld, (int)(t - r * U.d) * kVecOf<T>, cols, v);
 #pragma unroll
         for (int i = 0; i < kVecOf<T>; ++i) {
             const uint32_t b = abs_bits(v[i]);
@@ -115,41 +118,57 @@ __device__ void tile_bound(const float* n2, int U, int rows, float* out) {
     }
 }
 
-// One block: 128 rows x up to kQChunk columns.  A lane holds one 16-byte vector; a block of columns
-// is 2 to 8 neighbouring lanes.  Codes leave as 2 or 4 bytes a lane, scales through shared memory
-// in the atoms' order.  kSelf: the grid is this block alone, which then finds the matrix scale
-// itself (one launch for small matrices).  Tiles run from the last to the first: k_f4_amax has
-// just read the last ones into L2.
+// max(a, |b|), NaN when either is.
+__device__ __forceinline__ float max_abs_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(fabsf(b)));
+    return d;
+}
+
+// One block: 128 rows x up to kQChunk columns, a lane 8 columns; a block of columns is 2 or 4
+// neighbouring lanes.  Codes leave as 4 bytes a lane, scales through shared memory in the atoms'
+// order.  kSelf: the grid is this block alone, which then finds the matrix scale itself (one
+// launch for small matrices).  Tiles run from the last to the first: k_f4_amax has just read the
+// last ones into L2.  Integer operations issue at half the rate of fp32 ones here, and they bound
+// the kernel: hence the fp32 maxima, the table of scales and no division per lane.
 template <class T, bool kVec, int kNv, bool kSelf>
 __global__ void __launch_bounds__(kQThreads)
-k_f4_quantize(const T* __restrict__ x, long long ld, F4 m, FastDiv Ud) {
-    constexpr int kV = kVecOf<T>;
+k_f4_quantize(const T* __restrict__ x, long long ld, F4 m) {
     __shared__ uint32_t sf[kQChunk / 64 * kF4Atom / 4];
+    __shared__ float2 table[kNv ? 128 : 1];  // e4m3 values and their reciprocals
     __shared__ uint32_t s_amax;
     extern __shared__ float n2[];
     const int tile = gridDim.x - 1 - blockIdx.x;
     const int c0 = blockIdx.y * kQChunk;
     const int kc = min(kQChunk, m.Kp - c0);  // columns of this block (multiple of 64)
-    const int U = kc / kV;                   // vectors of a row; Ud divides by it but in the last chunk
+    const int U = kc / 8;
     const int r0 = tile * kF4Tile;
     const int nr = min(kF4Tile, m.rows - r0);
     const bool bounds = m.Kp <= kF4TopkK;
     const int atoms = kNv ? kc / 64 : (kc + 127) / 128;
     for (int i = threadIdx.x; i < atoms * (kF4Atom / 4); i += kQThreads) sf[i] = 0;
+    if (kNv && threadIdx.x < 128) {
+        const float s = e4m3_value(threadIdx.x);
+        table[threadIdx.x] = make_float2(s, s > 0.0f ? 1.0f / s : 0.0f);
+    }
     if (kSelf && threadIdx.x == 0) s_amax = 0;
     __syncthreads();
-    const bool whole = U == (int)Ud.d;
     const T* src = x + (long long)r0 * ld;
+    // a thread's units are threadIdx.x, + kQThreads, ...: their rows and columns by addition
+    const int q0 = threadIdx.x / U, u0 = threadIdx.x - q0 * U, dq = kQThreads / U, du = kQThreads - dq * U;
     float g = 1.0f;
     if (kNv) {
         uint32_t amax = 0;
         if (kSelf) {
-            for (int t = threadIdx.x; t < nr * U; t += kQThreads) {
-                const int q = t / U, u = t - q * U;
-                float v[kV];
-                load_vec<T, kVec>(src + (long long)q * ld, c0 + kV * u, m.cols, v);
+            for (int q = q0, u = u0; q < nr; q += dq, u += du) {
+                if (u >= U) {
+                    u -= U;
+                    if (++q >= nr) break;
+                }
+                float v[8];
+                load_cols<T, kVec, 8>(src + (long long)q * ld, c0 + 8 * u, m.cols, v);
 #pragma unroll
-                for (int i = 0; i < kV; ++i) {
+                for (int i = 0; i < 8; ++i) {
                     const uint32_t b = abs_bits(v[i]);
                     if (b < 0x7F800000u) amax = max(amax, b);
                 }
@@ -164,65 +183,65 @@ k_f4_quantize(const T* __restrict__ x, long long ld, F4 m, FastDiv Ud) {
     }
     if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) m.gs[0] = g;
     const float inv_g = 1.0f / g;
-    constexpr int kLanes = (kNv ? 16 : 32) / kV;  // lanes of a block of columns
-    constexpr int kCodes = kV / 2;                // bytes of codes of a lane
+    constexpr int kLanes = kNv ? 2 : 4;  // lanes of a block of columns
     uint8_t* dst = m.codes + (long long)r0 * m.pitch() + c0 / 2;
     // U is a multiple of 8, so a block of columns never straddles a warp's end, and every lane of
     // a warp makes the same number of rounds
+    const int rounds = kF4Tile * U / kQThreads;
+    int q = q0, u = u0;
 #pragma unroll 2
-    for (int t = threadIdx.x; t < kF4Tile * U; t += kQThreads) {
-        const int q = whole ? (int)Ud.quo((uint32_t)t) : t / U, u = t - q * U;
+    for (int round = 0; round < rounds; ++round) {
         const bool live = q < nr;
-        float v[kV];
+        float v[8];
         if (live) {
-            load_vec<T, kVec>(src + (long long)q * ld, c0 + kV * u, m.cols, v);
+            load_cols<T, kVec, 8>(src + (long long)q * ld, c0 + 8 * u, m.cols, v);
         } else {
 #pragma unroll
-            for (int i = 0; i < kV; ++i) v[i] = 0.0f;
+            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
         }
-        uint32_t amax = 0;
+        float amax = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kV; ++i) amax = max(amax, abs_bits(v[i]));
+        for (int i = 0; i < 8; ++i) amax = max_abs_nan(amax, v[i]);
 #pragma unroll
-        for (int o = 1; o < kLanes; o <<= 1) amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+        for (int o = 1; o < kLanes; o <<= 1) amax = max_abs_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+        const bool bad = !(amax < __int_as_float(0x7f800000));
         uint32_t byte;
         float s;  // the scale in units of g
         if (kNv) {
-            byte = cvt_e4m3x2(__uint_as_float(amax) * inv_g / 6.0f, 0.0f) & 0xFFu;
-            s = e4m3_value(byte);
-            // x / s correctly rounded from the rounded reciprocal (Markstein, IBM Journal of
-            // Research and Development 34(1), 1990)
-            const float r = s > 0.0f ? 1.0f / s : 0.0f;
+            // amax / (6 g) and x / s correctly rounded from rounded reciprocals (Markstein, IBM
+            // Journal of Research and Development 34(1), 1990)
+            constexpr float r6 = 1.0f / 6.0f;
+            const float w = amax * inv_g;
+            const float z = w * r6;
+            byte = cvt_e4m3x2(fmaf(fmaf(-z, 6.0f, w), r6, z), 0.0f) & 0x7Fu;
+            const float2 sr = table[byte];
+            s = sr.x;
 #pragma unroll
-            for (int i = 0; i < kV; ++i) {
+            for (int i = 0; i < 8; ++i) {
                 const float xs = v[i] * inv_g;
-                const float y = xs * r;
-                v[i] = fmaf(fmaf(-y, s, xs), r, y);
+                const float y = xs * sr.y;
+                v[i] = fmaf(fmaf(-y, s, xs), sr.y, y);
             }
         } else {
-            int e = (int)(amax >> 23) - 127;
-            e = (amax & 0x7FFFFFu) <= 0x400000u ? e - 2 : e - 1;  // 6 = 1.5 * 2^2
+            const uint32_t bits = __float_as_uint(amax);
+            int e = (int)(bits >> 23) - 127;
+            e = (bits & 0x7FFFFFu) <= 0x400000u ? e - 2 : e - 1;  // 6 = 1.5 * 2^2
             if (e < -127) e = -127;
             byte = (uint32_t)(e + 127);
             s = e8m0_value(byte);
             const float r = __int_as_float((127 - e) << 23);
 #pragma unroll
-            for (int i = 0; i < kV; ++i) v[i] *= r;
+            for (int i = 0; i < 8; ++i) v[i] *= r;
         }
-        uint32_t w;
-        if constexpr (kV == 8) w = cvt_e2m1x8(v);
-        else w = cvt_e2m1x4(v);
-        if (kNv && s == 0.0f) w = 0;
-        if (amax >= 0x7F800000u) {
+        uint32_t w = cvt_e2m1x8(v);
+        if (bad || (kNv && s == 0.0f)) w = 0;
+        if (bad) {
             byte = kNv ? 0x7Fu : 0xFFu;
-            w = 0;
             s = __int_as_float(0x7fc00000);
         }
         if (live) {
-            uint8_t* o = dst + (long long)q * m.pitch() + u * kCodes;
-            if (kV == 8) *reinterpret_cast<uint32_t*>(o) = w;
-            else *reinterpret_cast<uint16_t*>(o) = (uint16_t)w;
-            if (u % kLanes == 0 && c0 + kV * u < m.cols) {
+            reinterpret_cast<uint32_t*>(dst + (long long)q * m.pitch())[u] = w;
+            if (u % kLanes == 0 && c0 + 8 * u < m.cols) {
                 const int blk = u / kLanes;
                 reinterpret_cast<uint8_t*>(sf)[blk / 4 * kF4Atom + (q % 32) * 16 + q / 32 * 4 + blk % 4] = (uint8_t)byte;
             }
@@ -231,6 +250,12 @@ k_f4_quantize(const T* __restrict__ x, long long ld, F4 m, FastDiv Ud) {
                 n2[u * 129 + q] = (float)mag2(w) * (b * b);
             }
         }
+        q += dq;
+        u += du;
+        if (u >= U) {
+            u -= U;
+            ++q;
+        }
     }
     __syncthreads();
     uint32_t* out = reinterpret_cast<uint32_t*>(m.scales + ((long long)tile * m.natoms + c0 / (kNv ? 64 : 128)) * kF4Atom);
@@ -238,74 +263,71 @@ k_f4_quantize(const T* __restrict__ x, long long ld, F4 m, FastDiv Ud) {
     if (bounds) tile_bound(n2, U, nr, m.bounds + tile);
 }
 
-// Values of rows [r0, r1) to a contiguous, 16-byte aligned output: a thread per 16 bytes of it.
-// kWhole: they all lie in one row (cols a multiple of their number), and so in one block.
-template <class T, int kNv, bool kWhole>
-__global__ void k_f4_dequantize_flat(F4 m, int r0, uint32_t n, FastDiv cols, T* __restrict__ out) {
-    constexpr int kV = kVecOf<T>;
+// Values of rows [r0, r1) into out (row r0 first).  A block takes 128 rows x up to kQChunk columns;
+// their scales are decoded into shared memory once.  kVec: a thread writes 16 bytes at a time
+// (cols a multiple of them, rows 16-byte aligned); else a thread walks down one column, so that a
+// warp writes neighbouring elements whatever the alignment.
+template <class T, int kNv, bool kVec>
+__global__ void __launch_bounds__(kQThreads)
+k_f4_dequantize(F4 m, int r0, int r1, T* __restrict__ out, long long ld) {
+    constexpr int kV = kVec ? kVecOf<T> : 1;
     constexpr int sh = kNv ? 4 : 5;
-    const uint32_t step = gridDim.x * blockDim.x;
+    constexpr int kBlocks = kQChunk >> sh;   // scales of a row here
+    __shared__ float sc[kF4Tile * (kBlocks + 1)];
+    const int tile = r0 / kF4Tile + blockIdx.x;
+    const int c0 = blockIdx.y * kQChunk;
+    const int kc = min(kQChunk, m.cols - c0);
+    const int nb = (kc + (1 << sh) - 1) >> sh;
+    const int qa = max(0, r0 - tile * kF4Tile), qb = min(kF4Tile, r1 - tile * kF4Tile);
+    const uint8_t* atoms = m.scales + ((long long)tile * m.natoms + c0 / (kNv ? 64 : 128)) * kF4Atom;
+    for (int t = threadIdx.x; t < kF4Tile * nb; t += kQThreads) {
+        const int b = t >> 7, q = t & 127;
+        sc[q * (kBlocks + 1) + b] = f4_scale_value(kNv, __ldg(atoms + b / 4 * kF4Atom + (q % 32) * 16 + q / 32 * 4 + b % 4));
+    }
+    __syncthreads();
     const float g = __ldg(m.gs);
-    const uint32_t nvec = (n + kV - 1) / kV;
+    const uint8_t* codes = m.codes + (long long)tile * kF4Tile * m.pitch() + c0 / 2;
+    T* dst = out + ((long long)tile * kF4Tile - r0) * ld + c0;
+    if constexpr (kVec) {
+        const int U = kc / kV;
+        const int dq = kQThreads / U, du = kQThreads - dq * U;
+        int q = threadIdx.x / U, u = threadIdx.x - q * U;
+        q += qa;
 #pragma unroll 4
-    for (uint32_t t = blockIdx.x * blockDim.x + threadIdx.x; t < nvec; t += step) {
-        const uint32_t at = t * kV;
-        uint32_t r = cols.quo(at);
-        int c = (int)(at - r * cols.d);
-        T v[kV];
-        if (kWhole) {
-            const long long row = (long long)r0 + r;
-            const uint8_t* codes = m.codes + row * m.pitch() + c / 2;
-            const uint32_t w = kV == 8 ? __ldg(reinterpret_cast<const uint32_t*>(codes))
-                                       : (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(codes));
-            const float s = f4_scale_value(kNv, __ldg(m.scales + f4_scale_at(m, row, c >> sh)));
-            float f[kV];
-            e2m1_values<kV>(w, f);
+        while (q < qb) {
+            const uint8_t* p = codes + (long long)q * m.pitch() + u * (kV / 2);
+            uint32_t w;
+            if (kV == 8) w = __ldg(reinterpret_cast<const uint32_t*>(p));
+            else w = __ldg(reinterpret_cast<const uint16_t*>(p));
+            const float s = sc[q * (kBlocks + 1) + ((u * kV) >> sh)];
+            float f[kV == 8 ? 8 : 4];
+            e2m1_values<kV == 8 ? 8 : 4>(w, f);
+            T v[kV];
 #pragma unroll
             for (int i = 0; i < kV; ++i) v[i] = from_f32<T>(f[i] * s * g);
-        } else {
-            float s = 0.0f;
-            uint32_t b = 0;
-#pragma unroll
-            for (int i = 0; i < kV; ++i) {
-                if (at + i < n) {
-                    const long long row = (long long)r0 + r;
-                    if (i == 0 || (c & 1) == 0) b = __ldg(m.codes + row * m.pitch() + c / 2);
-                    if (i == 0 || (c & ((1 << sh) - 1)) == 0)
-                        s = f4_scale_value(kNv, __ldg(m.scales + f4_scale_at(m, row, c >> sh)));
-                    v[i] = from_f32<T>(e2m1_value((c & 1) ? b >> 4 : b & 15u) * s * g);
-                    if (++c == (int)cols.d) {
-                        c = 0;
-                        ++r;
-                    }
-                }
-            }
-        }
-        if (kWhole || at + kV <= n) {
             uint4 o;
             memcpy(&o, v, 16);
-            *reinterpret_cast<uint4*>(out + at) = o;
-        } else {
-#pragma unroll
-            for (int i = 0; i < kV; ++i)
-                if (at + i < n) out[at + i] = v[i];
+            *reinterpret_cast<uint4*>(dst + (long long)q * ld + u * kV) = o;
+            q += dq;
+            u += du;
+            if (u >= U) {
+                u -= U;
+                ++q;
+            }
         }
-    }
-}
-
-// The same for any leading dimension and alignment: a thread per element.
-template <class T>
-__global__ void k_f4_dequantize_any(F4 m, int r0, uint32_t n, FastDiv cols, T* __restrict__ out, long long ld) {
-    const uint32_t step = gridDim.x * blockDim.x;
-    const float g = __ldg(m.gs);
-    const int sh = m.nv ? 4 : 5;
-    for (uint32_t t = blockIdx.x * blockDim.x + threadIdx.x; t < n; t += step) {
-        const uint32_t r = cols.quo(t);
-        const int c = (int)(t - r * cols.d);
-        const long long row = (long long)r0 + r;
-        const uint32_t b = __ldg(m.codes + row * m.pitch() + c / 2);
-        const float s = f4_scale_value(m.nv, __ldg(m.scales + f4_scale_at(m, row, c >> sh)));
-        out[r * ld + c] = from_f32<T>(e2m1_value((c & 1) ? b >> 4 : b & 15u) * s * g);
+    } else if ((int)threadIdx.x < kc) {
+        const int c = threadIdx.x;
+        const uint8_t* p = codes + (long long)qa * m.pitch() + c / 2;
+        const float* s = sc + (c >> sh) + qa * (kBlocks + 1);
+        T* o = dst + (long long)qa * ld + c;
+        const int shift = (c & 1) * 4;
+#pragma unroll 8
+        for (int q = qa; q < qb; ++q) {
+            *o = from_f32<T>(e2m1_value(__ldg(p) >> shift & 15u) * *s * g);
+            p += m.pitch();
+            s += kBlocks + 1;
+            o += ld;
+        }
     }
 }
 
@@ -378,14 +400,13 @@ size_t bound_smem(const F4& m, int width) {
 template <class T, bool kVec>
 cudaError_t quantize_t(const T* x, long long ld, const F4& m, int sms, cudaStream_t st, int* launches) {
     const dim3 grid((unsigned)m.tiles(), (unsigned)((m.Kp + kQChunk - 1) / kQChunk));
-    const size_t smem = bound_smem(m, kVecOf<T>);
+    const size_t smem = bound_smem(m, 8);
     const bool self = grid.x == 1 && grid.y == 1;
-    const FastDiv U((uint32_t)(std::min(m.Kp, kQChunk) / kVecOf<T>));
     if (!m.nv) {
-        k_f4_quantize<T, kVec, 0, false><<<grid, kQThreads, smem, st>>>(x, ld, m, U);
+        k_f4_quantize<T, kVec, 0, false><<<grid, kQThreads, smem, st>>>(x, ld, m);
         *launches += 1;
     } else if (self) {
-        k_f4_quantize<T, kVec, 1, true><<<grid, kQThreads, smem, st>>>(x, ld, m, U);
+        k_f4_quantize<T, kVec, 1, true><<<grid, kQThreads, smem, st>>>(x, ld, m);
         *launches += 1;
     } else {
         cudaError_t e = cudaMemsetAsync(m.gs + 1, 0, 4, st);
@@ -399,7 +420,7 @@ cudaError_t quantize_t(const T* x, long long ld, const F4& m, int sms, cudaStrea
                                                       reinterpret_cast<uint32_t*>(m.gs) + 1);
             *launches += 1;
         }
-        k_f4_quantize<T, kVec, 1, false><<<grid, kQThreads, smem, st>>>(x, ld, m, U);
+        k_f4_quantize<T, kVec, 1, false><<<grid, kQThreads, smem, st>>>(x, ld, m);
         *launches += 1;
     }
     return cudaGetLastError();
@@ -413,25 +434,14 @@ cudaError_t quantize_d(const void* x, long long ld, const F4& m, int sms, cudaSt
 }
 
 template <class T>
-cudaError_t dequantize_d(const F4& m, int r0, int r1, T* out, long long ld, int sms, cudaStream_t st) {
+cudaError_t dequantize_d(const F4& m, int r0, int r1, T* out, long long ld, cudaStream_t st) {
     constexpr int kV = kVecOf<T>;
-    const FastDiv cols((uint32_t)m.cols);
-    // 2^30 elements a launch at most, and whole vectors of a contiguous output
-    const int most = (int)std::max<long long>(kV, std::min<long long>(r1 - r0, (1ll << 30) / m.cols) / kV * kV);
-    for (int r = r0; r < r1; r += std::min(most, r1 - r)) {
-        const int rows = std::min(most, r1 - r);
-        const uint32_t n = (uint32_t)rows * (uint32_t)m.cols;
-        T* o = out + (long long)(r - r0) * ld;
-        const bool flat = ((uintptr_t)o & 15) == 0 && (ld == m.cols || rows == 1);
-        const bool whole = m.cols % kV == 0;
-        const uint32_t threads = flat ? (n + kV - 1) / kV : n;
-        const int blocks = (int)std::min<uint32_t>((threads + 255) / 256, (uint32_t)sms * 32);
-        if (!flat) k_f4_dequantize_any<T><<<blocks, 256, 0, st>>>(m, r, n, cols, o, ld);
-        else if (m.nv && whole) k_f4_dequantize_flat<T, 1, true><<<blocks, 256, 0, st>>>(m, r, n, cols, o);
-        else if (m.nv) k_f4_dequantize_flat<T, 1, false><<<blocks, 256, 0, st>>>(m, r, n, cols, o);
-        else if (whole) k_f4_dequantize_flat<T, 0, true><<<blocks, 256, 0, st>>>(m, r, n, cols, o);
-        else k_f4_dequantize_flat<T, 0, false><<<blocks, 256, 0, st>>>(m, r, n, cols, o);
-    }
+    const bool vec = m.cols % kV == 0 && ((uintptr_t)out & 15) == 0 && (ld * (long long)sizeof(T)) % 16 == 0;
+    const dim3 grid((unsigned)((r1 - 1) / kF4Tile - r0 / kF4Tile + 1), (unsigned)((m.cols + kQChunk - 1) / kQChunk));
+    if (m.nv && vec) k_f4_dequantize<T, 1, true><<<grid, kQThreads, 0, st>>>(m, r0, r1, out, ld);
+    else if (m.nv) k_f4_dequantize<T, 1, false><<<grid, kQThreads, 0, st>>>(m, r0, r1, out, ld);
+    else if (vec) k_f4_dequantize<T, 0, true><<<grid, kQThreads, 0, st>>>(m, r0, r1, out, ld);
+    else k_f4_dequantize<T, 0, false><<<grid, kQThreads, 0, st>>>(m, r0, r1, out, ld);
     return cudaGetLastError();
 }
 
@@ -444,10 +454,10 @@ cudaError_t f4_quantize(const void* x, int dtype, long long ld, const F4& m, int
     return quantize_d<__half>(x, ld, m, sms, st, launches);
 }
 
-cudaError_t f4_dequantize(const F4& m, int r0, int r1, void* out, int dtype, long long ld, int sms, cudaStream_t st) {
-    if (dtype == RFX_F32) return dequantize_d<float>(m, r0, r1, (float*)out, ld, sms, st);
-    if (dtype == RFX_BF16) return dequantize_d<__nv_bfloat16>(m, r0, r1, (__nv_bfloat16*)out, ld, sms, st);
-    return dequantize_d<__half>(m, r0, r1, (__half*)out, ld, sms, st);
+cudaError_t f4_dequantize(const F4& m, int r0, int r1, void* out, int dtype, long long ld, cudaStream_t st) {
+    if (dtype == RFX_F32) return dequantize_d<float>(m, r0, r1, (float*)out, ld, st);
+    if (dtype == RFX_BF16) return dequantize_d<__nv_bfloat16>(m, r0, r1, (__nv_bfloat16*)out, ld, st);
+    return dequantize_d<__half>(m, r0, r1, (__half*)out, ld, st);
 }
 
 cudaError_t f4_pack(const uint8_t* codes, const uint8_t* scales, const float* g, const F4& m, cudaStream_t st) {

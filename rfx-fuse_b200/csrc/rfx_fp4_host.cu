@@ -198,8 +198,7 @@ int rfx_fp4_dequantize(const rfx_fp4_matrix* mat, int row_begin, int row_end, vo
         require(ld >= m.cols, RFX_ERR_ARG, "ld must be at least cols");
         if (row_begin == row_end) return;
         check_elements(out_dev, dtype, "out");
-        check_launch(rfx::f4_dequantize(m, row_begin, row_end, out_dev, dtype, ld, device_info().sms,
-                                        static_cast<cudaStream_t>(stream)),
+        check_launch(rfx::f4_dequantize(m, row_begin, row_end, out_dev, dtype, ld, static_cast<cudaStream_t>(stream)),
                      "rfx_fp4_dequantize");
     });
 }
@@ -306,7 +305,7 @@ int rfx_lowrank4_factors(void* ctx, float* A_host, int* rank_out, int* rows_out)
         if (A_host) {
             const size_t n = (size_t)m.rows * m.cols * 4;
             float* out = (float*)c.lr_out_v.get(n);
-            check_launch(rfx::f4_dequantize(m, 0, m.rows, out, RFX_F32, m.cols, c.sm_count, c.st), "rfx_lowrank4_factors");
+            check_launch(rfx::f4_dequantize(m, 0, m.rows, out, RFX_F32, m.cols, c.st), "rfx_lowrank4_factors");
             c.launches += 1;
             RFX_CUDA(cudaMemcpyAsync(A_host, out, n, cudaMemcpyDeviceToHost, c.st));
             RFX_CUDA(cudaStreamSynchronize(c.st));
