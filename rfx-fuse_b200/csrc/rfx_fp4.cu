@@ -67,15 +67,15 @@ __device__ __forceinline__ void load_cols(const T* row, int c, int cols, float* 
 // Largest finite |x|, by integer maximum (the order of the atomics does not matter).  Rows
 // [0, rows) of U vectors each, rows * U < 2^31.
 template <class T, bool kVec>
-__global__ void k_f4_amax(const T* __restrict__ x, long long ld, int rows, int cols, FastDiv U, uint32_t* out) {
+__global__ void k_f4_amax(const T* __restrict__ x, long long ld, int rows, int cols, FastDiv U, bool flat, uint32_t* out) {
     const uint32_t total = (uint32_t)rows * U.d;
     const uint32_t step = gridDim.x * blockDim.x;
     uint32_t m = 0;
 #pragma unroll 4
     for (uint32_t t = blockIdx.x * blockDim.x + threadIdx.x; t < total; t += step) {
-        const uint32_t r = U.quo(t);
         float v[kVecOf<T>];
-        load_cols<T, kVec, kVecOf<T>>(x + (long long)r * ld, (int)(t - r * U.d) * kVecOf<T>, cols, v);
+        const uint32_t r = flat ? 0u : U.quo(t);  // flat: rows of whole vectors that follow one another
+        load_cols<T, kVec, kVecOf<T>>(x + (long long)r * ld, (int)(t - r * U.d) * kVecOf<T>, flat ? 0x7FFFFFFF : cols, v);
 #pragma unroll
         for (int i = 0; i < kVecOf<T>; ++i) {
             const uint32_t b = abs_bits(v[i]);
@@ -154,17 +154,14 @@ k_f4_quantize(const T* __restrict__ x, long long ld, F4 m) {
     if (kSelf && threadIdx.x == 0) s_amax = 0;
     __syncthreads();
     const T* src = x + (long long)r0 * ld;
-    // a thread's units are threadIdx.x, + kQThreads, ...: their rows and columns by addition
-    const int q0 = threadIdx.x / U, u0 = threadIdx.x - q0 * U, dq = kQThreads / U, du = kQThreads - dq * U;
+    // a thread keeps its columns and walks down the rows
+    const int groups = kQThreads / U, grp = threadIdx.x / U, u = threadIdx.x - grp * U;
+    const bool active = grp < groups;
     float g = 1.0f;
     if (kNv) {
         uint32_t amax = 0;
         if (kSelf) {
-            for (int q = q0, u = u0; q < nr; q += dq, u += du) {
-                if (u >= U) {
-                    u -= U;
-                    if (++q >= nr) break;
-                }
+            for (int q = active ? grp : nr; q < nr; q += groups) {
                 float v[8];
                 load_cols<T, kVec, 8>(src + (long long)q * ld, c0 + 8 * u, m.cols, v);
 #pragma unroll
@@ -187,11 +184,11 @@ k_f4_quantize(const T* __restrict__ x, long long ld, F4 m) {
     uint8_t* dst = m.codes + (long long)r0 * m.pitch() + c0 / 2;
     // U is a multiple of 8, so a block of columns never straddles a warp's end, and every lane of
     // a warp makes the same number of rounds
-    const int rounds = kF4Tile * U / kQThreads;
-    int q = q0, u = u0;
-#pragma unroll 2
-    for (int round = 0; round < rounds; ++round) {
-        const bool live = q < nr;
+    const int rounds = (kF4Tile + groups - 1) / groups;
+    int q = grp;
+#pragma unroll 4
+    for (int round = 0; round < rounds; ++round, q += groups) {
+        const bool live = active && q < nr;
         float v[8];
         if (live) {
             load_cols<T, kVec, 8>(src + (long long)q * ld, c0 + 8 * u, m.cols, v);
@@ -250,12 +247,6 @@ k_f4_quantize(const T* __restrict__ x, long long ld, F4 m) {
                 n2[u * 129 + q] = (float)mag2(w) * (b * b);
             }
         }
-        q += dq;
-        u += du;
-        if (u >= U) {
-            u -= U;
-            ++q;
-        }
     }
     __syncthreads();
     uint32_t* out = reinterpret_cast<uint32_t*>(m.scales + ((long long)tile * m.natoms + c0 / (kNv ? 64 : 128)) * kF4Atom);
@@ -264,70 +255,80 @@ k_f4_quantize(const T* __restrict__ x, long long ld, F4 m) {
 }
 
 // Values of rows [r0, r1) into out (row r0 first).  A block takes 128 rows x up to kQChunk columns;
-// their scales are decoded into shared memory once.  kVec: a thread writes 16 bytes at a time
-// (cols a multiple of them, rows 16-byte aligned); else a thread walks down one column, so that a
-// warp writes neighbouring elements whatever the alignment.
-template <class T, int kNv, bool kVec>
+// their scales are decoded into shared memory once, while the first codes are on their way.  A
+// thread writes kV elements at a time: 16 bytes, 4, or one element, as columns and alignment allow;
+// neighbouring threads write neighbouring elements.
+template <class T, int kNv, int kV>
 __global__ void __launch_bounds__(kQThreads)
 k_f4_dequantize(F4 m, int r0, int r1, T* __restrict__ out, long long ld) {
-    constexpr int kV = kVec ? kVecOf<T> : 1;
     constexpr int sh = kNv ? 4 : 5;
     constexpr int kBlocks = kQChunk >> sh;   // scales of a row here
+    constexpr int kBatch = 8;                // loads in flight
     __shared__ float sc[kF4Tile * (kBlocks + 1)];
     const int tile = r0 / kF4Tile + blockIdx.x;
     const int c0 = blockIdx.y * kQChunk;
     const int kc = min(kQChunk, m.cols - c0);
     const int nb = (kc + (1 << sh) - 1) >> sh;
     const int qa = max(0, r0 - tile * kF4Tile), qb = min(kF4Tile, r1 - tile * kF4Tile);
-    const uint8_t* atoms = m.scales + ((long long)tile * m.natoms + c0 / (kNv ? 64 : 128)) * kF4Atom;
-    for (int t = threadIdx.x; t < kF4Tile * nb; t += kQThreads) {
-        const int b = t >> 7, q = t & 127;
-        sc[q * (kBlocks + 1) + b] = f4_scale_value(kNv, __ldg(atoms + b / 4 * kF4Atom + (q % 32) * 16 + q / 32 * 4 + b % 4));
-    }
-    __syncthreads();
     const float g = __ldg(m.gs);
     const uint8_t* codes = m.codes + (long long)tile * kF4Tile * m.pitch() + c0 / 2;
     T* dst = out + ((long long)tile * kF4Tile - r0) * ld + c0;
-    if constexpr (kVec) {
-        const int U = kc / kV;
-        const int dq = kQThreads / U, du = kQThreads - dq * U;
-        int q = threadIdx.x / U, u = threadIdx.x - q * U;
-        q += qa;
-#pragma unroll 4
-        while (q < qb) {
-            const uint8_t* p = codes + (long long)q * m.pitch() + u * (kV / 2);
-            uint32_t w;
-            if (kV == 8) w = __ldg(reinterpret_cast<const uint32_t*>(p));
-            else w = __ldg(reinterpret_cast<const uint16_t*>(p));
-            const float s = sc[q * (kBlocks + 1) + ((u * kV) >> sh)];
-            float f[kV == 8 ? 8 : 4];
-            e2m1_values<kV == 8 ? 8 : 4>(w, f);
-            T v[kV];
+    // a thread keeps its columns and walks down the rows
+    const int U = kc / kV, groups = kQThreads / U;
+    const int grp = threadIdx.x / U, u = threadIdx.x - grp * U;
+    int q = grp < groups ? qa + grp : qb;
+    const uint8_t* p = codes + (long long)q * m.pitch() + (u * kV) / 2;
+    const float* s = sc + q * (kBlocks + 1) + ((u * kV) >> sh);
+    T* o = dst + (long long)q * ld + u * kV;
+    const long long p_step = (long long)groups * m.pitch(), o_step = groups * ld;
+    for (bool first = true;; first = false) {
+        uint32_t w[kBatch];
 #pragma unroll
-            for (int i = 0; i < kV; ++i) v[i] = from_f32<T>(f[i] * s * g);
-            uint4 o;
-            memcpy(&o, v, 16);
-            *reinterpret_cast<uint4*>(dst + (long long)q * ld + u * kV) = o;
-            q += dq;
-            u += du;
-            if (u >= U) {
-                u -= U;
-                ++q;
+        for (int e = 0; e < kBatch; ++e) {
+            w[e] = 0;
+            if (q + e * groups < qb) {
+                if constexpr (kV == 8) w[e] = __ldg(reinterpret_cast<const uint32_t*>(p));
+                else if constexpr (kV == 4) w[e] = __ldg(reinterpret_cast<const uint16_t*>(p));
+                else w[e] = __ldg(p);
             }
+            p += p_step;
         }
-    } else if ((int)threadIdx.x < kc) {
-        const int c = threadIdx.x;
-        const uint8_t* p = codes + (long long)qa * m.pitch() + c / 2;
-        const float* s = sc + (c >> sh) + qa * (kBlocks + 1);
-        T* o = dst + (long long)qa * ld + c;
-        const int shift = (c & 1) * 4;
-#pragma unroll 8
-        for (int q = qa; q < qb; ++q) {
-            *o = from_f32<T>(e2m1_value(__ldg(p) >> shift & 15u) * *s * g);
-            p += m.pitch();
-            s += kBlocks + 1;
-            o += ld;
+        if (first) {
+            const uint8_t* atoms = m.scales + ((long long)tile * m.natoms + c0 / (kNv ? 64 : 128)) * kF4Atom;
+            for (int t = threadIdx.x; t < kF4Tile * nb; t += kQThreads) {
+                const int b = t >> 7, r = t & 127;
+                sc[r * (kBlocks + 1) + b] =
+                    f4_scale_value(kNv, __ldg(atoms + b / 4 * kF4Atom + (r % 32) * 16 + r / 32 * 4 + b % 4));
+            }
+            __syncthreads();
         }
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) {
+            if (q < qb) {
+                const float sv = *s;
+                if constexpr (kV >= 4) {
+                    float f[kV];
+                    e2m1_values<kV>(w[e], f);
+                    T v[kV];
+#pragma unroll
+                    for (int i = 0; i < kV; ++i) v[i] = from_f32<T>(f[i] * sv * g);
+                    uint4 x;
+                    memcpy(&x, v, 16);
+                    *reinterpret_cast<uint4*>(o) = x;
+                } else if constexpr (kV == 2) {
+                    T v[2] = {from_f32<T>(e2m1_value(w[e] & 15u) * sv * g), from_f32<T>(e2m1_value(w[e] >> 4) * sv * g)};
+                    uint32_t x;
+                    memcpy(&x, v, 4);
+                    *reinterpret_cast<uint32_t*>(o) = x;
+                } else {
+                    *o = from_f32<T>(e2m1_value(w[e] >> ((u & 1) * 4) & 15u) * sv * g);
+                }
+            }
+            q += groups;
+            s += groups * (kBlocks + 1);
+            o += o_step;
+        }
+        if (q >= qb) break;
     }
 }
 
@@ -412,11 +413,12 @@ cudaError_t quantize_t(const T* x, long long ld, const F4& m, int sms, cudaStrea
         cudaError_t e = cudaMemsetAsync(m.gs + 1, 0, 4, st);
         if (e != cudaSuccess) return e;
         const FastDiv vecs((uint32_t)((m.cols + kVecOf<T> - 1) / kVecOf<T>));
-        const int most = (int)std::min<long long>(m.rows, (1ll << 30) / vecs.d);  // rows of a launch
+        const int most = (int)std::min<long long>(m.rows, (1ll << 27) / vecs.d);  // rows of a launch
+        const bool flat = kVec && ld == m.cols && m.cols % kVecOf<T> == 0;
         for (int r0 = 0; r0 < m.rows; r0 += std::min(most, m.rows - r0)) {
             const int rows = std::min(most, m.rows - r0);
             const int blocks = (int)std::min<long long>(((long long)rows * vecs.d + 255) / 256, (long long)sms * 8);
-            k_f4_amax<T, kVec><<<blocks, 256, 0, st>>>(x + (long long)r0 * ld, ld, rows, m.cols, vecs,
+            k_f4_amax<T, kVec><<<blocks, 256, 0, st>>>(x + (long long)r0 * ld, ld, rows, m.cols, vecs, flat,
                                                       reinterpret_cast<uint32_t*>(m.gs) + 1);
             *launches += 1;
         }
@@ -433,16 +435,22 @@ cudaError_t quantize_d(const void* x, long long ld, const F4& m, int sms, cudaSt
                : quantize_t<T, false>((const T*)x, ld, m, sms, st, launches);
 }
 
+template <class T, int kV>
+cudaError_t dequantize_v(const F4& m, int r0, int r1, T* out, long long ld, cudaStream_t st) {
+    const dim3 grid((unsigned)((r1 - 1) / kF4Tile - r0 / kF4Tile + 1), (unsigned)((m.cols + kQChunk - 1) / kQChunk));
+    if (m.nv) k_f4_dequantize<T, 1, kV><<<grid, kQThreads, 0, st>>>(m, r0, r1, out, ld);
+    else k_f4_dequantize<T, 0, kV><<<grid, kQThreads, 0, st>>>(m, r0, r1, out, ld);
+    return cudaGetLastError();
+}
+
 template <class T>
 cudaError_t dequantize_d(const F4& m, int r0, int r1, T* out, long long ld, cudaStream_t st) {
-    constexpr int kV = kVecOf<T>;
-    const bool vec = m.cols % kV == 0 && ((uintptr_t)out & 15) == 0 && (ld * (long long)sizeof(T)) % 16 == 0;
-    const dim3 grid((unsigned)((r1 - 1) / kF4Tile - r0 / kF4Tile + 1), (unsigned)((m.cols + kQChunk - 1) / kQChunk));
-    if (m.nv && vec) k_f4_dequantize<T, 1, true><<<grid, kQThreads, 0, st>>>(m, r0, r1, out, ld);
-    else if (m.nv) k_f4_dequantize<T, 1, false><<<grid, kQThreads, 0, st>>>(m, r0, r1, out, ld);
-    else if (vec) k_f4_dequantize<T, 0, true><<<grid, kQThreads, 0, st>>>(m, r0, r1, out, ld);
-    else k_f4_dequantize<T, 0, false><<<grid, kQThreads, 0, st>>>(m, r0, r1, out, ld);
-    return cudaGetLastError();
+    auto fits = [&](int bytes) {
+        return m.cols * (int)sizeof(T) % bytes == 0 && (uintptr_t)out % bytes == 0 && ld * (long long)sizeof(T) % bytes == 0;
+    };
+    if (m.cols % kVecOf<T> == 0 && fits(16)) return dequantize_v<T, kVecOf<T>>(m, r0, r1, out, ld, st);
+    if (sizeof(T) == 2 && fits(4)) return dequantize_v<T, 2>(m, r0, r1, out, ld, st);
+    return dequantize_v<T, 1>(m, r0, r1, out, ld, st);
 }
 
 }  // namespace
