@@ -254,81 +254,77 @@ k_f4_quantize(const T* __restrict__ x, long long ld, F4 m) {
     if (bounds) tile_bound(n2, U, nr, m.bounds + tile);
 }
 
-// Values of rows [r0, r1) into out (row r0 first).  A block takes 128 rows x up to kQChunk columns;
-// their scales are decoded into shared memory once, while the first codes are on their way.  A
-// thread writes kV elements at a time: 16 bytes, 4, or one element, as columns and alignment allow;
-// neighbouring threads write neighbouring elements.
+// Values of rows [r0, r1) into out (row r0 first).  A block takes 128 rows x up to kQChunk columns:
+// their codes come into shared memory by 16-byte loads, all in flight at once, their scales decoded
+// beside them.  A thread then writes kV elements at a time: 16 bytes, 4, or one element, as columns
+// and alignment allow; neighbouring threads write neighbouring elements and walk down the rows.
 template <class T, int kNv, int kV>
 __global__ void __launch_bounds__(kQThreads)
 k_f4_dequantize(F4 m, int r0, int r1, T* __restrict__ out, long long ld) {
     constexpr int sh = kNv ? 4 : 5;
-    constexpr int kBlocks = kQChunk >> sh;   // scales of a row here
-    constexpr int kBatch = 8;                // loads in flight
+    constexpr int kBlocks = kQChunk >> sh;     // scales of a row here
+    constexpr int kRow = kQChunk / 2 + 16;     // bytes of a row of codes, padded against conflicts
+    __shared__ __align__(16) uint8_t cs[kF4Tile * kRow];
     __shared__ float sc[kF4Tile * (kBlocks + 1)];
+    __shared__ float lut[16];                  // the codes' values, for one element at a time
     const int tile = r0 / kF4Tile + blockIdx.x;
     const int c0 = blockIdx.y * kQChunk;
     const int kc = min(kQChunk, m.cols - c0);
     const int nb = (kc + (1 << sh) - 1) >> sh;
     const int qa = max(0, r0 - tile * kF4Tile), qb = min(kF4Tile, r1 - tile * kF4Tile);
     const float g = __ldg(m.gs);
-    const uint8_t* codes = m.codes + (long long)tile * kF4Tile * m.pitch() + c0 / 2;
-    T* dst = out + ((long long)tile * kF4Tile - r0) * ld + c0;
-    // a thread keeps its columns and walks down the rows
+    {
+        const uint8_t* codes = m.codes + (long long)tile * kF4Tile * m.pitch() + c0 / 2;
+        const int words = (min(kQChunk, m.Kp - c0) / 2) / 16;  // 16-byte words of a row: 2, 4, 6 or 8
+        for (int t = threadIdx.x; t < kF4Tile * words; t += kQThreads) {
+            const int q = t / words, w = t - q * words;
+            if (q >= qa && q < qb)
+                *reinterpret_cast<uint4*>(cs + q * kRow + 16 * w) =
+                    __ldg(reinterpret_cast<const uint4*>(codes + (long long)q * m.pitch()) + w);
+        }
+        if (kV < 4 && threadIdx.x < 16) lut[threadIdx.x] = e2m1_value(threadIdx.x);
+        const uint8_t* atoms = m.scales + ((long long)tile * m.natoms + c0 / (kNv ? 64 : 128)) * kF4Atom;
+        for (int t = threadIdx.x; t < kF4Tile * nb; t += kQThreads) {
+            const int b = t >> 7, r = t & 127;
+            sc[r * (kBlocks + 1) + b] =
+                f4_scale_value(kNv, __ldg(atoms + b / 4 * kF4Atom + (r % 32) * 16 + r / 32 * 4 + b % 4));
+        }
+    }
+    __syncthreads();
     const int U = kc / kV, groups = kQThreads / U;
     const int grp = threadIdx.x / U, u = threadIdx.x - grp * U;
-    int q = grp < groups ? qa + grp : qb;
-    const uint8_t* p = codes + (long long)q * m.pitch() + (u * kV) / 2;
-    const float* s = sc + q * (kBlocks + 1) + ((u * kV) >> sh);
-    T* o = dst + (long long)q * ld + u * kV;
-    const long long p_step = (long long)groups * m.pitch(), o_step = groups * ld;
-    for (bool first = true;; first = false) {
-        uint32_t w[kBatch];
+    if (grp >= groups) return;
+    const uint8_t* p = cs + (u * kV) / 2;
+    const float* s = sc + ((u * kV) >> sh);
+    T* o = out + ((long long)tile * kF4Tile - r0 + qa + grp) * ld + c0 + u * kV;
+    const long long step = groups * ld;
+    const int shift = (u & 1) * 4;
+#pragma unroll 4
+    for (int q = qa + grp; q < qb; q += groups, o += step) {
+        const float sv = s[q * (kBlocks + 1)];
+        if constexpr (kV >= 4) {
+            uint32_t w;
+            if constexpr (kV == 8) w = *reinterpret_cast<const uint32_t*>(p + q * kRow);
+            else w = *reinterpret_cast<const uint16_t*>(p + q * kRow);
+            float f[kV];
+            e2m1_values<kV>(w, f);
+            T v[kV];
 #pragma unroll
-        for (int e = 0; e < kBatch; ++e) {
-            w[e] = 0;
-            if (q + e * groups < qb) {
-                if constexpr (kV == 8) w[e] = __ldg(reinterpret_cast<const uint32_t*>(p));
-                else if constexpr (kV == 4) w[e] = __ldg(reinterpret_cast<const uint16_t*>(p));
-                else w[e] = __ldg(p);
+            for (int i = 0; i < kV; ++i) v[i] = from_f32<T>(f[i] * sv * g);
+            uint4 x;
+            memcpy(&x, v, 16);
+            *reinterpret_cast<uint4*>(o) = x;
+        } else {
+            const uint32_t w = p[q * kRow];
+            if constexpr (kV == 2) {
+                T v[2] = {from_f32<T>(lut[w & 15u] * sv * g), from_f32<T>(lut[w >> 4] * sv * g)};
+                uint32_t x;
+                memcpy(&x, v, 4);
+                *reinterpret_cast<uint32_t*>(o) = x;
+            } else {
+                *o = from_f32<T>(lut[w >> shift & 15u] * sv * g);
             }
-            p += p_step;
         }
-        if (first) {
-            const uint8_t* atoms = m.scales + ((long long)tile * m.natoms + c0 / (kNv ? 64 : 128)) * kF4Atom;
-            for (int t = threadIdx.x; t < kF4Tile * nb; t += kQThreads) {
-                const int b = t >> 7, r = t & 127;
-                sc[r * (kBlocks + 1) + b] =
-                    f4_scale_value(kNv, __ldg(atoms + b / 4 * kF4Atom + (r % 32) * 16 + r / 32 * 4 + b % 4));
-            }
-            __syncthreads();
-        }
-#pragma unroll
-        for (int e = 0; e < kBatch; ++e) {
-            if (q < qb) {
-                const float sv = *s;
-                if constexpr (kV >= 4) {
-                    float f[kV];
-                    e2m1_values<kV>(w[e], f);
-                    T v[kV];
-#pragma unroll
-                    for (int i = 0; i < kV; ++i) v[i] = from_f32<T>(f[i] * sv * g);
-                    uint4 x;
-                    memcpy(&x, v, 16);
-                    *reinterpret_cast<uint4*>(o) = x;
-                } else if constexpr (kV == 2) {
-                    T v[2] = {from_f32<T>(e2m1_value(w[e] & 15u) * sv * g), from_f32<T>(e2m1_value(w[e] >> 4) * sv * g)};
-                    uint32_t x;
-                    memcpy(&x, v, 4);
-                    *reinterpret_cast<uint32_t*>(o) = x;
-                } else {
-                    *o = from_f32<T>(e2m1_value(w[e] >> ((u & 1) * 4) & 15u) * sv * g);
-                }
-            }
-            q += groups;
-            s += groups * (kBlocks + 1);
-            o += o_step;
-        }
-        if (q >= qb) break;
     }
 }
 
