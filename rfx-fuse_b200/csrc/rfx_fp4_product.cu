@@ -206,12 +206,14 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
                 T* o = out + (long long)(i0 + cb) * p.ld + j;
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
+                    const int rows = ce - cb - 32 * c;
+                    if (rows >= 32) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        if (cb + 32 * c + e < ce) {
-                            *o = from_f32<T>(__uint_as_float(r[c][e]) * alpha);
-                            o += p.ld;
-                        }
+                        for (int e = 0; e < 32; ++e, o += p.ld) *o = from_f32<T>(__uint_as_float(r[c][e]) * alpha);
+                    } else if (rows > 0) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e, o += p.ld)
+                            if (e < rows) *o = from_f32<T>(__uint_as_float(r[c][e]) * alpha);
                     }
                 }
             }

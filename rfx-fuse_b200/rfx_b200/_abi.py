@@ -164,7 +164,7 @@ def load_library(path: str = LIB_PATH):
     L.rfx_lowrank4_topk.argtypes = [vp, C.c_int, C.c_int, C.c_int, _pi, _pf]
     L.rfx_lowrank4_product.argtypes = [vp, C.c_int, C.c_int, _pf]
     L.rfx_fp4_sizes.argtypes = [C.c_int, C.c_int, C.c_int, C.POINTER(Fp4Layout)]
-    pm, ll = C.POINTER(Fp4Struct), C.c_longlong
+    pm, ll = vp, C.c_longlong  # matrices by address
     L.rfx_fp4_quantize.argtypes = [vp, C.c_int, ll, pm, vp]
     L.rfx_fp4_dequantize.argtypes = [pm, C.c_int, C.c_int, vp, C.c_int, ll, vp]
     L.rfx_fp4_pack.argtypes = [vp, vp, vp, pm, vp]

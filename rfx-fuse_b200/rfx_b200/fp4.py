@@ -26,13 +26,29 @@ TOPK_MAX_COLS = 256
 TOPK_MAX_K = 64
 
 
-_lib = A.load_library
-_Matrix, _Layout = A.Fp4Struct, A.Fp4Layout
+# Bound on first use: torch, its dtypes' codes, the library.
+_torch = None
+_stream = None
+_DTYPES = {}
+_L = None
+
+
+def _load():
+    global _torch, _L, _stream
+    if _L is None:
+        import torch
+        L = A.load_library()
+        _DTYPES.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
+        # the current stream's handle without building a Stream object (3 us of a 14 us call)
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        _stream = raw or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+        _torch = torch
+        _L = L
+    return _L
 
 
 def _dtype_code(dtype):
-    import torch
-    code = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}.get(dtype)
+    code = _DTYPES.get(dtype)
     if code is None:
         raise TypeError(f"dtype must be float32, bfloat16 or float16, not {dtype}")
     return code
@@ -43,51 +59,52 @@ def _check_format(format):
         raise ValueError(f"format must be 'mxfp4' or 'nvfp4', not {format!r}")
 
 
-class _on:
-    """The tensors' device as the current one, and its current stream's handle."""
-
-    def __init__(self, device):
-        import torch
-        self._torch = torch
-        self._device = device
-        self._before = None
-
-    def __enter__(self):
-        cuda = self._torch.cuda
-        before = cuda.current_device()
-        if before != self._device.index:
-            self._before = before
-            cuda.set_device(self._device)
-        return cuda.current_stream(self._device).cuda_stream
-
-    def __exit__(self, *exc):
-        if self._before is not None:
-            self._torch.cuda.set_device(self._before)
+def _call(device, fn, *args):
+    """fn(*args, stream) with the tensors' device current and its current stream."""
+    cuda = _torch.cuda
+    index = device.index
+    before = cuda.current_device()
+    if before == index:
+        rc = fn(*args, _stream(index))
+    else:
+        cuda.set_device(index)
+        try:
+            rc = fn(*args, _stream(index))
+        finally:
+            cuda.set_device(before)
+    if rc:
+        A.check(rc)
 
 
 class Fp4Matrix:
     """A [rows, cols] matrix in 4 bits on a CUDA device.  Made by ``fp4_quantize`` or
     ``from_parts``; its layout is the library's.  Treated as constant once made."""
 
-    __slots__ = ("format", "shape", "device", "_c", "_layout", "_keep")
+    __slots__ = ("format", "shape", "device", "_c", "_p", "_pitch", "_tile_bytes", "_keep")
 
     def __init__(self, *_):
         raise TypeError("use fp4_quantize or Fp4Matrix.from_parts")
 
     @classmethod
     def _empty(cls, rows, cols, format, device):
-        import torch
         m = object.__new__(cls)
-        lay = _Layout()
-        A.check(_lib().rfx_fp4_sizes(FORMATS[format], rows, cols, C.byref(lay)))
-        codes = (lay.codes + 255) & ~255
-        buf = torch.empty(codes + lay.scales + 256 + lay.bounds, dtype=torch.uint8, device=device)
+        # the layout of rfx_fp4_sizes
+        padded = (cols + 63) // 64 * 64
+        tiles = (rows + 127) // 128
+        pitch = padded // 2
+        tile_bytes = 512 * (padded // 64 if format == "nvfp4" else (padded + 127) // 128)
+        codes = (rows * pitch + 255) & ~255
+        scales = tiles * tile_bytes
+        buf = _torch.empty(codes + scales + 256 + 4 * tiles, dtype=_torch.uint8, device=device)
         p = buf.data_ptr()
         m.format, m.shape, m.device = format, (rows, cols), buf.device
-        m._layout, m._keep = lay, buf
-        m._c = _Matrix(FORMATS[format], rows, cols, p, p + codes, p + codes + lay.scales,
-                       p + codes + lay.scales + 256)
+        m._pitch, m._tile_bytes, m._keep = pitch, tile_bytes, buf
+        m._set(A.Fp4Struct(FORMATS[format], rows, cols, p, p + codes, p + codes + scales, p + codes + scales + 256))
         return m
+
+    def _set(self, c):
+        self._c = c
+        self._p = C.addressof(c)
 
     @classmethod
     def from_parts(cls, codes, scales, scale=None, *, cols, format="nvfp4"):
@@ -95,7 +112,8 @@ class Fp4Matrix:
         scale bytes uint8 [rows, ceil(cols / block)] (e8m0 for "mxfp4", unsigned e4m3 for
         "nvfp4") and the matrix scale: a positive number or one-element float32 tensor on the
         same device ("nvfp4" only; None: 1)."""
-        import torch
+        L = _load()
+        torch = _torch
         _check_format(format)
         cols = int(cols)
         if cols < 1:
@@ -119,26 +137,24 @@ class Fp4Matrix:
             if format == "mxfp4" and scale != 1.0:
                 raise ValueError("mxfp4 has no matrix scale")
         m = cls._empty(codes.shape[0], cols, format, codes.device)
-        with _on(m.device) as st:
-            codes, scales = codes.contiguous(), scales.contiguous()
-            if scale is not None and not isinstance(scale, torch.Tensor):
-                scale = None if scale == 1.0 else torch.full((1,), scale, dtype=torch.float32, device=m.device)
-            A.check(_lib().rfx_fp4_pack(codes.data_ptr(), scales.data_ptr(),
-                                        None if scale is None else scale.data_ptr(), C.byref(m._c), st))
+        codes, scales = codes.contiguous(), scales.contiguous()
+        if scale is not None and not isinstance(scale, torch.Tensor):
+            scale = None if scale == 1.0 else torch.full((1,), scale, dtype=torch.float32, device=m.device)
+        _call(m.device, L.rfx_fp4_pack, codes.data_ptr(), scales.data_ptr(),
+              None if scale is None else scale.data_ptr(), m._p)
         return m
 
     def parts(self):
         """(codes, scales, scale), the arguments of ``from_parts``."""
-        import torch
+        torch = _torch
         rows, cols = self.shape
         codes = torch.empty((rows, (cols + 1) // 2), dtype=torch.uint8, device=self.device)
         scales = torch.empty((rows, -(-cols // _BLOCK[self.format])), dtype=torch.uint8, device=self.device)
-        with _on(self.device) as st:
-            A.check(_lib().rfx_fp4_unpack(C.byref(self._c), codes.data_ptr(), scales.data_ptr(), st))
+        _call(self.device, _L.rfx_fp4_unpack, self._p, codes.data_ptr(), scales.data_ptr())
         if self.format == "mxfp4":
             return codes, scales, None
         at = self._c.scale_dev - self._keep.data_ptr()
-        return codes, scales, self._keep[at:at + 4].view(torch.float32).clone()
+        return codes, scales, self._keep[at:at + 4].view(_torch.float32).clone()
 
     def rows(self, begin, end):
         """Rows [begin, end) as a matrix that shares this one's memory; begin a multiple of 128."""
@@ -149,21 +165,20 @@ class Fp4Matrix:
             raise ValueError("a view starts at a multiple of 128 rows")
         m = object.__new__(Fp4Matrix)
         m.format, m.shape, m.device = self.format, (end - begin, self.shape[1]), self.device
-        m._layout, m._keep = self._layout, self._keep
-        c, lay = self._c, self._layout
-        m._c = _Matrix(c.format, end - begin, c.cols, c.codes_dev + begin * lay.pitch,
-                       c.scales_dev + begin // 128 * lay.tile_bytes, c.scale_dev, c.bounds_dev + begin // 128 * 4)
+        m._pitch, m._tile_bytes, m._keep = self._pitch, self._tile_bytes, self._keep
+        c = self._c
+        m._set(A.Fp4Struct(c.format, end - begin, c.cols, c.codes_dev + begin * self._pitch,
+                           c.scales_dev + begin // 128 * self._tile_bytes, c.scale_dev,
+                           c.bounds_dev + begin // 128 * 4))
         return m
 
     def dequantize(self, dtype=None, *, out=None):
         """The values [rows, cols]; exact in float32 and bfloat16 for a quantised matrix."""
-        import torch
-        dtype = torch.float32 if dtype is None and out is None else (out.dtype if dtype is None else dtype)
+        if dtype is None:
+            dtype = _torch.float32 if out is None else out.dtype
         code = _dtype_code(dtype)
         out = _out(out, self.shape, dtype, self.device)
-        with _on(self.device) as st:
-            A.check(_lib().rfx_fp4_dequantize(C.byref(self._c), 0, self.shape[0], out.data_ptr(), code,
-                                              _row_stride(out), st))
+        _call(self.device, _L.rfx_fp4_dequantize, self._p, 0, self.shape[0], out.data_ptr(), code, _row_stride(out))
         return out
 
     def __repr__(self):
@@ -175,10 +190,9 @@ def _row_stride(t):
 
 
 def _out(out, shape, dtype, device):
-    import torch
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    if not isinstance(out, torch.Tensor) or out.device != device or out.dtype != dtype or tuple(out.shape) != tuple(shape):
+        return _torch.empty(shape, dtype=dtype, device=device)
+    if not isinstance(out, _torch.Tensor) or out.device != device or out.dtype != dtype or tuple(out.shape) != tuple(shape):
         raise ValueError(f"out must be a {dtype} tensor of shape {tuple(shape)} on {device}")
     if out.requires_grad:
         raise ValueError("out must not require a gradient")
@@ -196,32 +210,31 @@ def _pair(a, b):
 
 def fp4_quantize(x, format="nvfp4"):
     """x [rows, cols] (CUDA float32, bfloat16 or float16, unit stride along its rows) in 4 bits."""
-    import torch
+    L = _load()
     _check_format(format)
-    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+    if not isinstance(x, _torch.Tensor) or not x.is_cuda:
         raise TypeError("x must be a CUDA tensor")
     if x.dim() != 2 or x.shape[1] < 1:
         raise ValueError("x must be [rows, cols] with at least one column")
     code = _dtype_code(x.dtype)
     rows, cols = x.shape
-    if cols > 1 and x.stride(1) != 1 or rows > 1 and x.stride(0) < cols:
+    s0, s1 = x.stride()
+    if cols > 1 and s1 != 1 or rows > 1 and s0 < cols:
         raise ValueError("x must have unit stride along its rows and rows that do not overlap")
     m = Fp4Matrix._empty(rows, cols, format, x.device)
-    with _on(m.device) as st:
-        A.check(_lib().rfx_fp4_quantize(x.data_ptr(), code, _row_stride(x), C.byref(m._c), st))
+    _call(m.device, L.rfx_fp4_quantize, x.data_ptr(), code, s0 if rows > 1 else cols, m._p)
     return m
 
 
 def fp4_product(a, b, dtype=None, *, out=None):
     """a b^T [a.rows, b.rows]: fp32 accumulation on the tensor cores, rounded once to ``dtype``
     (float32 by default, bfloat16 or float16)."""
-    import torch
     _pair(a, b)
-    dtype = torch.float32 if dtype is None and out is None else (out.dtype if dtype is None else dtype)
+    if dtype is None:
+        dtype = _torch.float32 if out is None else out.dtype
     code = _dtype_code(dtype)
     out = _out(out, (a.shape[0], b.shape[0]), dtype, a.device)
-    with _on(a.device) as st:
-        A.check(_lib().rfx_fp4_product(C.byref(a._c), C.byref(b._c), out.data_ptr(), code, _row_stride(out), st))
+    _call(a.device, _L.rfx_fp4_product, a._p, b._p, out.data_ptr(), code, _row_stride(out))
     return out
 
 
@@ -230,35 +243,38 @@ def fp4_topk(queries, rows, k, *, self_offset=None):
     [queries, k], exact value descending, then index ascending; slots without a neighbour hold
     -1 and -inf.  self_offset: query i is row self_offset + i of ``rows`` and left out for it.
     k <= 64, at most 256 columns."""
-    import torch
     _pair(queries, rows)
     k = int(k)
     if not 1 <= k <= TOPK_MAX_K:
         raise ValueError(f"k must be in [1, {TOPK_MAX_K}]")
     if queries.shape[1] > TOPK_MAX_COLS:
         raise ValueError(f"fp4_topk takes at most {TOPK_MAX_COLS} columns")
+    n = queries.shape[0]
     off = -1
     if self_offset is not None:
         off = int(self_offset)
-        if off < 0 or off + queries.shape[0] > rows.shape[0]:
+        if off < 0 or off + n > rows.shape[0]:
             raise ValueError("self_offset must place the queries inside the rows")
-    L = _lib()
-    idx = torch.empty((queries.shape[0], k), dtype=torch.int32, device=queries.device)
-    val = torch.empty((queries.shape[0], k), dtype=torch.float32, device=queries.device)
-    with _on(queries.device) as st:
-        need = C.c_longlong()
-        A.check(L.rfx_fp4_topk_workspace(C.byref(queries._c), C.byref(rows._c), k, C.byref(need)))
-        ws = torch.empty(need.value, dtype=torch.uint8, device=queries.device)
-        A.check(L.rfx_fp4_topk(C.byref(queries._c), C.byref(rows._c), k, off, idx.data_ptr(), val.data_ptr(),
-                               ws.data_ptr(), need.value, st))
+    need = C.c_longlong()
+    _call(queries.device, _workspace, queries._p, rows._p, k, C.byref(need))
+    torch, device = _torch, queries.device
+    idx = torch.empty((n, k), dtype=torch.int32, device=device)
+    val = torch.empty((n, k), dtype=torch.float32, device=device)
+    ws = torch.empty(need.value, dtype=torch.uint8, device=device)
+    _call(device, _L.rfx_fp4_topk, queries._p, rows._p, k, off, idx.data_ptr(), val.data_ptr(), ws.data_ptr(),
+          need.value)
     return idx, val
+
+
+def _workspace(a, b, k, need, _stream):
+    return _L.rfx_fp4_topk_workspace(a, b, k, need)
 
 
 def fp4_status(device=None):
     """Wait for the device and raise RfxError if a 4-bit product or top-k kernel on it reported a
     pipeline wait that timed out since the last call."""
-    import torch
-    d = torch.device("cuda", torch.cuda.current_device() if device is None else torch.device(device).index
-                     if not isinstance(device, int) else device)
-    with _on(d):
-        A.check(_lib().rfx_fp4_status())
+    _load()
+    d = _torch.device("cuda" if device is None else (("cuda:%d" % device) if isinstance(device, int) else device))
+    if d.index is None:
+        d = _torch.device("cuda", _torch.cuda.current_device())
+    _call(d, lambda _stream: _L.rfx_fp4_status())
