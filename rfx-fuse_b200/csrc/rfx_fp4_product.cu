@@ -6,7 +6,9 @@
 // needs no transpose; the instruction's N holds up to 256 rows of a, and shrinks to the rows
 // there are (16 at least), so that a product of a few rows only reads b.
 //
-// A CTA walks the tiles t = blockIdx.x, + gridDim.x, ...
+// A block takes the tile of its index, then the tiles of blocks that have not started yet, by cluster
+// launch control: some SMs store at three quarters of the others' rate, and equal shares of 43 tiles
+// left those running for 50 us of 185 (1,024 x 200,000 fp32 outputs).
 //   warps 0-7  read an accumulator (quarter warp & 3) and store it.  With up to 128 rows of a the
 //              accumulators form a ring and the two groups of four warps take alternate tiles;
 //              with more, both take the one accumulator, half the columns each, and release it as
@@ -28,6 +30,7 @@ namespace {
 constexpr int kPThreads = 320;
 constexpr int kPMaxStage = 16;
 constexpr int kPSmem = 227 * 1024;
+constexpr int kPSched = 4;
 constexpr int kPBars = 1024;  // barriers and flags
 
 template <int kNv, int kCB, class T>
@@ -44,13 +47,16 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
     auto empty = [&](int s) { return bar0 + 8u * (16 + s); };
     auto accf = [&](int b) { return bar0 + 8u * (32 + b); };
     auto acce = [&](int b) { return bar0 + 8u * (40 + b); };
+    // answers of the tile scheduler: 4 slots of 16 bytes, their full and empty barriers
+    auto sslot = [&](int s) { return bar0 + 512u + 16u * s; };
+    auto sfull = [&](int s) { return bar0 + 576u + 8u * s; };
+    auto sempty = [&](int s) { return bar0 + 608u + 8u * s; };
     const uint32_t stage0 = bar0 + kPBars;
     constexpr int kAtoms = kCB == 32 ? 1 : (kNv ? 4 : 2);  // scale atoms of a whole chunk
     const int nrt = p.bn > kF4Tile ? 2 : 1;                // scale tiles of a's rows
     const uint32_t off_b = 128 * kCB;
     const uint32_t off_sb = off_b + (uint32_t)((p.bn * kCB + 1023) / 1024 * 1024);  // scales of b, then of a
     const uint32_t off_sa = off_sb + kAtoms * kF4Atom;
-    const int ntiles = p.njt * p.nit;
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
@@ -61,6 +67,10 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
         for (int b = 0; b < p.nacc; ++b) {
             mbar_init(accf(b), 1);
             mbar_init(acce(b), p.nacc > 1 ? 4 : 8);  // one arrival a warp
+        }
+        for (int s = 0; s < kPSched; ++s) {
+            mbar_init(sfull(s), 1);
+            mbar_init(sempty(s), 10);  // every warp
         }
         *abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -76,12 +86,30 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
+    RingPos sched;
+    bool ok = true;
+    // the next tile of this warp, or -1
+    auto next_tile = [&]() {
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait_fast(sfull(sched.slot), sched.parity, abort))) {
+            ok = false;
+            return -1;
+        }
+        const int t = __shfl_sync(0xFFFFFFFFu, clc_answer(sslot(sched.slot)), 0);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(sempty(sched.slot));
+        sched.next(kPSched);
+        return t;
+    };
 
     if (warp == 8) {
         int step = 0;
         RingPos st;
-        bool ok = true;
-        for (int t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
+        bool asked = false;
+        for (int t = blockIdx.x; ok && t >= 0; t = ok ? next_tile() : -1) {
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(sempty(sched.slot), sched.parity ^ 1u, abort));
+            if (!ok) break;
+            if (elect_one()) clc_request(sslot(sched.slot), sfull(sched.slot));
+            asked = true;
             const int jt = t % p.njt, i0 = t / p.njt * p.bn;
             const int rt0 = i0 / kF4Tile;
             const int rts = min(nrt, p.a.tiles() - rt0);
@@ -113,7 +141,8 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
             if (!*abort) atomicExch(p.err, 1);
             *abort = 1;
         }
-        // drain this warp's copies still in flight
+        // drain this warp's answer and copies still in flight (after next_tile the answer has been read)
+        if (!ok && asked) mbar_wait<false>(sfull(sched.slot), sched.parity, nullptr);
         for (int i = step > p.nstage ? step - p.nstage : 0; i < step; ++i)
             mbar_wait<false>(full(i % p.nstage), (uint32_t)(i / p.nstage) & 1u, nullptr);
         __syncwarp();
@@ -121,9 +150,8 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
         RingPos st, ac;
         int last = -1;
         uint32_t last_parity = 0;
-        bool ok = true;
         const uint32_t sfc = (uint32_t)(4 * kAtoms * (1 + nrt));  // TMEM columns of a stage's scales
-        for (int t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
+        for (int t = blockIdx.x; ok && t >= 0; t = ok ? next_tile() : -1) {
             ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(acce(ac.slot), ac.parity ^ 1u, abort));
             if (!ok) break;
             tc_fence_after();
@@ -177,16 +205,13 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
         const uint32_t lane_addr = (uint32_t)(32 * (warp & 3)) << 16;
         const float alpha = __ldg(p.a.gs) * __ldg(p.b.gs);
         T* out = (T*)p.out;
+        RingPos ac;
         int n = 0;
-        for (int t = blockIdx.x; t < ntiles; t += gridDim.x, ++n) {
+        for (int t = blockIdx.x; t >= 0; t = next_tile(), ++n, ac.next(p.nacc)) {
             if (p.nacc > 1 && (n & 1) != group) continue;
-            const int b = n % p.nacc;
-            const int w = mbar_wait<false>(accf(b), (uint32_t)(n / p.nacc) & 1u, abort);
-            if (__any_sync(0xFFFFFFFFu, w != kWaitOk)) {
-                if (!*abort) atomicExch(p.err, 3);
-                *abort = 1;
-                break;
-            }
+            const int b = ac.slot;
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(accf(b), ac.parity, abort));
+            if (!ok) break;
             tc_fence_after();
             const int jt = t % p.njt, i0 = t / p.njt * p.bn;
             const int cb = p.nacc > 1 ? 0 : 128 * group;   // first of this warp's columns (rows of a)
@@ -218,6 +243,10 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
                 }
             }
             __syncwarp();
+        }
+        if (!ok && lane == 0) {
+            if (!*abort) atomicExch(p.err, 3);
+            *abort = 1;
         }
     }
     tc_fence_before();
@@ -271,7 +300,7 @@ cudaError_t f4_product(const F4& a, const F4& b, void* out, int dtype, long long
     while (p.acc_cols < p.bn) p.acc_cols *= 2;
     p.nacc = 256 / p.acc_cols;
     const long long ntiles = (long long)p.nit * p.njt;
-    const int grid = (int)std::min<long long>(ntiles, sms);
+    const int grid = (int)ntiles;
     CUtensorMap ta, tb;
     if (!f4_map(&ta, a, p.bn, cb) || !f4_map(&tb, b, 128, cb)) return cudaErrorInvalidValue;
     *launches += 1;

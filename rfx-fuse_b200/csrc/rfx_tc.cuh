@@ -127,6 +127,32 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
+// Work by cluster launch control: a running block takes over the index of one that has not started.
+// The 16-byte answer arrives in shared memory at `slot`, completing on `bar`.
+__device__ __forceinline__ void clc_request(uint32_t slot, uint32_t bar) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // after the last answer's readers
+    mbar_expect_tx(bar, 16);
+    asm volatile(
+        "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(slot),
+        "r"(bar)
+        : "memory");
+}
+// The block index taken over, or -1 when none was left (no further request may follow).
+__device__ __forceinline__ int clc_answer(uint32_t slot) {
+    uint32_t ok, x;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b128 h;\n\t.reg .b32 y, z, w;\n\t"
+        "ld.shared.b128 h, [%2];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "mov.u32 %1, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, y, z, w}, h;\n\t}\n"
+        : "=r"(ok), "=r"(x)
+        : "r"(slot)
+        : "memory");
+    return ok ? (int)x : -1;
+}
+
 // 2-D tiled TMA load (box 64 x 128 of bf16) into shared memory, completing on `bar`.
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* tm, int x, int y,
                                          uint32_t bar) {
