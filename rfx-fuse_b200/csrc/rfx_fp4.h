@@ -78,6 +78,7 @@ struct F4ProductArgs {
     int dtype;        // RFX_F32 / RFX_BF16 / RFX_F16
     int bn;           // rows of a in a tile (multiple of 16, <= 256)
     int njt, nit;     // tiles of b and of a (njt * nit < 2^31)
+    int ntiles, group; // their number, tiles of a unit of scheduling
     int nchunk;       // chunks of the inner axis
     int nstage, nacc; // shared-memory ring, accumulator ring
     int acc_cols;     // TMEM columns of an accumulator

@@ -6,7 +6,7 @@
 // needs no transpose; the instruction's N holds up to 256 rows of a, and shrinks to the rows
 // there are (16 at least), so that a product of a few rows only reads b.
 //
-// A block takes the tile of its index, then the tiles of blocks that have not started yet, by cluster
+// A block takes the unit (p.group neighbouring tiles) of its index, then the units of blocks that have not started yet, by cluster
 // launch control: some SMs store at three quarters of the others' rate, and equal shares of 43 tiles
 // left those running for 50 us of 185 (1,024 x 200,000 fp32 outputs).
 //   warps 0-7  read an accumulator (quarter warp & 3) and store it.  With up to 128 rows of a the
@@ -88,8 +88,8 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
     RingPos sched;
     bool ok = true;
-    // the next tile of this warp, or -1
-    auto next_tile = [&]() {
+    // the next unit of this warp, or -1
+    auto next_unit = [&]() {
         if (!__all_sync(0xFFFFFFFFu, mbar_wait_fast(sfull(sched.slot), sched.parity, abort))) {
             ok = false;
             return -1;
@@ -105,11 +105,12 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
         int step = 0;
         RingPos st;
         bool asked = false;
-        for (int t = blockIdx.x; ok && t >= 0; t = ok ? next_tile() : -1) {
+        for (int unit = blockIdx.x; ok && unit >= 0; unit = ok ? next_unit() : -1) {
             ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(sempty(sched.slot), sched.parity ^ 1u, abort));
             if (!ok) break;
             if (elect_one()) clc_request(sslot(sched.slot), sfull(sched.slot));
             asked = true;
+            for (int t = unit * p.group, te = min(t + p.group, p.ntiles); ok && t < te; ++t) {
             const int jt = t % p.njt, i0 = t / p.njt * p.bn;
             const int rt0 = i0 / kF4Tile;
             const int rts = min(nrt, p.a.tiles() - rt0);
@@ -136,6 +137,7 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
                 sa += kAtoms * kF4Atom;
                 st.next(p.nstage);
             }
+            }
         }
         if (!ok && lane == 0) {
             if (!*abort) atomicExch(p.err, 1);
@@ -151,7 +153,8 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
         int last = -1;
         uint32_t last_parity = 0;
         const uint32_t sfc = (uint32_t)(4 * kAtoms * (1 + nrt));  // TMEM columns of a stage's scales
-        for (int t = blockIdx.x; ok && t >= 0; t = ok ? next_tile() : -1) {
+        for (int unit = blockIdx.x; ok && unit >= 0; unit = ok ? next_unit() : -1) {
+            for (int t = unit * p.group, te = min(t + p.group, p.ntiles); ok && t < te; ++t) {
             ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(acce(ac.slot), ac.parity ^ 1u, abort));
             if (!ok) break;
             tc_fence_after();
@@ -191,6 +194,7 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
                 st.next(p.nstage);
             }
             ac.next(p.nacc);
+            }
         }
         if (!ok && lane == 0) {
             if (!*abort) atomicExch(p.err, 2);
@@ -207,7 +211,8 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
         T* out = (T*)p.out;
         RingPos ac;
         int n = 0;
-        for (int t = blockIdx.x; t >= 0; t = next_tile(), ++n, ac.next(p.nacc)) {
+        for (int unit = blockIdx.x; ok && unit >= 0; unit = ok ? next_unit() : -1) {
+            for (int t = unit * p.group, te = min(t + p.group, p.ntiles); t < te; ++t, ++n, ac.next(p.nacc)) {
             if (p.nacc > 1 && (n & 1) != group) continue;
             const int b = ac.slot;
             ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(accf(b), ac.parity, abort));
@@ -237,12 +242,18 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
                         for (int e = 0; e < 32; ++e, o += p.ld) *o = from_f32<T>(__uint_as_float(r[c][e]) * alpha);
                     } else if (rows > 0) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e, o += p.ld)
-                            if (e < rows) *o = from_f32<T>(__uint_as_float(r[c][e]) * alpha);
+                        for (int f = 0; f < 32; f += 4) {  // few rows leave most of these branches
+                            if (f < rows) {
+#pragma unroll
+                                for (int e = f; e < f + 4; ++e, o += p.ld)
+                                    if (e < rows) *o = from_f32<T>(__uint_as_float(r[c][e]) * alpha);
+                            }
+                        }
                     }
                 }
             }
             __syncwarp();
+            }
         }
         if (!ok && lane == 0) {
             if (!*abort) atomicExch(p.err, 3);
@@ -300,7 +311,11 @@ cudaError_t f4_product(const F4& a, const F4& b, void* out, int dtype, long long
     while (p.acc_cols < p.bn) p.acc_cols *= 2;
     p.nacc = 256 / p.acc_cols;
     const long long ntiles = (long long)p.nit * p.njt;
-    const int grid = (int)ntiles;
+    p.ntiles = (int)ntiles;
+    // a tile of few rows takes less than a request for the next one: several to a unit, eight units
+    // a block; else single tiles, which balance best
+    p.group = p.bn > 64 ? 1 : (int)std::max(1ll, std::min(8ll, ntiles / (8ll * sms)));
+    const int grid = (p.ntiles + p.group - 1) / p.group;
     CUtensorMap ta, tb;
     if (!f4_map(&ta, a, p.bn, cb) || !f4_map(&tb, b, 128, cb)) return cudaErrorInvalidValue;
     *launches += 1;
