@@ -60,18 +60,23 @@ __device__ __forceinline__ uint32_t cvt_e2m1x4(const float* v) {
     return d & 0xFFFFu;
 }
 
-// Twice the magnitudes (0, 1, 2, 3, 4, 6, 8, 12) of the four codes in the low half of w, as bytes.
-__device__ __forceinline__ uint32_t e2m1_mag4(uint32_t w) {
-    return __byte_perm(0x03020100u, 0x0C080604u, w & 0x7777u);
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
+    uint32_t d;  // (__byte_perm drops the selectors' top bits)
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(sel));
+    return d;
 }
+
+// Twice the magnitudes (0, 1, 2, 3, 4, 6, 8, 12) of those of the four codes in the low half of w
+// that have no sign, as bytes; 0 for the others: a selector with its top bit set replicates the
+// sign of the byte it selects, and no byte here has one.  With w ^ 0x8888: of those that have one.
+__device__ __forceinline__ uint32_t e2m1_pos4(uint32_t w) { return prmt(0x03020100u, 0x0C080604u, w); }
+// Of all four.
+__device__ __forceinline__ uint32_t e2m1_mag4(uint32_t w) { return e2m1_pos4(w & 0x7777u); }
 
 // 0x7F in the bytes whose code (low half of w) has its sign bit set, else 0.
 __device__ __forceinline__ uint32_t e2m1_neg4(uint32_t w) {
-    // a selector of 8 replicates the sign of byte 0 (0xFF), 0 copies it (0x80); __byte_perm drops
-    // the selectors' top bits
-    uint32_t d;
-    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(0x80u), "r"(0u), "r"(w & 0x8888u));
-    return d & 0x7F7F7F7Fu;
+    // a selector of 8 replicates the sign of byte 0 (0xFF), 0 copies it (0x80)
+    return prmt(0x80u, 0u, w & 0x8888u) & 0x7F7F7F7Fu;
 }
 
 // The values of kN (4 or 8) codes in a word, through the upper bytes of their fp16 forms.
@@ -96,15 +101,14 @@ __device__ __forceinline__ float e2m1_value(uint32_t code) {
     return (code & 8u) ? -m : m;
 }
 
-// Four times the dot product of eight codes with eight codes, exactly.
-__device__ __forceinline__ int e2m1_dot8(uint32_t a, uint32_t b, int acc) {
-    const uint32_t s = a ^ b;
-    const uint32_t mb0 = e2m1_mag4(b), mb1 = e2m1_mag4(b >> 16);
-    const uint32_t ma0 = e2m1_mag4(a), ma1 = e2m1_mag4(a >> 16);
-    uint32_t all = __dp4a(ma0, mb0, 0u), neg = __dp4a(ma0, mb0 & e2m1_neg4(s), 0u);
-    all = __dp4a(ma1, mb1, all);
-    neg = __dp4a(ma1, mb1 & e2m1_neg4(s >> 16), neg);
-    return acc + (int)all - 2 * (int)neg;
+// acc + four times the dot product of eight codes (decoded as signed bytes of twice their values, q
+// four, r the next four) with the eight codes of w, exactly.
+__device__ __forceinline__ int e2m1_dot8(int q, int r, uint32_t w, int acc) {
+    const uint32_t x = w ^ 0x88888888u;
+    acc = __dp4a(q, (int)e2m1_pos4(w), acc);
+    acc = __dp4a(r, (int)e2m1_pos4(w >> 16), acc);
+    const int neg = __dp4a(r, (int)e2m1_pos4(x >> 16), __dp4a(q, (int)e2m1_pos4(x), 0));
+    return acc - neg;
 }
 
 template <class T> __device__ __forceinline__ float to_f32(T v);

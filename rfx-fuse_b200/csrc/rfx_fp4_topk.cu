@@ -34,10 +34,7 @@ constexpr int kSpan = 6;                     // tiles of b in a unit of work: tw
 constexpr int kSpanKeys = 4 * kSpan;         // keys of a row and a span
 constexpr float kEps = 1.0f / 32768.0f;
 constexpr uint32_t kAlways = 0xFFFFu;        // key of a chunk that has to be looked at (no float's)
-constexpr int kScan = 256;                   // units a round turns into chunks
-constexpr int kList = 8 * kScan + 256;       // chunks waiting for their evaluation
-constexpr int kUnits = 4096;                 // units of keys: a key, or every 4096th vector of 8
-constexpr int kFound = 1024;                 // values waiting to be ranked
+constexpr int kSmallKeys = 1024;             // keys of a row that 128 threads take
 
 struct KeysArgs {
     F4 a, b;
@@ -388,13 +385,6 @@ __device__ __forceinline__ bool f4_better(double va, int ja, double vb, int jb) 
     return va > vb || (va == vb && ja < jb);
 }
 
-// 4 x the dot product of four decoded codes (signed bytes, doubled) with the four codes in the
-// low half of w.
-__device__ __forceinline__ int dot4(int qa, uint32_t w, int acc) {
-    const uint32_t m = e2m1_mag4(w);
-    return __dp4a(qa, (int)m, acc) - 2 * __dp4a(qa, (int)(m & e2m1_neg4(w)), 0);
-}
-
 // Four times the exact value of the row (decoded in qa, scales in sa) with a row of b (codes cb,
 // first scale sb), without the matrix scales; NaN when a scale is.
 template <int kNv>
@@ -407,13 +397,8 @@ __device__ __noinline__ double f4_exact(const int* qa, const float* sa, const ui
         for (int h = 0; h < 2; ++h) {  // 32 columns
             const uint4 y = __ldg(cb + 2 * c + h);
             const int* q = qa + 16 * c + 8 * h;
-            int lo = dot4(q[0], y.x, 0), hi = dot4(q[4], y.z, 0);
-            lo = dot4(q[1], y.x >> 16, lo);
-            hi = dot4(q[5], y.z >> 16, hi);
-            lo = dot4(q[2], y.y, lo);
-            hi = dot4(q[6], y.w, hi);
-            lo = dot4(q[3], y.y >> 16, lo);
-            hi = dot4(q[7], y.w >> 16, hi);
+            const int lo = e2m1_dot8(q[2], q[3], y.y, e2m1_dot8(q[0], q[1], y.x, 0));
+            const int hi = e2m1_dot8(q[6], q[7], y.w, e2m1_dot8(q[4], q[5], y.z, 0));
             if (kNv) {
                 // e4m3 times e4m3 times the integer: exact, and so is every sum
                 v += (double)sa[4 * c + 2 * h] * (double)e4m3_value((wb >> (16 * h)) & 0xFFu) * (double)lo;
@@ -438,36 +423,28 @@ __device__ __forceinline__ float f4_estimate64(const int* qa, const float* sa, u
         const uint4 y = h ? y1 : y0;
         const int4 q0 = *reinterpret_cast<const int4*>(qa + 8 * h);
         const int4 q1 = *reinterpret_cast<const int4*>(qa + 8 * h + 4);
-        int lo = 0, hi = 0, nlo = 0, nhi = 0;  // all terms, and those of negative codes
-        const int qs[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
-        const uint32_t ws[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const uint32_t w = (e & 1) ? ws[e >> 1] >> 16 : ws[e >> 1];
-            const uint32_t m = e2m1_mag4(w);
-            const uint32_t mn = m & e2m1_neg4(w);
-            if (e < 4) {
-                lo = __dp4a(qs[e], (int)m, lo);
-                nlo = __dp4a(qs[e], (int)mn, nlo);
-            } else {
-                hi = __dp4a(qs[e], (int)m, hi);
-                nhi = __dp4a(qs[e], (int)mn, nhi);
-            }
-        }
+        const int lo = e2m1_dot8(q0.z, q0.w, y.y, e2m1_dot8(q0.x, q0.y, y.x, 0));
+        const int hi = e2m1_dot8(q1.z, q1.w, y.w, e2m1_dot8(q1.x, q1.y, y.z, 0));
         if (kNv) {
-            v = fmaf(sa[2 * h] * e4m3_value((wb >> (16 * h)) & 0xFFu), (float)(lo - 2 * nlo), v);
-            v = fmaf(sa[2 * h + 1] * e4m3_value((wb >> (16 * h + 8)) & 0xFFu), (float)(hi - 2 * nhi), v);
+            v = fmaf(sa[2 * h] * e4m3_value((wb >> (16 * h)) & 0xFFu), (float)lo, v);
+            v = fmaf(sa[2 * h + 1] * e4m3_value((wb >> (16 * h + 8)) & 0xFFu), (float)hi, v);
         } else {
-            v = fmaf(sa[h] * e8m0_value((wb >> (8 * h)) & 0xFFu), (float)(lo + hi - 2 * (nlo + nhi)), v);
+            v = fmaf(sa[h] * e8m0_value((wb >> (8 * h)) & 0xFFu), (float)(lo + hi), v);
         }
     }
     return v;
 }
 
-// kT threads a row: 256, several rows an SM; 1024 when there are too few rows to fill the GPU.
+// kT threads a row: 256, four rows an SM; 128, eight rows an SM, when a row has few keys (each step
+// then waits for memory or a barrier, and rows hide one another's waits: 10,000 x 10,000 top-10
+// 136 us with 256); 1024 when there are too few rows to fill the GPU.
 template <int kNv, int kT>
-__global__ void __launch_bounds__(kT, kT == 256 ? 4 : 1)
+__global__ void __launch_bounds__(kT, kT == 1024 ? 1 : 1024 / kT)
 k_f4_pick(PickArgs p) {
+    constexpr int kUnits = kT == 128 ? kSmallKeys : 4096;  // units of keys: a key, or every kUnits-th vector of 8
+    constexpr int kFound = kT == 128 ? 512 : 1024;         // columns waiting to be ranked
+    constexpr int kScan = kT == 128 ? 128 : 256;           // units a round turns into chunks
+    constexpr int kList = (kT == 128 ? 1 : 8) * kScan + 256;  // chunks waiting to be looked at
     __shared__ __align__(16) int qa[kF4TopkK / 4];
     __shared__ float sa[kF4TopkK / 16];
     __shared__ double fv[kFound];       // found: values (4 x) of the first n_known, columns of all
@@ -492,7 +469,7 @@ k_f4_pick(PickArgs p) {
     auto scales_of = [=](int j) {
         return b_scales + (long long)(j >> 7) * tile_bytes + (j & 31) * 16 + ((j >> 5) & 3) * 4;
     };
-    const bool small = nvec * 8 <= kUnits;       // a unit is a key
+    const bool small = kT == 128 || nvec * 8 <= kUnits;  // a unit is a key
     const int nunits = small ? nvec * 8 : min(nvec, kUnits);
 
     // the largest key of every unit, four vectors in flight; thread t owns the units t, t + kT, ...
@@ -673,7 +650,7 @@ k_f4_pick(PickArgs p) {
             }
         }
         __syncthreads();
-        const bool room = n_list <= kList - 8 * kScan;
+        const bool room = n_list <= 256;
         __syncthreads();  // everyone has read n_list before anyone adds to it
         if (!room) look();
     }
@@ -768,10 +745,13 @@ cudaError_t f4_topk(const F4& a, const F4& b, int k, long long self, int* idx, f
         if (e != cudaSuccess) return e;
         q.row0 = (int)r0;
         q.nerrs = grid;
-        const int threads = rows <= 2 * sms ? 1024 : 256;
+        const int threads = rows <= 2 * sms ? 1024 : plan.nspan * kSpanKeys <= kSmallKeys ? 128 : 256;
         if (threads == 1024) {
             if (b.nv) k_f4_pick<1, 1024><<<rows, 1024, 0, st>>>(q);
             else k_f4_pick<0, 1024><<<rows, 1024, 0, st>>>(q);
+        } else if (threads == 128) {
+            if (b.nv) k_f4_pick<1, 128><<<rows, 128, 0, st>>>(q);
+            else k_f4_pick<0, 128><<<rows, 128, 0, st>>>(q);
         } else {
             if (b.nv) k_f4_pick<1, 256><<<rows, 256, 0, st>>>(q);
             else k_f4_pick<0, 256><<<rows, 256, 0, st>>>(q);
