@@ -583,43 +583,58 @@ k_f4_pick(PickArgs p) {
         if (n_known == p.k) floor_v = fmax(floor_v, 0.25 * fv[p.k - 1]);
         __syncthreads();
     };
-    // Looks at the chunks of the list, a lane a column, as many at a time as surely have room.
+    // Looks at the chunks [c0, c1) of the list, a warp a chunk, a lane a column; what overflows is
+    // only counted.
+    auto look_at = [&](int c0, int c1) {
+        const float least = 4.0f * __double2float_rd(floor_v - err);
+        // the next chunk's first 64 columns are loaded under this one's arithmetic
+        uint4 y0, y1;
+        uint32_t sc;
+        auto fetch = [&](int c) {
+            const int j = min((int)list[c] * 32 + lane, p.b.rows - 1);
+            y0 = __ldg(codes_of(j));
+            y1 = __ldg(codes_of(j) + 1);
+            sc = __ldg(reinterpret_cast<const uint32_t*>(scales_of(j)));
+        };
+        if (c0 + warp < c1) fetch(c0 + warp);
+        for (int c = c0 + warp; c < c1; c += kT / 32) {
+            const int j = (int)list[c] * 32 + lane;
+            const uint4 z0 = y0, z1 = y1;
+            const uint32_t zs = sc;
+            if (c + kT / 32 < c1) fetch(c + kT / 32);
+            float v = f4_estimate64<kNv>(qa, sa, z0, z1, zs, 0.0f);
+            for (int st = 1; st < steps; ++st) {
+                const int jc = min(j, p.b.rows - 1);
+                const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(scales_of(jc) + (kNv ? st : st >> 1) * kF4Atom));
+                v = f4_estimate64<kNv>(qa + 16 * st, sa + (kNv ? 4 : 2) * st, __ldg(codes_of(jc) + 2 * st),
+                                       __ldg(codes_of(jc) + 2 * st + 1), !kNv && (st & 1) ? w >> 16 : w, v);
+            }
+            // without a bound on the terms fp32 could overflow: rank_found decides
+            if (j < p.b.rows && j != self && (forced || v >= least)) {
+                const int at = atomicAdd(&n_found, 1);
+                if (at < kFound) fj[at] = j;
+            }
+        }
+        __syncthreads();
+    };
+    // The whole list; where that finds more than there is room for (ties in masses), again from the
+    // start, as many chunks at a time as surely have room.
     auto look = [&]() {
         __syncthreads();
-        const int n = n_list;
-        for (int c0 = 0; c0 < n;) {
-            const int room = (kFound - n_found) / 32;
-            __syncthreads();  // everyone has read n_found before anyone adds to it
-            const int c1 = min(n, c0 + room);
-            const float least = 4.0f * __double2float_rd(floor_v - err);
-            // the next chunk's first 64 columns are loaded under this one's arithmetic
-            uint4 y0, y1;
-            uint32_t sc;
-            auto fetch = [&](int c) {
-                const int j = min((int)list[c] * 32 + lane, p.b.rows - 1);
-                y0 = __ldg(codes_of(j));
-                y1 = __ldg(codes_of(j) + 1);
-                sc = __ldg(reinterpret_cast<const uint32_t*>(scales_of(j)));
-            };
-            if (c0 + warp < c1) fetch(c0 + warp);
-            for (int c = c0 + warp; c < c1; c += kT / 32) {
-                const int j = (int)list[c] * 32 + lane;
-                const uint4 z0 = y0, z1 = y1;
-                const uint32_t zs = sc;
-                if (c + kT / 32 < c1) fetch(c + kT / 32);
-                float v = f4_estimate64<kNv>(qa, sa, z0, z1, zs, 0.0f);
-                for (int st = 1; st < steps; ++st) {
-                    const int jc = min(j, p.b.rows - 1);
-                    const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(scales_of(jc) + (kNv ? st : st >> 1) * kF4Atom));
-                    v = f4_estimate64<kNv>(qa + 16 * st, sa + (kNv ? 4 : 2) * st, __ldg(codes_of(jc) + 2 * st),
-                                           __ldg(codes_of(jc) + 2 * st + 1), !kNv && (st & 1) ? w >> 16 : w, v);
-                }
-                // without a bound on the terms fp32 could overflow: rank_found decides
-                if (j < p.b.rows && j != self && (forced || v >= least)) fj[atomicAdd(&n_found, 1)] = j;
-            }
-            c0 = c1;
-            if (c0 < n) rank_found();
+        const int n = n_list, before = n_found;
+        __syncthreads();  // everyone has read n_found before anyone adds to it
+        look_at(0, n);
+        if (n_found > kFound) {
             __syncthreads();
+            if (tid == 0) n_found = before;
+            __syncthreads();
+            for (int c0 = 0; c0 < n;) {
+                const int c1 = min(n, c0 + (kFound - n_found) / 32);
+                __syncthreads();
+                look_at(c0, c1);
+                c0 = c1;
+                rank_found();
+            }
         }
         if (tid == 0) n_list = 0;
         __syncthreads();

@@ -298,3 +298,43 @@ def test_estimator_in_4_bits(fmt):
     for c in range(0, 24, bs):
         big = np.abs(A8[:, c:c + bs]).max(1, keepdims=True) + step
         assert (np.abs(A[:, c:c + bs] - A8[:, c:c + bs]) <= big / 3 + step).all()
+
+
+@pytest.mark.parametrize("fmt,m,n,k,top", [("nvfp4", 320, 40000, 64, 50), ("mxfp4", 300, 140000, 40, 64), ("nvfp4", 310, 3000, 130, 64),
+                                           ("mxfp4", 2, 1200000, 20, 50)])
+def test_topk_many_rows(fmt, m, n, k, top):
+    """The forms the selection takes by rows of a and keys of a row (units of one key, of eight, of
+    several vectors), with duplicated rows; a sample of the queries is checked."""
+    import rfx_b200
+    rng = np.random.default_rng(n)
+    ca, sa = _parts(rng, m, k, fmt, spread=2)
+    cb, sb = _parts(rng, n, k, fmt, spread=2)
+    src = rng.integers(0, n, 3000)
+    dst = rng.integers(0, n, 3000)
+    cb[dst], sb[dst] = cb[src], sb[src]
+    a, b = _matrix(ca, sa, k, fmt), _matrix(cb, sb, k, fmt)
+    idx, val = rfx_b200.fp4_topk(a, b, top)
+    rfx_b200.fp4_status()
+    pick = np.unique(np.concatenate([[0, m - 1], rng.integers(0, m, 12)]))
+    wi, wv = ref.topk(ref.values(ca[pick], sa[pick], 1.0, fmt), ref.values(cb, sb, 1.0, fmt), top, None, fmt)
+    assert np.array_equal(idx.cpu().numpy()[pick], wi)
+    assert np.array_equal(val.cpu().numpy()[pick], wv)
+
+
+def test_topk_masses_of_ties():
+    """Few distinct rows, each thousands of times: more columns reach the bar than the selection has
+    room for at once, in each of its forms."""
+    import rfx_b200
+    rng = np.random.default_rng(12)
+    for m, n in ((3, 50000), (300, 40000), (300, 20000)):
+        c, s = _parts(rng, 7, 64, "nvfp4", spread=1)
+        which = rng.integers(0, 7, n)
+        cb, sb = c[which], s[which]
+        a, b = _matrix(cb[:m], sb[:m], 64, "nvfp4"), _matrix(cb, sb, 64, "nvfp4")
+        idx, val = rfx_b200.fp4_topk(a, b, 33, self_offset=0)
+        rfx_b200.fp4_status()
+        pick = np.array([0, 1, m - 1])
+        vb = ref.values(cb, sb, 1.0, "nvfp4")
+        for i in pick:
+            wi, wv = ref.topk(vb[i:i + 1], vb, 33, int(i), "nvfp4")
+            assert np.array_equal(idx[i].cpu().numpy(), wi[0]) and np.array_equal(val[i].cpu().numpy(), wv[0])
