@@ -137,7 +137,7 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
+    constexpr uint32_t tmem = 0;  // all 512 columns are this block's: they start at column 0
     const int steps = p.b.Kp / 64;
     const int atoms = kNv ? steps : (steps + 1) / 2;
 
@@ -191,17 +191,15 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
         RingPos st, sl;
         uint32_t uses = 0;  // a parity bit for every accumulator
         int last = -1;
-        bool ok = true;
         uint32_t tsa = 0;
         uint64_t da = 0;
         int span = (int)(u0 % p.nspan);
-        for (int u = 0; ok && u < nu; ++u) {
+        for (int u = 0; u < nu; ++u) {
             if (u == 0 || span == 0) {
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(afull(sl.slot), sl.parity, abort));
-                if (!ok) break;
+                mbar_wait_issue(afull(sl.slot), sl.parity, abort, p.err, 2);
                 tc_fence_after();
                 const uint32_t src = slot0 + (uint32_t)(sl.slot * kSlot);
-                tsa = tmem + 384u + (uint32_t)(4 * kAtoms * sl.slot);
+                tsa = 384u + (uint32_t)(4 * kAtoms * sl.slot);
                 if (elect_one())
                     for (int k0 = 0; k0 < atoms; ++k0) f4_copy_atom(tsa + 4 * k0, f4_atom_desc(src + kBox + k0 * kF4Atom));
                 da = f4_operand_desc<kCB>(src);
@@ -209,24 +207,21 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
             const int nt = min(kSpan, p.ntiles - span * kSpan);
 #pragma unroll
             for (int t = 0; t < kSpan; t += 2) {
-                if (t >= nt || !ok) break;
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(full(st.slot), st.parity, abort));
-                if (!ok) break;
-                tc_fence_after();
+                if (t >= nt) break;
+                mbar_wait_issue(full(st.slot), st.parity, abort, p.err, 2);
                 const uint32_t src = ring0 + (uint32_t)(st.slot * kStage);
-                const uint32_t tsb = tmem + 384u + (uint32_t)(8 * kAtoms * (1 + st.slot));
+                const uint32_t tsb = 384u + (uint32_t)(8 * kAtoms * (1 + st.slot));
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     if (t + h >= nt) break;
                     const int ac = (t + h) % kAccs;
-                    const uint32_t tsh = tsb + 4 * kAtoms * h;
-                    const uint64_t dsc = f4_atom_desc(src + 2 * kBox + h * atoms * kF4Atom);
-                    const uint64_t db = f4_operand_desc<kCB>(src + h * kBox);
-                    ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(acce(ac), ((uses >> ac) & 1u) ^ 1u, abort));
-                    if (!ok) break;
+                    mbar_wait_issue(acce(ac), ((uses >> ac) & 1u) ^ 1u, abort, p.err, 2);
                     tc_fence_after();
-                    const uint32_t d = tmem + (uint32_t)(128 * ac);
                     if (elect_one()) {
+                        const uint32_t tsh = tsb + 4 * kAtoms * h;
+                        const uint64_t dsc = f4_atom_desc(src + 2 * kBox + h * atoms * kF4Atom);
+                        const uint64_t db = f4_operand_desc<kCB>(src + h * kBox);
+                        const uint32_t d = (uint32_t)(128 * ac);
                         if (kCB == 32) {
                             f4_copy_atom(tsh, dsc);
                             f4_mma<kNv>(d, da, db, f4_idesc<kNv>(128, 0), tsa, tsh, 0u);
@@ -241,20 +236,18 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
                         mma_commit(accf(ac));
                         if (h == 1 || t + 1 >= nt) mma_commit(empty(st.slot));
                     }
+                    __syncwarp();
                     last = ac;
                     uses ^= 1u << ac;
                 }
                 st.next(kStages);
             }
             if (++span == p.nspan) span = 0;
-            if (ok && (span == 0 || u == nu - 1)) {
+            if (span == 0 || u == nu - 1) {
                 if (elect_one()) mma_commit(aempty(sl.slot));
+                __syncwarp();
                 sl.next(2);
             }
-        }
-        if (!ok && lane == 0) {
-            if (!*abort) atomicExch(p.err, 2);
-            *abort = 1;
         }
         // the last products must finish before the accumulators are freed
         if (last >= 0) mbar_wait<false>(accf(last), ((uses >> last) & 1u) ^ 1u, nullptr);
@@ -376,7 +369,7 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
     __syncthreads();
     if (warp == 13) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "r"(512)
                      : "memory");
     }
 }

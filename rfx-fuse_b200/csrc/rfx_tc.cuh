@@ -78,6 +78,20 @@ __device__ __forceinline__ bool mbar_wait_fast(uint32_t bar, uint32_t parity, vo
     return mbar_try<false>(bar, parity) || mbar_wait_slow(bar, parity, abort);
 }
 
+// For the issuing warps: no result, so that their control flow stays uniform.  A wait that runs out
+// records `code` in *err and sets *abort, after which every wait returns at once: the warp runs
+// through the rest of its loop on whatever the buffers hold, and the call ends with its error.
+__device__ __noinline__ void mbar_wait_issue_slow(uint32_t bar, uint32_t parity, volatile int* abort, int* err, int code) {
+    if (mbar_wait<false>(bar, parity, abort) != kWaitOk && !*abort) {
+        atomicExch(err, code);
+        *abort = 1;
+    }
+}
+__device__ __forceinline__ void mbar_wait_issue(uint32_t bar, uint32_t parity, volatile int* abort, int* err, int code) {
+    if (!mbar_try<false>(bar, parity)) mbar_wait_issue_slow(bar, parity, abort, err, code);
+    __syncwarp();
+}
+
 // True in one lane of a converged warp.  The single-issuer roles run their loops in the whole warp
 // and issue under this predicate: addresses and descriptors then stay in uniform registers, which
 // the TMA and tcgen05 instructions take (a loop inside one lane moves each of them there first).
