@@ -85,7 +85,7 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
+    constexpr uint32_t tmem = 0;  // all 512 columns are this block's: they start at column 0
     RingPos sched;
     bool ok = true;
     // the next unit of this warp, or -1
@@ -111,32 +111,32 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
             if (elect_one()) clc_request(sslot(sched.slot), sfull(sched.slot));
             asked = true;
             for (int t = unit * p.group, te = min(t + p.group, p.ntiles); ok && t < te; ++t) {
-            const int jt = t % p.njt, i0 = t / p.njt * p.bn;
-            const int rt0 = i0 / kF4Tile;
-            const int rts = min(nrt, p.a.tiles() - rt0);
-            const uint8_t* sb = p.b.scales + (long long)jt * p.b.natoms * kF4Atom;
-            const uint8_t* sa = p.a.scales + (long long)rt0 * p.a.natoms * kF4Atom;
-            int left = p.b.Kp / 64;  // steps to go
-            for (int c = 0; c < p.nchunk; ++c, ++step) {
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(empty(st.slot), st.parity ^ 1u, abort));
-                if (!ok) break;
-                const int steps = min(left, kCB / 32);
-                left -= steps;
-                if (elect_one()) {
-                    const uint32_t dst = stage0 + (uint32_t)(st.slot * p.stage_bytes), bar = full(st.slot);
-                    const uint32_t sfb = (uint32_t)((kNv ? steps : (steps + 1) / 2) * kF4Atom);
-                    mbar_expect_tx(bar, (uint32_t)((128 + p.bn) * kCB) + sfb * (1 + rts));
-                    tma_load(dst, &tmb, c * kCB, jt * 128, bar);
-                    tma_load(dst + off_b, &tma, c * kCB, i0, bar);
-                    bulk_load(dst + off_sb, sb, sfb, bar);
-                    bulk_load(dst + off_sa, sa, sfb, bar);
-                    if (rts > 1)
-                        bulk_load(dst + off_sa + kAtoms * kF4Atom, sa + (long long)p.a.natoms * kF4Atom, sfb, bar);
+                const int jt = t % p.njt, i0 = t / p.njt * p.bn;
+                const int rt0 = i0 / kF4Tile;
+                const int rts = min(nrt, p.a.tiles() - rt0);
+                const uint8_t* sb = p.b.scales + (long long)jt * p.b.natoms * kF4Atom;
+                const uint8_t* sa = p.a.scales + (long long)rt0 * p.a.natoms * kF4Atom;
+                int left = p.b.Kp / 64;  // steps to go
+                for (int c = 0; c < p.nchunk; ++c, ++step) {
+                    ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(empty(st.slot), st.parity ^ 1u, abort));
+                    if (!ok) break;
+                    const int steps = min(left, kCB / 32);
+                    left -= steps;
+                    if (elect_one()) {
+                        const uint32_t dst = stage0 + (uint32_t)(st.slot * p.stage_bytes), bar = full(st.slot);
+                        const uint32_t sfb = (uint32_t)((kNv ? steps : (steps + 1) / 2) * kF4Atom);
+                        mbar_expect_tx(bar, (uint32_t)((128 + p.bn) * kCB) + sfb * (1 + rts));
+                        tma_load(dst, &tmb, c * kCB, jt * 128, bar);
+                        tma_load(dst + off_b, &tma, c * kCB, i0, bar);
+                        bulk_load(dst + off_sb, sb, sfb, bar);
+                        bulk_load(dst + off_sa, sa, sfb, bar);
+                        if (rts > 1)
+                            bulk_load(dst + off_sa + kAtoms * kF4Atom, sa + (long long)p.a.natoms * kF4Atom, sfb, bar);
+                    }
+                    sb += kAtoms * kF4Atom;
+                    sa += kAtoms * kF4Atom;
+                    st.next(p.nstage);
                 }
-                sb += kAtoms * kF4Atom;
-                sa += kAtoms * kF4Atom;
-                st.next(p.nstage);
-            }
             }
         }
         if (!ok && lane == 0) {
@@ -153,47 +153,46 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
         int last = -1;
         uint32_t last_parity = 0;
         const uint32_t sfc = (uint32_t)(4 * kAtoms * (1 + nrt));  // TMEM columns of a stage's scales
-        for (int unit = blockIdx.x; ok && unit >= 0; unit = ok ? next_unit() : -1) {
-            for (int t = unit * p.group, te = min(t + p.group, p.ntiles); ok && t < te; ++t) {
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(acce(ac.slot), ac.parity ^ 1u, abort));
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t d = tmem + (uint32_t)(ac.slot * p.acc_cols);
-            int left = p.b.Kp / 64;
-            for (int c = 0; c < p.nchunk; ++c) {
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(full(st.slot), st.parity, abort));
-                if (!ok) break;
+        for (int unit = blockIdx.x; unit >= 0; unit = next_unit()) {
+            for (int t = unit * p.group, te = min(t + p.group, p.ntiles); t < te; ++t) {
+                mbar_wait_issue(acce(ac.slot), ac.parity ^ 1u, abort, p.err, 2);
                 tc_fence_after();
-                const uint32_t src = stage0 + (uint32_t)(st.slot * p.stage_bytes);
-                const int steps = min(left, kCB / 32);
-                left -= steps;
-                const int atoms = kNv ? steps : (steps + 1) / 2;
-                const uint32_t tsb = tmem + 256u + (uint32_t)st.slot * sfc, tsa = tsb + 4 * kAtoms;
-                const uint64_t db = f4_operand_desc<kCB>(src), da = f4_operand_desc<kCB>(src + off_b);
-                const uint64_t dsb = f4_atom_desc(src + off_sb), dsa = f4_atom_desc(src + off_sa);
-                if (elect_one()) {
+                const uint32_t d = tmem + (uint32_t)(ac.slot * p.acc_cols);
+                int left = p.b.Kp / 64;
+                for (int c = 0; c < p.nchunk; ++c) {
+                    mbar_wait_issue(full(st.slot), st.parity, abort, p.err, 2);
+                    tc_fence_after();
+                    const uint32_t src = stage0 + (uint32_t)(st.slot * p.stage_bytes);
+                    const int steps = min(left, kCB / 32);
+                    left -= steps;
+                    const int atoms = kNv ? steps : (steps + 1) / 2;
+                    const uint32_t tsb = tmem + 256u + (uint32_t)st.slot * sfc, tsa = tsb + 4 * kAtoms;
+                    const uint64_t db = f4_operand_desc<kCB>(src), da = f4_operand_desc<kCB>(src + off_b);
+                    const uint64_t dsb = f4_atom_desc(src + off_sb), dsa = f4_atom_desc(src + off_sa);
+                    if (elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < kAtoms; ++k) {
-                        if (k >= atoms) break;
-                        f4_copy_atom(tsb + 4 * k, dsb + k * (kF4Atom >> 4));
-                        f4_copy_atom(tsa + 4 * k * nrt, dsa + k * (kF4Atom >> 4));
-                        if (nrt > 1) f4_copy_atom(tsa + 8 * k + 4, dsa + (kAtoms + k) * (kF4Atom >> 4));
-                    }
+                        for (int k = 0; k < kAtoms; ++k) {
+                            if (k >= atoms) break;
+                            f4_copy_atom(tsb + 4 * k, dsb + k * (kF4Atom >> 4));
+                            f4_copy_atom(tsa + 4 * k * nrt, dsa + k * (kF4Atom >> 4));
+                            if (nrt > 1) f4_copy_atom(tsa + 8 * k + 4, dsa + (kAtoms + k) * (kF4Atom >> 4));
+                        }
 #pragma unroll
-                    for (int k = 0; k < kCB / 32; ++k) {
-                        if (k >= steps) break;
-                        const int at = kNv ? k : k >> 1;
-                        f4_mma<kNv>(d, db + 2 * k, da + 2 * k, f4_idesc<kNv>(p.bn, kNv ? 0 : k & 1),
-                                    tsb + 4 * at, tsa + 4 * nrt * at, (c | k) ? 1u : 0u);
+                        for (int k = 0; k < kCB / 32; ++k) {
+                            if (k >= steps) break;
+                            const int at = kNv ? k : k >> 1;
+                            f4_mma<kNv>(d, db + 2 * k, da + 2 * k, f4_idesc<kNv>(p.bn, kNv ? 0 : k & 1),
+                                        tsb + 4 * at, tsa + 4 * nrt * at, (c | k) ? 1u : 0u);
+                        }
+                        mma_commit(empty(st.slot));
+                        if (c == p.nchunk - 1) mma_commit(accf(ac.slot));
                     }
-                    mma_commit(empty(st.slot));
-                    if (c == p.nchunk - 1) mma_commit(accf(ac.slot));
+                    __syncwarp();
+                    last = st.slot;
+                    last_parity = st.parity;
+                    st.next(p.nstage);
                 }
-                last = st.slot;
-                last_parity = st.parity;
-                st.next(p.nstage);
-            }
-            ac.next(p.nacc);
+                ac.next(p.nacc);
             }
         }
         if (!ok && lane == 0) {
@@ -213,46 +212,46 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
         int n = 0;
         for (int unit = blockIdx.x; ok && unit >= 0; unit = ok ? next_unit() : -1) {
             for (int t = unit * p.group, te = min(t + p.group, p.ntiles); t < te; ++t, ++n, ac.next(p.nacc)) {
-            if (p.nacc > 1 && (n & 1) != group) continue;
-            const int b = ac.slot;
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(accf(b), ac.parity, abort));
-            if (!ok) break;
-            tc_fence_after();
-            const int jt = t % p.njt, i0 = t / p.njt * p.bn;
-            const int cb = p.nacc > 1 ? 0 : 128 * group;   // first of this warp's columns (rows of a)
-            const int ce = min(min(p.bn, cb + 128), p.a.rows - i0);
-            uint32_t r[4][32];
+                if (p.nacc > 1 && (n & 1) != group) continue;
+                const int b = ac.slot;
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(accf(b), ac.parity, abort));
+                if (!ok) break;
+                tc_fence_after();
+                const int jt = t % p.njt, i0 = t / p.njt * p.bn;
+                const int cb = p.nacc > 1 ? 0 : 128 * group;   // first of this warp's columns (rows of a)
+                const int ce = min(min(p.bn, cb + 128), p.a.rows - i0);
+                uint32_t r[4][32];
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (cb + 32 * c < ce) tmem_ld32_issue(tmem + lane_addr + (uint32_t)(b * p.acc_cols + cb + 32 * c), r[c]);
-            tmem_wait();
+                for (int c = 0; c < 4; ++c)
+                    if (cb + 32 * c < ce) tmem_ld32_issue(tmem + lane_addr + (uint32_t)(b * p.acc_cols + cb + 32 * c), r[c]);
+                tmem_wait();
 #pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_pin32(r[c]);
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(acce(b));
-            const long long j = (long long)jt * 128 + jl;
-            if (j < p.b.rows) {
-                T* o = out + (long long)(i0 + cb) * p.ld + j;
+                for (int c = 0; c < 4; ++c) tmem_pin32(r[c]);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(acce(b));
+                const long long j = (long long)jt * 128 + jl;
+                if (j < p.b.rows) {
+                    T* o = out + (long long)(i0 + cb) * p.ld + j;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int rows = ce - cb - 32 * c;
-                    if (rows >= 32) {
+                    for (int c = 0; c < 4; ++c) {
+                        const int rows = ce - cb - 32 * c;
+                        if (rows >= 32) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e, o += p.ld) *o = from_f32<T>(__uint_as_float(r[c][e]) * alpha);
-                    } else if (rows > 0) {
+                            for (int e = 0; e < 32; ++e, o += p.ld) *o = from_f32<T>(__uint_as_float(r[c][e]) * alpha);
+                        } else if (rows > 0) {
 #pragma unroll
-                        for (int f = 0; f < 32; f += 4) {  // few rows leave most of these branches
-                            if (f < rows) {
+                            for (int f = 0; f < 32; f += 4) {  // few rows leave most of these branches
+                                if (f < rows) {
 #pragma unroll
-                                for (int e = f; e < f + 4; ++e, o += p.ld)
-                                    if (e < rows) *o = from_f32<T>(__uint_as_float(r[c][e]) * alpha);
+                                    for (int e = f; e < f + 4; ++e, o += p.ld)
+                                        if (e < rows) *o = from_f32<T>(__uint_as_float(r[c][e]) * alpha);
+                                }
                             }
                         }
                     }
                 }
-            }
-            __syncwarp();
+                __syncwarp();
             }
         }
         if (!ok && lane == 0) {
@@ -264,7 +263,7 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
     __syncthreads();
     if (warp == 9) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "r"(512)
                      : "memory");
     }
 }
@@ -327,7 +326,7 @@ k_f4_product_rows(const __grid_constant__ CUtensorMap tma, const __grid_constant
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
+    constexpr uint32_t tmem = 0;  // all 512 columns are this block's: they start at column 0
     const int steps = p.b.Kp / 64;
     const int atoms = kNv ? steps : (steps + 1) / 2;
     bool ok = true;
@@ -368,17 +367,16 @@ k_f4_product_rows(const __grid_constant__ CUtensorMap tma, const __grid_constant
         RingPos st, ac;
         int last = -1;
         uint32_t last_parity = 0;
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(afull, 0, abort));
+        mbar_wait_issue(afull, 0, abort, p.err, 2);
         const uint32_t tsa = tmem + 256u;
         const uint64_t da = f4_operand_desc<kCB>(s_a);
-        if (ok) {
+        tc_fence_after();
+        if (elect_one())
+            for (int k = 0; k < atoms; ++k) f4_copy_atom(tsa + 4 * k, f4_atom_desc(s_sa + k * kF4Atom));
+        __syncwarp();
+        for (int g = blockIdx.x; g < ngroups; g += gridDim.x) {
+            mbar_wait_issue(full(st.slot), st.parity, abort, p.err, 2);
             tc_fence_after();
-            if (elect_one())
-                for (int k = 0; k < atoms; ++k) f4_copy_atom(tsa + 4 * k, f4_atom_desc(s_sa + k * kF4Atom));
-        }
-        for (int g = blockIdx.x; ok && g < ngroups; g += gridDim.x) {
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(full(st.slot), st.parity, abort));
-            if (!ok) break;
             const uint32_t src = ring0 + (uint32_t)(st.slot * kStage);
             const uint32_t tsb = tmem + 272u + (uint32_t)(st.slot * kSGroup * 4 * kAtoms);
             const int nt = min(kSGroup, p.njt - g * kSGroup);
@@ -386,8 +384,7 @@ k_f4_product_rows(const __grid_constant__ CUtensorMap tma, const __grid_constant
             for (int h = 0; h < kSGroup; ++h) {
                 if (h >= nt) break;
                 if (h % kPer == 0) {
-                    ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(acce(ac.slot), ac.parity ^ 1u, abort));
-                    if (!ok) break;
+                    mbar_wait_issue(acce(ac.slot), ac.parity ^ 1u, abort, p.err, 2);
                     tc_fence_after();
                 }
                 const uint32_t d = tmem + (uint32_t)(32 * ac.slot + h % kPer * kBn);
@@ -405,6 +402,7 @@ k_f4_product_rows(const __grid_constant__ CUtensorMap tma, const __grid_constant
                     if (end) mma_commit(accf(ac.slot));
                     if (h == nt - 1) mma_commit(empty(st.slot));
                 }
+                __syncwarp();
                 if (end) {
                     last = ac.slot;
                     last_parity = ac.parity;
@@ -412,10 +410,6 @@ k_f4_product_rows(const __grid_constant__ CUtensorMap tma, const __grid_constant
                 }
             }
             st.next(kStages);
-        }
-        if (!ok && lane == 0) {
-            if (!*abort) atomicExch(p.err, 2);
-            *abort = 1;
         }
         // the last products must finish before the accumulators are freed
         if (last >= 0) mbar_wait<false>(accf(last), last_parity, nullptr);
@@ -467,7 +461,7 @@ k_f4_product_rows(const __grid_constant__ CUtensorMap tma, const __grid_constant
     __syncthreads();
     if (warp == 9) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "r"(512)
                      : "memory");
     }
 }
