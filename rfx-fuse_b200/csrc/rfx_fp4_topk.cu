@@ -140,6 +140,7 @@ k_f4_keys(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUten
     constexpr uint32_t tmem = 0;  // all 512 columns are this block's: they start at column 0
     const int steps = p.b.Kp / 64;
     const int atoms = kNv ? steps : (steps + 1) / 2;
+    let_next_start();  // k_f4_pick's blocks take the places of the blocks that end
 
     if (warp == 12) {
         const uint32_t sfb = (uint32_t)(atoms * kF4Atom);
@@ -465,6 +466,17 @@ k_f4_pick(PickArgs p) {
     const bool small = kT == 128 || nvec * 8 <= kUnits;  // a unit is a key
     const int nunits = small ? nvec * 8 : min(nvec, kUnits);
 
+    // the row, decoded, and its scales
+    for (int t = tid; t < p.a.Kp / 4; t += kT) {
+        const uint32_t w = *reinterpret_cast<const uint16_t*>(p.a.codes + i * p.a.pitch() + 2 * t);
+        int d = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d |= ((int)(2.0f * e2m1_value((w >> (4 * e)) & 15u)) & 0xFF) << (8 * e);
+        qa[t] = d;
+    }
+    for (int t = tid; t < p.a.Kp / (kNv ? 16 : 32); t += kT)
+        sa[t] = f4_scale_value(kNv, p.a.scales[f4_scale_at(p.a, i, t)]);
+    wait_for_previous();  // the keys
     // the largest key of every unit, four vectors in flight; thread t owns the units t, t + kT, ...
     for (int t0 = tid; t0 < nvec; t0 += 4 * kT) {
         uint4 x[4];
@@ -485,16 +497,6 @@ k_f4_pick(PickArgs p) {
             }
         }
     }
-    // the row, decoded, and its scales
-    for (int t = tid; t < p.a.Kp / 4; t += kT) {
-        const uint32_t w = *reinterpret_cast<const uint16_t*>(p.a.codes + i * p.a.pitch() + 2 * t);
-        int d = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) d |= ((int)(2.0f * e2m1_value((w >> (4 * e)) & 15u)) & 0xFF) << (8 * e);
-        qa[t] = d;
-    }
-    for (int t = tid; t < p.a.Kp / (kNv ? 16 : 32); t += kT)
-        sa[t] = f4_scale_value(kNv, p.a.scales[f4_scale_at(p.a, i, t)]);
     if (warp == kT / 32 - 1) {
         float e = 0.0f;
         bool f = false;
@@ -705,6 +707,20 @@ cudaError_t launch_keys(const CUtensorMap& ta, const CUtensorMap& tb, KeysArgs& 
     return cudaGetLastError();
 }
 
+template <int kNv, int kT>
+cudaError_t launch_pick(const PickArgs& q, int rows, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)rows);
+    cfg.blockDim = dim3((unsigned)kT);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k_f4_pick<kNv, kT>, q);
+}
+
 }  // namespace
 
 long long f4_topk_workspace(const F4& a, const F4& b, int k, int sms) {
@@ -754,16 +770,11 @@ cudaError_t f4_topk(const F4& a, const F4& b, int k, long long self, int* idx, f
         q.row0 = (int)r0;
         q.nerrs = grid;
         const int threads = rows <= 2 * sms ? 1024 : plan.nspan * kSpanKeys <= kSmallKeys ? 128 : 256;
-        if (threads == 1024) {
-            if (b.nv) k_f4_pick<1, 1024><<<rows, 1024, 0, st>>>(q);
-            else k_f4_pick<0, 1024><<<rows, 1024, 0, st>>>(q);
-        } else if (threads == 128) {
-            if (b.nv) k_f4_pick<1, 128><<<rows, 128, 0, st>>>(q);
-            else k_f4_pick<0, 128><<<rows, 128, 0, st>>>(q);
-        } else {
-            if (b.nv) k_f4_pick<1, 256><<<rows, 256, 0, st>>>(q);
-            else k_f4_pick<0, 256><<<rows, 256, 0, st>>>(q);
-        }
+        if (b.nv) e = threads == 1024 ? launch_pick<1, 1024>(q, rows, st) : threads == 128 ? launch_pick<1, 128>(q, rows, st)
+                                                                                           : launch_pick<1, 256>(q, rows, st);
+        else e = threads == 1024 ? launch_pick<0, 1024>(q, rows, st) : threads == 128 ? launch_pick<0, 128>(q, rows, st)
+                                                                                      : launch_pick<0, 256>(q, rows, st);
+        if (e != cudaSuccess) return e;
         *launches += 2;
         if ((e = cudaGetLastError()) != cudaSuccess) return e;
     }

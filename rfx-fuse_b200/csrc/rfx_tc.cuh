@@ -141,6 +141,11 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
+// Programmatic dependent launch: a kernel lets the next one's blocks start, and a kernel started so
+// waits for the one before (its memory included) to end.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // Work by cluster launch control: a running block takes over the index of one that has not started.
 // The 16-byte answer arrives in shared memory at `slot`, completing on `bar`.
 __device__ __forceinline__ void clc_request(uint32_t slot, uint32_t bar) {
