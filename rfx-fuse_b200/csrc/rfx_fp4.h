@@ -80,6 +80,7 @@ struct F4ProductArgs {
     int njt, nit;     // tiles of b and of a (njt * nit < 2^31)
     int ntiles, group; // their number, tiles of a unit of scheduling
     int nchunk;       // chunks of the inner axis
+    int split;        // blocks of a cluster that share one tile's inner axis
     int nstage, nacc; // shared-memory ring, accumulator ring
     int acc_cols;     // TMEM columns of an accumulator
     int stage_bytes;

@@ -483,6 +483,198 @@ cudaError_t launch_rows(const CUtensorMap& ta, const CUtensorMap& tb, const F4Pr
     return launch_rows_bn<kNv, kCB, T, 32>(ta, tb, p, grid, st);
 }
 
+// Few rows of a over a long inner axis give few tiles: the blocks of a cluster split the axis of one
+// tile, leave their fp32 sums in shared memory and each adds up a share of the rows over the
+// cluster's blocks, in the order of their shares of the axis (no atomics: the same sums every time).
+// 16 x 8,192 x 8,192: 14.3 us in the general kernel, where 64 tiles keep 64 of 148 SMs busy.
+//   warps 0-3  accumulator to shared memory, then the sums; warp 4 loads; warp 5 multiplies.
+constexpr int kXThreads = 192;
+constexpr int kXRows = 64;   // rows of a at most
+constexpr int kXStages = 6;
+
+template <int kNv, class T>
+__global__ void __launch_bounds__(kXThreads, 1)
+k_f4_product_split(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUtensorMap tmb, F4ProductArgs p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint64_t* bars = (uint64_t*)sm;
+    // full[6], empty[6], acc_full
+    uint32_t* tmem_slot = (uint32_t*)(bars + 16);
+    volatile int* abort = (volatile int*)(tmem_slot + 1);
+    const uint32_t bar0 = smem_u32(bars);
+    auto full = [&](int s) { return bar0 + 8u * s; };
+    auto empty = [&](int s) { return bar0 + 8u * (kXStages + s); };
+    const uint32_t accf = bar0 + 8u * 12;
+    constexpr int kCB = 128, kAtoms = kNv ? 4 : 2;
+    const uint32_t stage0 = bar0 + kPBars;
+    const uint32_t off_b = 128 * kCB, off_sb = off_b + kXRows * kCB, off_sa = off_sb + kAtoms * kF4Atom;
+    constexpr uint32_t kStage = (128 + kXRows) * kCB + 2 * kAtoms * kF4Atom;
+    const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const int part = blockIdx.x % p.split, jt = blockIdx.x / p.split;
+    const int c0 = p.nchunk * part / p.split, c1 = p.nchunk * (part + 1) / p.split;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kXStages; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), 1);
+        }
+        mbar_init(accf, 1);
+        *abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 5) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_u32(tmem_slot)),
+                     "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    constexpr uint32_t tmem = 0;  // all 512 columns are this block's: they start at column 0
+    bool ok = true;
+
+    if (warp == 4) {
+        RingPos st;
+        int n = 0;
+        const uint8_t* sb = p.b.scales + ((long long)jt * p.b.natoms + c0 * kAtoms) * kF4Atom;
+        const uint8_t* sa = p.a.scales + (long long)c0 * kAtoms * kF4Atom;
+        for (int c = c0; c < c1; ++c, ++n) {
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(empty(st.slot), st.parity ^ 1u, abort));
+            if (!ok) break;
+            const int steps = min(p.b.Kp / 64 - 4 * c, 4);
+            if (elect_one()) {
+                const uint32_t dst = stage0 + (uint32_t)st.slot * kStage, bar = full(st.slot);
+                const uint32_t sfb = (uint32_t)((kNv ? steps : (steps + 1) / 2) * kF4Atom);
+                mbar_expect_tx(bar, (uint32_t)((128 + p.bn) * kCB) + 2 * sfb);
+                tma_load(dst, &tmb, c * kCB, jt * 128, bar);
+                tma_load(dst + off_b, &tma, c * kCB, 0, bar);
+                bulk_load(dst + off_sb, sb, sfb, bar);
+                bulk_load(dst + off_sa, sa, sfb, bar);
+            }
+            sb += kAtoms * kF4Atom;
+            sa += kAtoms * kF4Atom;
+            st.next(kXStages);
+        }
+        if (!ok && lane == 0) {
+            if (!*abort) atomicExch(p.err, 1);
+            *abort = 1;
+        }
+        // drain this warp's copies still in flight
+        for (int i = n > kXStages ? n - kXStages : 0; i < n; ++i)
+            mbar_wait<false>(full(i % kXStages), (uint32_t)(i / kXStages) & 1u, nullptr);
+        __syncwarp();
+    } else if (warp == 5) {
+        RingPos st;
+        for (int c = c0; c < c1; ++c) {
+            mbar_wait_issue(full(st.slot), st.parity, abort, p.err, 2);
+            tc_fence_after();
+            const uint32_t src = stage0 + (uint32_t)st.slot * kStage;
+            const int steps = min(p.b.Kp / 64 - 4 * c, 4);
+            const int atoms = kNv ? steps : (steps + 1) / 2;
+            const uint32_t tsb = 64u + (uint32_t)(st.slot * 8 * kAtoms), tsa = tsb + 4 * kAtoms;
+            const uint64_t db = f4_operand_desc<kCB>(src), da = f4_operand_desc<kCB>(src + off_b);
+            const uint64_t dsb = f4_atom_desc(src + off_sb), dsa = f4_atom_desc(src + off_sa);
+            if (elect_one()) {
+#pragma unroll
+                for (int k = 0; k < kAtoms; ++k) {
+                    if (k >= atoms) break;
+                    f4_copy_atom(tsb + 4 * k, dsb + k * (kF4Atom >> 4));
+                    f4_copy_atom(tsa + 4 * k, dsa + k * (kF4Atom >> 4));
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if (k >= steps) break;
+                    const int at = kNv ? k : k >> 1;
+                    f4_mma<kNv>(tmem, db + 2 * k, da + 2 * k, f4_idesc<kNv>(p.bn, kNv ? 0 : k & 1), tsb + 4 * at,
+                                tsa + 4 * at, (c > c0 || k) ? 1u : 0u);
+                }
+                mma_commit(empty(st.slot));
+                if (c == c1 - 1) mma_commit(accf);
+            }
+            __syncwarp();
+            st.next(kXStages);
+        }
+        // the products must finish before the accumulator is freed
+        mbar_wait<false>(accf, 0, nullptr);
+        __syncwarp();
+    }
+    // every copy has landed and every product is done: the ring's memory takes the sums
+    if (warp < 4) {
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(accf, 0, abort));
+        if (!ok && lane == 0) {
+            if (!*abort) atomicExch(p.err, 3);
+            *abort = 1;
+        }
+    }
+    __syncwarp();
+    __syncthreads();
+    float* sums = (float*)(sm + kPBars);  // [row of a][128]
+    if (warp < 4) {
+        tc_fence_after();
+#pragma unroll
+        for (int h = 0; h < kXRows / 32; ++h) {
+            if (32 * h >= p.bn) break;
+            uint32_t r[32];
+            tmem_ld32_issue(tmem + ((uint32_t)(32 * warp) << 16) + 32 * h, r);
+            tmem_wait();
+            tmem_pin32(r);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) sums[(32 * h + e) * 128 + 32 * warp + lane] = __uint_as_float(r[e]);
+        }
+        tc_fence_before();
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    {
+        const float alpha = __ldg(p.a.gs) * __ldg(p.b.gs);
+        T* out = (T*)p.out;
+        const uint32_t mine = smem_u32(sums);
+        for (int t = part * kXThreads + threadIdx.x; t < p.a.rows * 128; t += p.split * kXThreads) {
+            const long long j = (long long)jt * 128 + (t & 127);
+            if (j >= p.b.rows) continue;
+            float v = 0.0f;
+            for (int s = 0; s < p.split; ++s) {
+                uint32_t at;
+                float x;
+                asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(mine + 4u * (uint32_t)t), "r"(s));
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory");
+                v += x;
+            }
+            out[(long long)(t >> 7) * p.ld + j] = from_f32<T>(v * alpha);
+        }
+    }
+    __syncwarp();
+    // no block leaves while another reads its sums
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (warp == 5) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "r"(512)
+                     : "memory");
+    }
+}
+
+template <int kNv, class T>
+cudaError_t launch_split(const CUtensorMap& ta, const CUtensorMap& tb, const F4ProductArgs& p, cudaStream_t st) {
+    constexpr int kAtoms = kNv ? 4 : 2;
+    const int smem = 1024 + kPBars + kXStages * ((128 + kXRows) * 128 + 2 * kAtoms * kF4Atom);
+    auto f = k_f4_product_split<kNv, T>;
+    cudaError_t e = cudaFuncSetAttribute((const void*)f, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(p.njt * p.split));
+    cfg.blockDim = dim3((unsigned)kXThreads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)p.split;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, f, ta, tb, p);
+}
+
 template <int kNv, int kCB, class T>
 cudaError_t launch(const CUtensorMap& ta, const CUtensorMap& tb, const F4ProductArgs& p, int grid, cudaStream_t st) {
     const int smem = 1024 + kPBars + p.nstage * p.stage_bytes;
@@ -491,6 +683,13 @@ cudaError_t launch(const CUtensorMap& ta, const CUtensorMap& tb, const F4Product
     if (e != cudaSuccess) return e;
     f<<<grid, kPThreads, smem, st>>>(ta, tb, p);
     return cudaGetLastError();
+}
+
+template <int kNv>
+cudaError_t launch_split_t(const CUtensorMap& ta, const CUtensorMap& tb, const F4ProductArgs& p, cudaStream_t st) {
+    if (p.dtype == RFX_F32) return launch_split<kNv, float>(ta, tb, p, st);
+    if (p.dtype == RFX_BF16) return launch_split<kNv, __nv_bfloat16>(ta, tb, p, st);
+    return launch_split<kNv, __half>(ta, tb, p, st);
 }
 
 template <int kNv, int kCB>
@@ -533,6 +732,15 @@ cudaError_t f4_product(const F4& a, const F4& b, void* out, int dtype, long long
         return b.nv ? launch_rows_t<1, 128>(ta, tb, p, grid, st) : launch_rows_t<0, 128>(ta, tb, p, grid, st);
     }
     p.nchunk = (b.Kp + 2 * cb - 1) / (2 * cb);
+    // at most half the SMs' tiles, and at least four chunks (1,024 columns) for every block of a cluster
+    const int most = std::min(std::min(8, sms / p.njt), p.nchunk / 4);
+    p.split = most >= 8 ? 8 : most >= 4 ? 4 : most >= 2 ? 2 : 1;
+    if (a.rows <= kXRows && p.split >= 2) {
+        CUtensorMap ta, tb;
+        if (!f4_map(&ta, a, p.bn, cb) || !f4_map(&tb, b, 128, cb)) return cudaErrorInvalidValue;
+        *launches += 1;
+        return b.nv ? launch_split_t<1>(ta, tb, p, st) : launch_split_t<0>(ta, tb, p, st);
+    }
     const int atoms = cb == 32 ? 1 : (b.nv ? 4 : 2);
     const int nrt = p.bn > kF4Tile ? 2 : 1;
     p.stage_bytes = ((128 * cb + (p.bn * cb + 1023) / 1024 * 1024 + atoms * kF4Atom * (1 + nrt)) + 1023) / 1024 * 1024;

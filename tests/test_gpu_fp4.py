@@ -172,7 +172,8 @@ def _product_check(rng, fmt, m, n, k, dtype="float32", spread=4):
 @pytest.mark.parametrize("m,n,k", [(16, 128, 64), (1, 1, 1), (128, 128, 64), (256, 256, 64), (1, 300, 17), (17, 129, 128),
                                    (129, 130, 192), (100, 257, 256), (33, 200, 320), (300, 500, 1000), (257, 640, 65),
                                    (513, 3000, 64), (70, 1000, 4100), (8, 1000, 64), (9, 1025, 64),
-                                   (17, 5000, 64), (32, 700, 200), (33, 40, 64), (5, 200000, 64), (3, 30000, 256)])
+                                   (17, 5000, 64), (32, 700, 200), (33, 40, 64), (5, 200000, 64), (3, 30000, 256),
+                                   (1, 100, 2048), (16, 4000, 4096), (64, 1000, 3000), (33, 129, 9000), (7, 8192, 2100)])
 def test_product(fmt, m, n, k):
     _product_check(np.random.default_rng(m + 1000 * n + k), fmt, m, n, k)
 
