@@ -390,6 +390,8 @@ __global__ void k_f4_unpack(F4 m, uint8_t* __restrict__ codes, uint8_t* __restri
     }
 }
 
+__global__ void k_f4_unit_scale(float* gs) { gs[0] = 1.0f; }
+
 size_t bound_smem(const F4& m, int width) {
     return m.Kp <= kF4TopkK ? (size_t)(m.Kp / width) * 129 * sizeof(float) : 0;
 }
@@ -450,6 +452,12 @@ cudaError_t dequantize_d(const F4& m, int r0, int r1, T* out, long long ld, cuda
 }
 
 }  // namespace
+
+// The matrix scale of a matrix without rows.
+cudaError_t f4_unit_scale(const F4& m, cudaStream_t st) {
+    k_f4_unit_scale<<<1, 1, 0, st>>>(m.gs);
+    return cudaGetLastError();
+}
 
 cudaError_t f4_quantize(const void* x, int dtype, long long ld, const F4& m, int sms, cudaStream_t st,
                         int* launches) {

@@ -61,6 +61,7 @@ __host__ __device__ inline long long f4_scale_at(const F4& m, long long r, int b
 }
 
 // Launchers: enqueue on `st`, return the launch status.
+cudaError_t f4_unit_scale(const F4& m, cudaStream_t st);
 cudaError_t f4_quantize(const void* x, int dtype, long long ld, const F4& m, int sms, cudaStream_t st,
                         int* launches);
 cudaError_t f4_dequantize(const F4& m, int r0, int r1, void* out, int dtype, long long ld, cudaStream_t st);

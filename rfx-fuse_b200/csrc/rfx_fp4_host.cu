@@ -183,7 +183,7 @@ int rfx_fp4_quantize(const void* x_dev, int dtype, long long row_stride, const r
         require(row_stride >= m.cols, RFX_ERR_ARG, "row_stride must be at least cols");
         cudaStream_t st = static_cast<cudaStream_t>(stream);
         int launches = 0;
-        if (m.rows == 0) return;
+        if (m.rows == 0) return check_launch(rfx::f4_unit_scale(m, st), "rfx_fp4_quantize");
         check_elements(x_dev, dtype, "x");
         check_launch(rfx::f4_quantize(x_dev, dtype, row_stride, m, device_info().sms, st, &launches), "rfx_fp4_quantize");
     });
@@ -207,7 +207,7 @@ int rfx_fp4_pack(const uint8_t* codes_dev, const uint8_t* scales_dev, const floa
                  const rfx_fp4_matrix* out, void* stream) {
     return guarded([&] {
         const F4 m = matrix_of(out, "out");
-        if (m.rows == 0) return;
+        if (m.rows == 0) return check_launch(rfx::f4_unit_scale(m, static_cast<cudaStream_t>(stream)), "rfx_fp4_pack");
         require(codes_dev && scales_dev, RFX_ERR_ARG, "null codes or scales");
         require(!scale_dev || aligned(scale_dev, 4), RFX_ERR_ARG, "unaligned scale");
         check_launch(rfx::f4_pack(codes_dev, scales_dev, scale_dev, m, static_cast<cudaStream_t>(stream)), "rfx_fp4_pack");

@@ -474,9 +474,16 @@ k_f4_pick(PickArgs p) {
         for (int e = 0; e < 4; ++e) d |= ((int)(2.0f * e2m1_value((w >> (4 * e)) & 15u)) & 0xFF) << (8 * e);
         qa[t] = d;
     }
-    for (int t = tid; t < p.a.Kp / (kNv ? 16 : 32); t += kT)
-        sa[t] = f4_scale_value(kNv, p.a.scales[f4_scale_at(p.a, i, t)]);
+    float s0 = 0.0f;
+    if (tid < p.a.Kp / (kNv ? 16 : 32)) sa[tid] = s0 = f4_scale_value(kNv, p.a.scales[f4_scale_at(p.a, i, tid)]);
     wait_for_previous();  // the keys
+    if (__syncthreads_or(!(s0 == s0))) {  // a NaN row is nobody's neighbour and has none
+        for (int s = tid; s < p.k; s += kT) {
+            p.idx[i * p.k + s] = -1;
+            p.val[i * p.k + s] = -__int_as_float(0x7f800000);
+        }
+        return;
+    }
     // the largest key of every unit, four vectors in flight; thread t owns the units t, t + kT, ...
     for (int t0 = tid; t0 < nvec; t0 += 4 * kT) {
         uint4 x[4];
