@@ -381,33 +381,37 @@ k_f4_product_rows(const __grid_constant__ CUtensorMap tma, const __grid_constant
             const uint32_t tsb = tmem + 272u + (uint32_t)(st.slot * kSGroup * 4 * kAtoms);
             const int nt = min(kSGroup, p.njt - g * kSGroup);
 #pragma unroll
-            for (int h = 0; h < kSGroup; ++h) {
-                if (h >= nt) break;
-                if (h % kPer == 0) {
-                    mbar_wait_issue(acce(ac.slot), ac.parity ^ 1u, abort, p.err, 2);
-                    tc_fence_after();
-                }
-                const uint32_t d = tmem + (uint32_t)(32 * ac.slot + h % kPer * kBn);
-                const uint32_t tsh = tsb + 4 * kAtoms * h;
-                const uint64_t db = f4_operand_desc<kCB>(src + h * kBox);
-                const uint64_t dsc = f4_atom_desc(src + kSGroup * kBox + h * atoms * kF4Atom);
-                const bool end = h % kPer == kPer - 1 || h == nt - 1;
+            for (int h0 = 0; h0 < kSGroup; h0 += kPer) {
+                if (h0 >= nt) break;
+                mbar_wait_issue(acce(ac.slot), ac.parity ^ 1u, abort, p.err, 2);
+                tc_fence_after();
                 if (elect_one()) {
-                    for (int k = 0; k < atoms; ++k) f4_copy_atom(tsh + 4 * k, dsc + k * (kF4Atom >> 4));
-                    for (int k = 0; k < steps; ++k) {
-                        const int at = kNv ? k : k >> 1;
-                        f4_mma<kNv>(d, db + 2 * k, da + 2 * k, f4_idesc<kNv>(kBn, kNv ? 0 : k & 1), tsh + 4 * at,
-                                    tsa + 4 * at, k ? 1u : 0u);
+#pragma unroll
+                    for (int h = h0; h < h0 + kPer; ++h) {
+                        if (h >= nt) break;
+                        const uint32_t d = tmem + (uint32_t)(32 * ac.slot + (h - h0) * kBn);
+                        const uint32_t tsh = tsb + 4 * kAtoms * h;
+                        const uint64_t db = f4_operand_desc<kCB>(src + h * kBox);
+                        const uint64_t dsc = f4_atom_desc(src + kSGroup * kBox + h * atoms * kF4Atom);
+                        if (kCB == 32) {
+                            f4_copy_atom(tsh, dsc);
+                            f4_mma<kNv>(d, db, da, f4_idesc<kNv>(kBn, 0), tsh, tsa, 0u);
+                        } else {
+                            for (int k = 0; k < atoms; ++k) f4_copy_atom(tsh + 4 * k, dsc + k * (kF4Atom >> 4));
+                            for (int k = 0; k < steps; ++k) {
+                                const int at = kNv ? k : k >> 1;
+                                f4_mma<kNv>(d, db + 2 * k, da + 2 * k, f4_idesc<kNv>(kBn, kNv ? 0 : k & 1), tsh + 4 * at,
+                                            tsa + 4 * at, k ? 1u : 0u);
+                            }
+                        }
                     }
-                    if (end) mma_commit(accf(ac.slot));
-                    if (h == nt - 1) mma_commit(empty(st.slot));
+                    mma_commit(accf(ac.slot));
+                    if (h0 + kPer >= nt) mma_commit(empty(st.slot));
                 }
                 __syncwarp();
-                if (end) {
-                    last = ac.slot;
-                    last_parity = ac.parity;
-                    ac.next(kSAcc);
-                }
+                last = ac.slot;
+                last_parity = ac.parity;
+                ac.next(kSAcc);
             }
             st.next(kStages);
         }
