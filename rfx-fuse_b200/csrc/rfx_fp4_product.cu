@@ -9,8 +9,8 @@
 // A block takes the unit (p.group neighbouring tiles) of its index, then the units of blocks that have not started yet, by cluster
 // launch control: some SMs store at three quarters of the others' rate, and equal shares of 43 tiles
 // left those running for 50 us of 185 (1,024 x 200,000 fp32 outputs).
-//   warps 0-7  read an accumulator (quarter warp & 3) and store it.  With up to 128 rows of a the
-//              accumulators form a ring and the two groups of four warps take alternate tiles;
+//   warps 0-7  read an accumulator (quarter warp & 3) and store it.  With tiles of up to 128 rows of
+//              a the accumulators form a ring and the two groups of four warps take alternate tiles;
 //              with more, both take the one accumulator, half the columns each, and release it as
 //              soon as it is in registers, so the next tile's products run under the stores;
 //   warp 8     loads code rows by TMA and scale atoms by bulk copies into a ring of
@@ -721,7 +721,11 @@ cudaError_t f4_product(const F4& a, const F4& b, void* out, int dtype, long long
     p.ld = ld;
     p.dtype = dtype;
     p.err = err;
-    p.bn = std::min(256, (a.rows + 15) / 16 * 16);
+    // Up to 512 columns the stores bound a tile, and tiles of 128 rows overlap them better (two
+    // accumulators); beyond, the products do, and tiles of 256 rows read b half as often.  1,024 x
+    // 40,000 fp32 outputs, 128 against 256 rows: 64 columns 33.5 / 38.9 us, 512 36.9 / 38.9,
+    // 1,024 48.2 / 44.9, 4,096 143 / 105.
+    p.bn = std::min(b.Kp <= 512 ? 128 : 256, (a.rows + 15) / 16 * 16);
     p.nit = (int)(((long long)a.rows + p.bn - 1) / p.bn);
     p.njt = b.tiles();
     const int cb = b.Kp == 64 ? 32 : 128;
