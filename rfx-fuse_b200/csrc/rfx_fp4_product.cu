@@ -6,9 +6,9 @@
 // needs no transpose; the instruction's N holds up to 256 rows of a, and shrinks to the rows
 // there are (16 at least), so that a product of a few rows only reads b.
 //
-// A block takes the unit (p.group neighbouring tiles) of its index, then the units of blocks that have not started yet, by cluster
-// launch control: some SMs store at three quarters of the others' rate, and equal shares of 43 tiles
-// left those running for 50 us of 185 (1,024 x 200,000 fp32 outputs).
+// A block takes the unit (p.group neighbouring tiles) of its index, then the units of blocks that have
+// not started yet, by cluster launch control: some SMs store at three quarters of the others' rate,
+// and equal shares of 43 tiles left those running for 50 us of 185 (1,024 x 200,000 fp32 outputs).
 //   warps 0-7  read an accumulator (quarter warp & 3) and store it.  With tiles of up to 128 rows of
 //              a the accumulators form a ring and the two groups of four warps take alternate tiles;
 //              with more, both take the one accumulator, half the columns each, and release it as
@@ -634,18 +634,33 @@ k_f4_product_split(const __grid_constant__ CUtensorMap tma, const __grid_constan
         const float alpha = __ldg(p.a.gs) * __ldg(p.b.gs);
         T* out = (T*)p.out;
         const uint32_t mine = smem_u32(sums);
-        for (int t = part * kXThreads + threadIdx.x; t < p.a.rows * 128; t += p.split * kXThreads) {
-            const long long j = (long long)jt * 128 + (t & 127);
-            if (j >= p.b.rows) continue;
-            float v = 0.0f;
-            for (int s = 0; s < p.split; ++s) {
-                uint32_t at;
-                float x;
-                asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(mine + 4u * (uint32_t)t), "r"(s));
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory");
-                v += x;
+        // four outputs at a time, all their parts on the way before the first is added
+        const int step = p.split * kXThreads, n = p.a.rows * 128;
+        for (int t0 = part * kXThreads + threadIdx.x; t0 < n; t0 += 4 * step) {
+            float x[4][8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int t = min(t0 + e * step, n - 1);
+#pragma unroll
+                for (int s = 0; s < 8; ++s) {
+                    x[e][s] = 0.0f;
+                    if (s < p.split) {
+                        uint32_t at;
+                        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(mine + 4u * (uint32_t)t), "r"(s));
+                        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x[e][s]) : "r"(at) : "memory");
+                    }
+                }
             }
-            out[(long long)(t >> 7) * p.ld + j] = from_f32<T>(v * alpha);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int t = t0 + e * step;
+                const long long j = (long long)jt * 128 + (t & 127);
+                if (t >= n || j >= p.b.rows) continue;
+                float v = 0.0f;
+#pragma unroll
+                for (int s = 0; s < 8; ++s) v += x[e][s];
+                out[(long long)(t >> 7) * p.ld + j] = from_f32<T>(v * alpha);
+            }
         }
     }
     __syncwarp();
