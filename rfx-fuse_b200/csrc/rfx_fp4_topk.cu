@@ -11,16 +11,18 @@
 //   k_f4_keys  products of 128 rows of a with b's tiles of 128 rows (tcgen05, block-scaled); of
 //              every row's 32 neighbouring accumulators only the maximum is kept, as the upper 16
 //              bits of its order-preserving integer (rounded down).
-//   k_f4_pick  a block per row of a.  The keys form as many groups as threads at most; the k-th largest of the
-//              groups' largest keys, L, is a lower bound of the k-th largest key: there are k
-//              columns with accumulators of L or more, so the k-th value is at least L - err, and
-//              a column of the answer has an accumulator of at least L - 2 err.  Only chunks whose
-//              key reaches that (about k of them) are evaluated, all 32 columns exactly, and
-//              what reaches L - err is ranked by counting who is better.
+//   k_f4_pick  a block per row of a.  Its threads' shares of the keys are groups; the k-th largest of
+//              the groups' largest keys, L, is a lower bound of the k-th largest accumulator: k
+//              columns have L or more, so the k-th value is at least L - err, and a column of the
+//              answer has an accumulator of at least L - 2 err.  Of the chunks whose key reaches that
+//              (about k, 1.2 k where groups are few) every column is estimated in fp32; what
+//              reaches L - 2 err is evaluated exactly and ranked by counting who is better.
 //
-// What the first kernel leaves is 2 bytes for 32 pairs; rows are taken in batches whose keys stay
-// in L2.  k_f4_keys is bound by reading accumulators back (one 3-input maximum for two), k_f4_pick
-// by the exact evaluations.
+// What the first kernel leaves is 2 bytes for 32 pairs.  Rows are taken in batches of 256 MB of keys
+// (4,096 x 1,000,000 in one: 441 us, in batches of 120 MB 490: each batch ends with idle SMs).
+// k_f4_keys: 300 cycles a tile of 128 x 128, of which the ALU's 128 for maxima (a 3-input maximum
+// takes two issue slots) and 90 for keys and bookkeeping; k_f4_pick: half the issue slots, latency
+// of its barriers and loads between them.  Times of both at 4,096 x 1,000,000: 301 and 155 us.
 #include <algorithm>
 
 #include "rfx_fp4_mma.cuh"
@@ -40,7 +42,7 @@ struct KeysArgs {
     F4 a, b;
     int q0;               // first row tile of a in this batch
     int nq;               // row tiles of a in it
-    int ntiles, nspan;     // tiles of b, and spans of them
+    int ntiles, nspan;    // tiles of b, and spans of them
     uint32_t* keys;       // [rows of the batch][nspan][12] pairs of keys
     float* errs;          // [grid] largest err of a block's tiles; negative: some tiles have none
     int* err;
@@ -688,7 +690,7 @@ __global__ void k_f4_topk_none(long long n, int* idx, float* val) {
     }
 }
 
-// Rows of a whose keys are made before they are read.
+// Rows of a whose keys are made before they are read: whole tiles, about kKeyMB of keys.
 constexpr long long kKeyMB = 256;
 struct TopkPlan {
     int nspan, rows;
