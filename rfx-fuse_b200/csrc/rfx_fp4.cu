@@ -344,19 +344,25 @@ k_f4_pack(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
     const int atoms = m.nv ? kc / 64 : (kc + 127) / 128;
     const bool bounds = m.Kp <= kF4TopkK;
     const int in_pitch = (m.cols + 1) / 2;
+    const bool words = in_pitch % 4 == 0 && (uintptr_t)codes % 4 == 0;  // rows of whole 4-byte words
     for (int i = threadIdx.x; i < atoms * (kF4Atom / 4); i += kQThreads) sf[i] = 0;
     __syncthreads();
+#pragma unroll 4
     for (int t = threadIdx.x; t < nr * U; t += kQThreads) {
         const int q = t / U, u = t - q * U;
         const uint8_t* src = codes + (long long)(r0 + q) * in_pitch;
         uint32_t w = 0;
+        if (words && c0 + 8 * u + 8 <= m.cols) {
+            w = __ldg(reinterpret_cast<const uint32_t*>(src + c0 / 2) + u);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int c = c0 + 8 * u + 2 * i;
-            if (c < m.cols) {
-                uint32_t b = src[c / 2];
-                if (c + 1 >= m.cols) b &= 15u;
-                w |= b << (8 * i);
+            for (int i = 0; i < 4; ++i) {
+                const int c = c0 + 8 * u + 2 * i;
+                if (c < m.cols) {
+                    uint32_t b = src[c / 2];
+                    if (c + 1 >= m.cols) b &= 15u;
+                    w |= b << (8 * i);
+                }
             }
         }
         reinterpret_cast<uint32_t*>(m.codes + (long long)(r0 + q) * m.pitch() + c0 / 2)[u] = w;
