@@ -283,6 +283,7 @@ int rfx_lowrank_pack4(void* ctx, int format) {
         const F4 f = rfx::f4_of(m);
         const size_t codes = round_up((size_t)m.rows * f.pitch(), 256);
         const size_t scales = (size_t)f.tiles() * f.natoms * rfx::kF4Atom;
+        c.lr4_ready = false;  // until the new factors are there
         uint8_t* p = (uint8_t*)c.lr4_buf.get(codes + scales + 256 + (size_t)f.tiles() * 4);
         m.codes_dev = p;
         m.scales_dev = p + codes;

@@ -68,6 +68,19 @@ __device__ __forceinline__ void f4_mma(uint32_t d, uint64_t da, uint64_t db, uin
     }
 }
 
+// The two matrices' scales as factors of an accumulator, x * lead * rest.  Their product alone may
+// leave fp32 where the result does not (0 * inf, 2^20 * 2^-160): then the larger comes first, so that
+// x * lead is infinite only if the result is (rest >= 1) and small only by an exact power of two.
+struct F4Alpha {
+    float lead, rest;
+};
+__device__ __forceinline__ F4Alpha f4_alpha(const float* ga, const float* gb) {
+    const float x = __ldg(ga), y = __ldg(gb);
+    const float lead = x > y ? x : y, rest = x > y ? y : x, both = lead * rest;
+    if (both >= 1.17549435e-38f && both <= 3.40282347e38f) return {both, 1.0f};
+    return {lead, rest};
+}
+
 // Untiled copy of `bytes` (a multiple of 16) into shared memory, completing on `bar`.
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile(

@@ -206,7 +206,7 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
         const int group = warp >> 2;
         const int jl = 32 * (warp & 3) + lane;
         const uint32_t lane_addr = (uint32_t)(32 * (warp & 3)) << 16;
-        const float alpha = __ldg(p.a.gs) * __ldg(p.b.gs);
+        const F4Alpha alpha = f4_alpha(p.a.gs, p.b.gs);
         T* out = (T*)p.out;
         RingPos ac;
         int n = 0;
@@ -238,14 +238,14 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
                         const int rows = ce - cb - 32 * c;
                         if (rows >= 32) {
 #pragma unroll
-                            for (int e = 0; e < 32; ++e, o += p.ld) *o = from_f32<T>(__uint_as_float(r[c][e]) * alpha);
+                            for (int e = 0; e < 32; ++e, o += p.ld) *o = from_f32<T>(__uint_as_float(r[c][e]) * alpha.lead * alpha.rest);
                         } else if (rows > 0) {
 #pragma unroll
                             for (int f = 0; f < 32; f += 4) {  // few rows leave most of these branches
                                 if (f < rows) {
 #pragma unroll
                                     for (int e = f; e < f + 4; ++e, o += p.ld)
-                                        if (e < rows) *o = from_f32<T>(__uint_as_float(r[c][e]) * alpha);
+                                        if (e < rows) *o = from_f32<T>(__uint_as_float(r[c][e]) * alpha.lead * alpha.rest);
                                 }
                             }
                         }
@@ -422,7 +422,7 @@ k_f4_product_rows(const __grid_constant__ CUtensorMap tma, const __grid_constant
         const int set = warp >> 2;
         const int jl = 32 * (warp & 3) + lane;
         const uint32_t lane_addr = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-        const float alpha = __ldg(p.a.gs) * __ldg(p.b.gs);
+        const F4Alpha alpha = f4_alpha(p.a.gs, p.b.gs);
         T* out = (T*)p.out;
         RingPos ac;
         for (int g = blockIdx.x; ok && g < ngroups; g += gridDim.x) {
@@ -449,7 +449,7 @@ k_f4_product_rows(const __grid_constant__ CUtensorMap tma, const __grid_constant
 #pragma unroll
                             for (int e = 0; e < kPer; ++e)
                                 if (j + 128 * e < p.b.rows)
-                                    o[128 * e] = from_f32<T>(__uint_as_float(r[e * kBn + i]) * alpha);
+                                    o[128 * e] = from_f32<T>(__uint_as_float(r[e * kBn + i]) * alpha.lead * alpha.rest);
                         }
                     }
                 }
@@ -631,7 +631,7 @@ k_f4_product_split(const __grid_constant__ CUtensorMap tma, const __grid_constan
     }
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     {
-        const float alpha = __ldg(p.a.gs) * __ldg(p.b.gs);
+        const F4Alpha alpha = f4_alpha(p.a.gs, p.b.gs);
         T* out = (T*)p.out;
         const uint32_t mine = smem_u32(sums);
         // four outputs at a time, all their parts on the way before the first is added
@@ -659,7 +659,7 @@ k_f4_product_split(const __grid_constant__ CUtensorMap tma, const __grid_constan
                 float v = 0.0f;
 #pragma unroll
                 for (int s = 0; s < 8; ++s) v += x[e][s];
-                out[(long long)(t >> 7) * p.ld + j] = from_f32<T>(v * alpha);
+                out[(long long)(t >> 7) * p.ld + j] = from_f32<T>(v * alpha.lead * alpha.rest);
             }
         }
     }

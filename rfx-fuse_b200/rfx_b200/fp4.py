@@ -194,8 +194,8 @@ def _out(out, shape, dtype, device):
         return _torch.empty(shape, dtype=dtype, device=device)
     if not isinstance(out, _torch.Tensor) or out.device != device or out.dtype != dtype or tuple(out.shape) != tuple(shape):
         raise ValueError(f"out must be a {dtype} tensor of shape {tuple(shape)} on {device}")
-    if out.requires_grad:
-        raise ValueError("out must not require a gradient")
+    if out.requires_grad or out.is_neg():
+        raise ValueError("out must not require a gradient or be a negated view")
     if out.shape[1] > 1 and out.stride(1) != 1 or out.shape[0] > 1 and out.stride(0) < out.shape[1]:
         raise ValueError("out must have unit stride along its rows and rows that do not overlap")
     return out
@@ -221,6 +221,9 @@ def fp4_quantize(x, format="nvfp4"):
     s0, s1 = x.stride()
     if cols > 1 and s1 != 1 or rows > 1 and s0 < cols:
         raise ValueError("x must have unit stride along its rows and rows that do not overlap")
+    if x.is_neg():
+        x = x.resolve_neg()
+        s0 = x.stride(0)
     m = Fp4Matrix._empty(rows, cols, format, x.device)
     _call(m.device, L.rfx_fp4_quantize, x.data_ptr(), code, s0 if rows > 1 else cols, m._p)
     return m

@@ -186,6 +186,52 @@ def test_product_half_outputs(fmt, dtype):
         _product_check(rng, fmt, m, n, k, dtype, spread=1)
 
 
+@pytest.mark.parametrize("m,k", [(4, 64), (4, 4096), (40, 200), (300, 300)])
+def test_product_of_scales_outside_fp32(m, k):
+    """Matrix scales whose product overflows or vanishes, where the results need not."""
+    import torch
+    import rfx_b200
+    rng = np.random.default_rng(m + k)
+    n = 200
+    x = rng.integers(1, 7, (m, k)).astype(np.float32)
+    y = rng.integers(1, 7, (n, k)).astype(np.float32)
+    x[1], y[3] = 0, 0
+    x[2, : k // 2], y[4, k // 2:] = 0, 0  # halves of which nothing meets: x[2] . y[4] = 0
+    def product(e, f):
+        mats, vals = [], []
+        for t, s in ((x, e), (y, f)):
+            t = t * np.float32(2.0 ** s)
+            mats.append(rfx_b200.fp4_quantize(torch.from_numpy(t).cuda()))
+            vals.append(ref.values(*ref.quantize(t, "nvfp4"), "nvfp4"))
+        got = rfx_b200.fp4_product(*mats).double().cpu().numpy()
+        rfx_b200.fp4_status()
+        return got, vals[0] @ vals[1].T
+    got, want = product(120, 110)  # every nonzero result is beyond fp32
+    assert np.array_equal(got, np.where(want > 0, np.inf, 0.0)) and (want == 0).sum() >= n + m
+    for e, f in ((-20, -118), (-118, -20), (100, -90)):
+        got, want = product(e, f)
+        # k additions of exact terms, all positive, off by at most 2^-23 each; one rounding, to a
+        # multiple of 2^-149 where the result has few bits left
+        assert (np.abs(got - want) <= (k * 2.0 ** -23 + 2.0 ** -24) * want + 2.0 ** -150).all()
+        assert (want > 0).sum() > 0.9 * (m - 1) * (n - 1)
+
+
+@pytest.mark.parametrize("m,k", [(4, 64), (4, 4096), (40, 200), (300, 300)])
+@pytest.mark.parametrize("fmt", FMTS)
+def test_product_of_nan_rows(fmt, m, k):
+    """A block that is not finite makes its row's products NaN and no others."""
+    import torch
+    import rfx_b200
+    rng = np.random.default_rng(m + k)
+    x, y = rng.standard_normal((m, k)).astype(np.float32), rng.standard_normal((150, k)).astype(np.float32)
+    x[2, k - 1], y[7, 0], y[130, 20] = np.nan, np.inf, -np.inf
+    got = rfx_b200.fp4_product(*(rfx_b200.fp4_quantize(torch.from_numpy(t).cuda(), format=fmt) for t in (x, y)))
+    rfx_b200.fp4_status()
+    want = np.zeros((m, 150), bool)
+    want[2], want[:, [7, 130]] = True, True
+    assert np.array_equal(np.isnan(got.cpu().numpy()), want)
+
+
 def _topk_check(a, b, va, vb, k, fmt, self_offset=None):
     import rfx_b200
     idx, val = rfx_b200.fp4_topk(a, b, k, self_offset=self_offset)
