@@ -446,7 +446,8 @@ int rfx_prox_apply(void* ctx, const float* X_dev, int ncols, const int* nout_dev
 enum { RFX_FP4_MX = 0, RFX_FP4_NV = 1 };
 enum { RFX_F32 = 0, RFX_BF16 = 1, RFX_F16 = 2 };
 
-/* A matrix's device buffers, sized by rfx_fp4_sizes, 16-byte aligned.  The layout is the
+/* A matrix's device buffers, sized by rfx_fp4_sizes, 16-byte aligned; rows <= 2^31 - 256, cols
+ * <= 16,776,960.  The layout is the
  * library's (tiles of 128 rows); a view of rows [r, r + n) with r a multiple of 128 is the same
  * struct with codes_dev + r * pitch, scales_dev + r / 128 * tile_bytes, bounds_dev + r / 128. */
 typedef struct {

@@ -38,7 +38,7 @@ namespace {
 using rfx::F4;
 
 constexpr int kMaxDevices = 64;
-constexpr int kMaxCols = 1 << 24;
+constexpr int kMaxCols = 65535 * 256;  // a grid's second axis of 256 columns a block
 
 // What a call needs to know about the current device, looked up once per device.
 struct DeviceInfo {
@@ -68,7 +68,7 @@ bool aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 void check_shape(int format, int rows, int cols) {
     require(format == RFX_FP4_MX || format == RFX_FP4_NV, RFX_ERR_ARG, "format must be RFX_FP4_MX or RFX_FP4_NV");
     require(rows >= 0 && rows <= 0x7fffff00, RFX_ERR_ARG, "rows out of range");
-    require(cols >= 1 && cols <= kMaxCols, RFX_ERR_ARG, "cols must be in [1, 2^24]");
+    require(cols >= 1 && cols <= kMaxCols, RFX_ERR_ARG, "cols must be in [1, 16776960]");
 }
 
 F4 matrix_of(const rfx_fp4_matrix* m, const char* what) {

@@ -22,6 +22,7 @@ from . import _abi as A
 
 FORMATS = A.FP4_FORMATS
 _BLOCK = {"mxfp4": 32, "nvfp4": 16}
+MAX_ROWS, MAX_COLS = 2 ** 31 - 256, 16776960
 TOPK_MAX_COLS = 256
 TOPK_MAX_K = 64
 
@@ -59,6 +60,11 @@ def _check_format(format):
         raise ValueError(f"format must be 'mxfp4' or 'nvfp4', not {format!r}")
 
 
+def _check_shape(rows, cols):
+    if rows > MAX_ROWS or not 1 <= cols <= MAX_COLS:
+        raise ValueError(f"a matrix has at most {MAX_ROWS} rows and 1 to {MAX_COLS} columns, not {rows} x {cols}")
+
+
 def _call(device, fn, *args):
     """fn(*args, stream) with the tensors' device current and its current stream."""
     cuda = _torch.cuda
@@ -87,6 +93,7 @@ class Fp4Matrix:
 
     @classmethod
     def _empty(cls, rows, cols, format, device):
+        _check_shape(rows, cols)
         m = object.__new__(cls)
         # the layout of rfx_fp4_sizes
         padded = (cols + 63) // 64 * 64

@@ -42,6 +42,19 @@ def test_sizes():
     _fails(L.rfx_fp4_sizes(0, 1, 1, None), "null")
 
 
+def test_largest_shapes():
+    """Rows and columns beyond a 32-bit count or a launch's grid are refused, not cut short."""
+    L = A.load_library()
+    lay = A.Fp4Layout()
+    assert L.rfx_fp4_sizes(1, fp4.MAX_ROWS, fp4.MAX_COLS, C.byref(lay)) == 0
+    assert lay.codes == fp4.MAX_ROWS * (fp4.MAX_COLS // 2)
+    _fails(L.rfx_fp4_sizes(1, fp4.MAX_ROWS + 1, 1, C.byref(lay)), "rows")
+    _fails(L.rfx_fp4_sizes(1, 1, fp4.MAX_COLS + 1, C.byref(lay)), "cols")
+    for rows, cols in ((fp4.MAX_ROWS + 1, 1), (2 ** 32 + 3, 64), (1, fp4.MAX_COLS + 1), (1, 0)):
+        with pytest.raises(ValueError, match="at most"):
+            fp4._check_shape(rows, cols)
+
+
 def test_abi_refusals():
     L = A.load_library()
     at = C.addressof

@@ -146,6 +146,26 @@ def test_parts_round_trip(fmt, rows, cols):
         assert float(gs) == g
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+def test_widest_matrix(fmt):
+    """One row of the most columns, and its product with itself."""
+    import torch
+    import rfx_b200
+    from rfx_b200 import fp4
+    x = torch.zeros(1, fp4.MAX_COLS, device="cuda", dtype=torch.bfloat16)
+    x[0, -5:] = torch.tensor([1.0, -2.0, 3.0, 4.0, 6.0])
+    x[0, 7] = 6.0
+    m = rfx_b200.fp4_quantize(x, format=fmt)
+    assert torch.equal(m.dequantize(torch.bfloat16), x)
+    assert float(rfx_b200.fp4_product(m, m)[0, 0]) == 1 + 4 + 9 + 16 + 36 + 36
+    c, s, g = m.parts()
+    again = rfx_b200.Fp4Matrix.from_parts(c, s, g, cols=fp4.MAX_COLS, format=fmt)
+    assert torch.equal(again.dequantize(torch.bfloat16), x)
+    rfx_b200.fp4_status()
+    with pytest.raises(ValueError, match="at most"):
+        rfx_b200.fp4_quantize(torch.zeros(1, 1, device="cuda").expand(1, fp4.MAX_COLS + 1).contiguous(), format=fmt)
+
+
 def _product_check(rng, fmt, m, n, k, dtype="float32", spread=4):
     import torch
     import rfx_b200
