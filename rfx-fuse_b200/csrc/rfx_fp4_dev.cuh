@@ -23,6 +23,14 @@ __device__ __forceinline__ float e4m3_value(uint32_t byte) {
     return __half2float(__ushort_as_half((unsigned short)(h2 & 0xFFFF)));
 }
 
+// The two e4m3 bytes in the low half of w -> two floats, exactly.
+__device__ __forceinline__ float2 e4m3_pair(uint32_t w) {
+    uint32_t h2;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"((uint16_t)w));
+    return make_float2(__half2float(__ushort_as_half((unsigned short)(h2 & 0xFFFFu))),
+                       __half2float(__ushort_as_half((unsigned short)(h2 >> 16))));
+}
+
 // e8m0 byte -> 2^(byte - 127) (0: the denormal 2^-127; 255: NaN).
 __device__ __forceinline__ float e8m0_value(uint32_t byte) {
     if (byte == 255u) return __int_as_float(0x7fc00000);
@@ -101,13 +109,18 @@ __device__ __forceinline__ float e2m1_value(uint32_t code) {
     return (code & 8u) ? -m : m;
 }
 
-// acc + four times the dot product of eight codes (decoded as signed bytes of twice their values, q
-// four, r the next four) with the eight codes of w, exactly.
-__device__ __forceinline__ int e2m1_dot8(int q, int r, uint32_t w, int acc) {
-    const uint32_t x = w ^ 0x88888888u;
-    acc = __dp4a(q, (int)e2m1_pos4(w), acc);
-    acc = __dp4a(r, (int)e2m1_pos4(w >> 16), acc);
-    const int neg = __dp4a(r, (int)e2m1_pos4(x >> 16), __dp4a(q, (int)e2m1_pos4(x), 0));
+// acc + four times the dot product of sixteen codes (decoded as signed bytes of twice their values)
+// with the sixteen codes of w0 and w1, exactly.
+__device__ __forceinline__ int e2m1_dot16(int4 q, uint32_t w0, uint32_t w1, int acc) {
+    const uint32_t x0 = w0 ^ 0x88888888u, x1 = w1 ^ 0x88888888u;
+    int neg = __dp4a(q.x, (int)e2m1_pos4(x0), 0);
+    acc = __dp4a(q.x, (int)e2m1_pos4(w0), acc);
+    neg = __dp4a(q.y, (int)e2m1_pos4(x0 >> 16), neg);
+    acc = __dp4a(q.y, (int)e2m1_pos4(w0 >> 16), acc);
+    neg = __dp4a(q.z, (int)e2m1_pos4(x1), neg);
+    acc = __dp4a(q.z, (int)e2m1_pos4(w1), acc);
+    neg = __dp4a(q.w, (int)e2m1_pos4(x1 >> 16), neg);
+    acc = __dp4a(q.w, (int)e2m1_pos4(w1 >> 16), acc);
     return acc - neg;
 }
 

@@ -11,7 +11,7 @@
 //   k_f4_keys  products of 128 rows of a with b's tiles of 128 rows (tcgen05, block-scaled); of
 //              every row's 32 neighbouring accumulators only the maximum is kept, as the upper 16
 //              bits of its order-preserving integer (rounded down).
-//   k_f4_pick  a block per row of a.  Its threads' shares of the keys are groups; the k-th largest of
+//   k_f4_pick  a block per row of a (k_f4_pick_warp: a warp, for many rows with few keys).  Its threads' shares of the keys are groups; the k-th largest of
 //              the groups' largest keys, L, is a lower bound of the k-th largest accumulator: k
 //              columns have L or more, so the k-th value is at least L - err, and a column of the
 //              answer has an accumulator of at least L - 2 err.  Of the chunks whose key reaches that
@@ -392,9 +392,8 @@ __device__ __noinline__ double f4_exact(const int* qa, const float* sa, const ui
 #pragma unroll
         for (int h = 0; h < 2; ++h) {  // 32 columns
             const uint4 y = __ldg(cb + 2 * c + h);
-            const int* q = qa + 16 * c + 8 * h;
-            const int lo = e2m1_dot8(q[2], q[3], y.y, e2m1_dot8(q[0], q[1], y.x, 0));
-            const int hi = e2m1_dot8(q[6], q[7], y.w, e2m1_dot8(q[4], q[5], y.z, 0));
+            const int4* q = reinterpret_cast<const int4*>(qa + 16 * c + 8 * h);
+            const int lo = e2m1_dot16(q[0], y.x, y.y, 0), hi = e2m1_dot16(q[1], y.z, y.w, 0);
             if (kNv) {
                 // e4m3 times e4m3 times the integer: exact, and so is every sum
                 v += (double)sa[4 * c + 2 * h] * (double)e4m3_value((wb >> (16 * h)) & 0xFFu) * (double)lo;
@@ -414,26 +413,28 @@ __device__ __noinline__ double f4_exact(const int* qa, const float* sa, const ui
 // a few units of 2^-24 of the terms' sum), so that the same err covers it.
 template <int kNv>
 __device__ __forceinline__ float f4_estimate64(const int* qa, const float* sa, uint4 y0, uint4 y1, uint32_t wb, float v) {
+    // an integer dot product added to the bits of 1.5 * 2^23 is a float, less 1.5 * 2^23
+    constexpr int kMagic = 0x4B400000;
+    constexpr float kMagicF = 12582912.0f;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const uint4 y = h ? y1 : y0;
-        const int4 q0 = *reinterpret_cast<const int4*>(qa + 8 * h);
-        const int4 q1 = *reinterpret_cast<const int4*>(qa + 8 * h + 4);
-        const int lo = e2m1_dot8(q0.z, q0.w, y.y, e2m1_dot8(q0.x, q0.y, y.x, 0));
-        const int hi = e2m1_dot8(q1.z, q1.w, y.w, e2m1_dot8(q1.x, q1.y, y.z, 0));
+        const int4* q = reinterpret_cast<const int4*>(qa + 8 * h);
         if (kNv) {
-            v = fmaf(sa[2 * h] * e4m3_value((wb >> (16 * h)) & 0xFFu), (float)lo, v);
-            v = fmaf(sa[2 * h + 1] * e4m3_value((wb >> (16 * h + 8)) & 0xFFu), (float)hi, v);
+            const float2 sb = e4m3_pair(wb >> (16 * h));
+            v = fmaf(sa[2 * h] * sb.x, __int_as_float(e2m1_dot16(q[0], y.x, y.y, kMagic)) - kMagicF, v);
+            v = fmaf(sa[2 * h + 1] * sb.y, __int_as_float(e2m1_dot16(q[1], y.z, y.w, kMagic)) - kMagicF, v);
         } else {
-            v = fmaf(sa[h] * e8m0_value((wb >> (8 * h)) & 0xFFu), (float)(lo + hi), v);
+            const int dot = e2m1_dot16(q[1], y.z, y.w, e2m1_dot16(q[0], y.x, y.y, kMagic));
+            v = fmaf(sa[h] * e8m0_value((wb >> (8 * h)) & 0xFFu), __int_as_float(dot) - kMagicF, v);
         }
     }
     return v;
 }
 
 // kT threads a row: 256, four rows an SM; 128, eight rows an SM, when a row has few keys (each step
-// then waits for memory or a barrier, and rows hide one another's waits: 10,000 x 10,000 top-10
-// 136 us with 256); 1024 when there are too few rows to fill the GPU.
+// then waits for memory or a barrier, and rows hide one another's waits); 1024 when there are too few
+// rows to fill the GPU.
 template <int kNv, int kT>
 __global__ void __launch_bounds__(kT, kT == 1024 ? 1 : 1024 / kT)
 k_f4_pick(PickArgs p) {
@@ -524,16 +525,19 @@ k_f4_pick(PickArgs p) {
     }
     __syncthreads();
     const bool forced = s_forced != 0;
-    // a thread's units are a group: L is the kp-th largest of the groups' largest keys, by
-    // bisection of its 16 bits (0: there are fewer)
+    // a thread's units are a group: L is the kp-th largest of the groups' largest keys, by bisection of
+    // its 16 bits (0: there are fewer), or a little less, as soon as kp groups have it
     uint32_t top = 0;
     for (int t = tid; t < nunits; t += kT) {
         const uint32_t key = tops[t];
         if (key != kAlways) top = max(top, key);
     }
     uint32_t s_key = 0;
-    for (uint32_t bit = 0x8000u; bit; bit >>= 1)
-        if (__syncthreads_count(top >= (s_key | bit)) >= kp) s_key |= bit;
+    for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
+        const int c = __syncthreads_count(top >= (s_key | bit));
+        if (c >= kp) s_key |= bit;
+        if (c == kp) break;
+    }
     const double err = (double)s_err;
     // the k-th value is at least this
     double floor_v = s_key > key_of(-__int_as_float(0x7f800000)) ? (double)key_floor(s_key) - err : kNegInf;
@@ -683,6 +687,198 @@ k_f4_pick(PickArgs p) {
     }
 }
 
+// The same for rows with few keys, a warp a row: the keys stay in registers, nothing waits for a
+// barrier, and an SM works on 32 rows (10,000 x 10,000, top 10: 52 us, 81 with a block of 128 threads a
+// row; it issues 0.84 instructions a cycle and scheduler, 4,200 a row, half of them estimates).  A group
+// is a word of two keys.
+constexpr int kWFound = 128;  // columns waiting to be ranked: 32 more always fit beside the best 64
+
+template <int kNv>
+__global__ void __launch_bounds__(128, 8)
+k_f4_pick_warp(PickArgs p, int rows) {
+    __shared__ __align__(16) int s_qa[4][kF4TopkK / 4];
+    __shared__ float s_sa[4][kF4TopkK / 16];
+    __shared__ double s_fv[4][kWFound];  // as in k_f4_pick
+    __shared__ int s_fj[4][kWFound];
+    __shared__ uint16_t s_list[4][kSmallKeys];
+    constexpr uint32_t kAll = 0xFFFFFFFFu;
+    const double kNegInf = -__longlong_as_double(0x7ff0000000000000ll);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int* qa = s_qa[warp];
+    float* sa = s_sa[warp];
+    double* fv = s_fv[warp];
+    int* fj = s_fj[warp];
+    uint16_t* list = s_list[warp];
+    const int q = blockIdx.x * 4 + warp;  // row of the batch
+    const long long i = (long long)p.row0 + q;
+    if (q >= rows) return;
+    const int kp = p.self >= 0 ? p.k + 1 : p.k;
+    const int self = p.self >= 0 ? (int)(p.self + i) : -1;
+    const uint4* keys = reinterpret_cast<const uint4*>(p.keys + (long long)q * p.nspan * (kSpanKeys / 2));
+    const int nvec = p.nspan * (kSpanKeys / 8), steps = p.b.Kp / 64;
+    auto codes_of = [&](int j) { return reinterpret_cast<const uint4*>(p.b.codes + (long long)j * p.b.pitch()); };
+    auto scales_of = [&](int j) {
+        return p.b.scales + (long long)(j >> 7) * (p.b.natoms * kF4Atom) + (j & 31) * 16 + ((j >> 5) & 3) * 4;
+    };
+
+    for (int t = lane; t < p.a.Kp / 4; t += 32) {
+        const uint32_t w = *reinterpret_cast<const uint16_t*>(p.a.codes + i * p.a.pitch() + 2 * t);
+        int d = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d |= ((int)(2.0f * e2m1_value((w >> (4 * e)) & 15u)) & 0xFF) << (8 * e);
+        qa[t] = d;
+    }
+    float s0 = 0.0f;
+    if (lane < p.a.Kp / (kNv ? 16 : 32)) sa[lane] = s0 = f4_scale_value(kNv, p.a.scales[f4_scale_at(p.a, i, lane)]);
+    wait_for_previous();  // the keys
+    int n_known = 0, n_found = 0;
+    if (!__any_sync(kAll, !(s0 == s0))) {  // a NaN row is nobody's neighbour and has none
+        uint32_t x[16];  // words of two keys
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint4 y = lane + 32 * e < nvec ? __ldg(keys + lane + 32 * e) : make_uint4(0, 0, 0, 0);
+            x[4 * e] = y.x;
+            x[4 * e + 1] = y.y;
+            x[4 * e + 2] = y.z;
+            x[4 * e + 3] = y.w;
+        }
+        float worst = 0.0f;
+        bool forced = false;
+        for (int t = lane; t < p.nerrs; t += 32) {
+            const float y = __ldg(p.errs + t);
+            forced |= y < 0.0f;
+            worst = fmaxf(worst, fabsf(y));
+        }
+        for (int o = 16; o; o >>= 1) worst = fmaxf(worst, __shfl_xor_sync(kAll, worst, o));
+        forced = __any_sync(kAll, forced);
+        const double err = (double)fmaxf(worst, 1e-37f);
+        // L: the kp-th largest of the words' larger keys, by bisection as in k_f4_pick
+        uint32_t s_key = 0;
+        {
+            uint32_t top[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const uint32_t lo = x[e] & 0xFFFFu, hi = x[e] >> 16;
+                top[e] = max(lo == kAlways ? 0u : lo, hi == kAlways ? 0u : hi);
+            }
+            for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
+                int c = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (32 * e < nvec) {
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) c += top[4 * e + h] >= (s_key | bit);
+                    }
+                }
+                c = __reduce_add_sync(kAll, c);
+                if (c >= kp) s_key |= bit;
+                if (c == kp) break;
+            }
+        }
+        double floor_v = s_key > key_of(-__int_as_float(0x7f800000)) ? (double)key_floor(s_key) - err : kNegInf;
+        int n_list = 0;
+        {
+            const uint32_t bar = max(key_of(__double2float_rd(floor_v - err)), 1u);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (32 * e < nvec) {
+                    const int vec = lane + 32 * e;
+                    const int chunk0 = (vec / kAccs * kSpan + vec % kAccs) * 4;  // as in k_f4_pick
+#pragma unroll
+                    for (int h = 0; h < 8; ++h) {
+                        const bool in = (h & 1 ? x[4 * e + h / 2] >> 16 : x[4 * e + h / 2] & 0xFFFFu) >= bar;
+                        const uint32_t who = __ballot_sync(kAll, in);
+                        if (in) list[n_list + __popc(who & ((1u << lane) - 1))] = (uint16_t)(chunk0 + 4 * kAccs * (h >> 2) + (h & 3));
+                        n_list += __popc(who);
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        float least = 4.0f * __double2float_rd(floor_v - err);  // of an estimate
+        // Evaluates what was found exactly, ranks it, keeps the best k at the front, raises the floor.
+        auto rank_found = [&]() {
+            __syncwarp();
+            for (int t = n_known + lane; t < n_found; t += 32) {
+                const double y = f4_exact<kNv>(qa, sa, codes_of(fj[t]), scales_of(fj[t]), steps);
+                const bool in = y * 0.25 >= floor_v;  // false for NaN
+                fv[t] = in ? y : kNegInf;
+                if (!in) fj[t] = 0x7FFFFFFF;
+            }
+            __syncwarp();
+            double v[kWFound / 32];
+            int j[kWFound / 32], r[kWFound / 32], kept = 0;
+#pragma unroll
+            for (int e = 0; e < kWFound / 32; ++e) {
+                const int t = lane + 32 * e;
+                v[e] = t < n_found ? fv[t] : kNegInf;
+                j[e] = t < n_found ? fj[t] : 0x7FFFFFFF;
+                r[e] = 0;
+            }
+#pragma unroll
+            for (int e = 0; e < kWFound / 32; ++e) {
+                if (32 * e < n_found) {
+                    int c = 0;
+#pragma unroll 4
+                    for (int o = 0; o < n_found; ++o) c += f4_better(fv[o], fj[o], v[e], j[e]);
+                    r[e] = c;
+                }
+                if (j[e] == 0x7FFFFFFF) r[e] = kWFound;
+                kept += r[e] < p.k;
+            }
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < kWFound / 32; ++e)
+                if (r[e] < p.k) {
+                    fv[r[e]] = v[e];
+                    fj[r[e]] = j[e];
+                }
+            n_known = n_found = __reduce_add_sync(kAll, kept);
+            __syncwarp();
+            if (n_known == p.k) floor_v = fmax(floor_v, 0.25 * fv[p.k - 1]);
+            least = 4.0f * __double2float_rd(floor_v - err);
+        };
+        // the listed chunks, a lane a column; the next chunk's first 64 columns are loaded under
+        // this one's arithmetic
+        const int most = min(kWFound, 2 * p.k + 32) - 32;  // the cost of ranking grows as its square
+        uint4 y0, y1;
+        uint32_t sc;
+        auto fetch = [&](int c) {
+            const int j = min((int)list[c] * 32 + lane, p.b.rows - 1);
+            y0 = __ldg(codes_of(j));
+            y1 = __ldg(codes_of(j) + 1);
+            sc = __ldg(reinterpret_cast<const uint32_t*>(scales_of(j)));
+        };
+        if (n_list > 0) fetch(0);
+        for (int c = 0; c < n_list; ++c) {
+            const int j = (int)list[c] * 32 + lane;
+            const uint4 z0 = y0, z1 = y1;
+            const uint32_t zs = sc;
+            if (c + 1 < n_list) fetch(c + 1);
+            float v = f4_estimate64<kNv>(qa, sa, z0, z1, zs, 0.0f);
+            for (int st = 1; st < steps; ++st) {
+                const int jc = min(j, p.b.rows - 1);
+                const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(scales_of(jc) + (kNv ? st : st >> 1) * kF4Atom));
+                v = f4_estimate64<kNv>(qa + 16 * st, sa + (kNv ? 4 : 2) * st, __ldg(codes_of(jc) + 2 * st),
+                                       __ldg(codes_of(jc) + 2 * st + 1), !kNv && (st & 1) ? w >> 16 : w, v);
+            }
+            if (n_found > most) rank_found();
+            // without a bound on the terms fp32 could overflow: rank_found decides
+            const bool in = j < p.b.rows && j != self && (forced || v >= least);
+            const uint32_t who = __ballot_sync(kAll, in);
+            if (in) fj[n_found + __popc(who & ((1u << lane) - 1))] = j;
+            n_found += __popc(who);
+        }
+        rank_found();
+    }
+    const double g = (double)__ldg(p.a.gs) * (double)__ldg(p.b.gs);
+    for (int s = lane; s < p.k; s += 32) {
+        const bool in = s < n_known;
+        p.idx[i * p.k + s] = in ? fj[s] : -1;
+        p.val[i * p.k + s] = in ? (float)(fv[s] * 0.25 * g) : -__int_as_float(0x7f800000);
+    }
+}
+
 __global__ void k_f4_topk_none(long long n, int* idx, float* val) {
     for (long long t = (long long)blockIdx.x * blockDim.x + threadIdx.x; t < n; t += (long long)gridDim.x * blockDim.x) {
         idx[t] = -1;
@@ -728,6 +924,20 @@ cudaError_t launch_pick(const PickArgs& q, int rows, cudaStream_t st) {
     cfg.attrs = at;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, k_f4_pick<kNv, kT>, q);
+}
+
+template <int kNv>
+cudaError_t launch_pick_warp(const PickArgs& q, int rows, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((rows + 3) / 4));
+    cfg.blockDim = dim3(128);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k_f4_pick_warp<kNv>, q, rows);
 }
 
 }  // namespace
@@ -778,8 +988,14 @@ cudaError_t f4_topk(const F4& a, const F4& b, int k, long long self, int* idx, f
         if (e != cudaSuccess) return e;
         q.row0 = (int)r0;
         q.nerrs = grid;
-        const int threads = rows <= 2 * sms ? 1024 : plan.nspan * kSpanKeys <= kSmallKeys ? 128 : 256;
-        if (b.nv) e = threads == 1024 ? launch_pick<1, 1024>(q, rows, st) : threads == 128 ? launch_pick<1, 128>(q, rows, st)
+        const bool few_keys = plan.nspan * kSpanKeys <= kSmallKeys;
+        // A warp takes about 25 us for its row (10,000 columns) to 80 (32,000), a block 3 to 5, so
+        // the warps' kernel needs an SM nearly full of rows: at 1,200 rows 32.8 against 23.7 us (both
+        // kernels, 10,000 columns) and 90 / 47 (32,000), at 2,400 32.8 / 32.7, at 4,000 100 / 108,
+        // at 10,000 62.6 / 89, at 20,000 356 / 458.
+        const int threads = rows <= 2 * sms ? 1024 : !few_keys ? 256 : rows < 24 * sms ? 128 : 32;
+        if (threads == 32) e = b.nv ? launch_pick_warp<1>(q, rows, st) : launch_pick_warp<0>(q, rows, st);
+        else if (b.nv) e = threads == 1024 ? launch_pick<1, 1024>(q, rows, st) : threads == 128 ? launch_pick<1, 128>(q, rows, st)
                                                                                            : launch_pick<1, 256>(q, rows, st);
         else e = threads == 1024 ? launch_pick<0, 1024>(q, rows, st) : threads == 128 ? launch_pick<0, 128>(q, rows, st)
                                                                                       : launch_pick<0, 256>(q, rows, st);

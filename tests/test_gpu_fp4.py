@@ -406,3 +406,34 @@ def test_topk_masses_of_ties():
         for i in pick:
             wi, wv = ref.topk(vb[i:i + 1], vb, 33, int(i), "nvfp4")
             assert np.array_equal(idx[i].cpu().numpy(), wi[0]) and np.array_equal(val[i].cpu().numpy(), wv[0])
+
+
+@pytest.mark.parametrize("fmt,n,k,top,kind", [
+    ("nvfp4", 10, 64, 20, "plain"), ("mxfp4", 1, 20, 1, "plain"), ("nvfp4", 3700, 64, 64, "plain"), ("mxfp4", 3700, 50, 10, "self"),
+    ("nvfp4", 3700, 64, 33, "ties"), ("mxfp4", 3700, 64, 64, "ties"), ("nvfp4", 32700, 256, 50, "self"),
+    ("mxfp4", 30000, 200, 64, "extreme"), ("nvfp4", 5000, 130, 1, "extreme"), ("mxfp4", 3700, 64, 50, "equal")])
+def test_topk_a_warp_a_row(fmt, n, k, top, kind):
+    """Thousands of rows against few keys; a sample of the queries is checked."""
+    import rfx_b200
+    m = 3700
+    rng = np.random.default_rng(n + k + top)
+    cb, sb = _parts(rng, n, k, fmt, spread=2)
+    if kind in ("ties", "equal"):
+        which = rng.integers(0, 5 if kind == "ties" else 1, n)
+        cb, sb = cb[which], sb[which]
+    if kind == "extreme":
+        sb[rng.integers(0, n, n // 50), 0] = 255 if fmt == "mxfp4" else 127
+        sb[50:90] = rng.integers(0, 8, (40, sb.shape[1]))
+        sb[100:110] = rng.integers(180, 200, (10, sb.shape[1])) if fmt == "mxfp4" else 126
+    same = kind != "plain" and n >= m
+    ca, sa = (cb[:m], sb[:m]) if same else _parts(rng, m, k, fmt, spread=2)
+    a, b = _matrix(ca, sa, k, fmt), _matrix(cb, sb, k, fmt)
+    idx, val = rfx_b200.fp4_topk(a, b, top, self_offset=0 if same else None)
+    rfx_b200.fp4_status()
+    idx, val = idx.cpu().numpy(), val.cpu().numpy()
+    pick = np.unique(np.concatenate([[0, m - 1], np.arange(48, 56), np.arange(99, 103), rng.integers(0, m, 12)]))
+    vb = ref.values(cb, sb, 1.0, fmt)
+    with np.errstate(all="ignore"):
+        for i in pick:
+            wi, wv = ref.topk(ref.values(ca[i:i + 1], sa[i:i + 1], 1.0, fmt), vb, top, int(i) if same else None, fmt)
+            assert np.array_equal(idx[i], wi[0]) and np.array_equal(val[i], wv[0]), i
