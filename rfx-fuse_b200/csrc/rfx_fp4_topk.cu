@@ -11,18 +11,18 @@
 //   k_f4_keys  products of 128 rows of a with b's tiles of 128 rows (tcgen05, block-scaled); of
 //              every row's 32 neighbouring accumulators only the maximum is kept, as the upper 16
 //              bits of its order-preserving integer (rounded down).
-//   k_f4_pick  a block per row of a (k_f4_pick_warp: a warp, for many rows with few keys).  Its threads' shares of the keys are groups; the k-th largest of
-//              the groups' largest keys, L, is a lower bound of the k-th largest accumulator: k
+//   k_f4_pick  a block per row of a (k_f4_pick_warp: a warp, for many rows with few keys).  The
+//              keys are dealt to groups; the k-th largest of the groups' largest keys, L, is a lower bound of the k-th largest accumulator: k
 //              columns have L or more, so the k-th value is at least L - err, and a column of the
 //              answer has an accumulator of at least L - 2 err.  Of the chunks whose key reaches that
 //              (about k, 1.2 k where groups are few) every column is estimated in fp32; what
 //              reaches L - 2 err is evaluated exactly and ranked by counting who is better.
 //
 // What the first kernel leaves is 2 bytes for 32 pairs.  Rows are taken in batches of 256 MB of keys
-// (4,096 x 1,000,000 in one: 441 us, in batches of 120 MB 490: each batch ends with idle SMs).
+// (4,096 x 1,000,000 in one: 411 us; when it took 441, in batches of 120 MB 490: each batch ends with idle SMs).
 // k_f4_keys: 300 cycles a tile of 128 x 128, of which the ALU's 128 for maxima (a 3-input maximum
 // takes two issue slots) and 90 for keys and bookkeeping; k_f4_pick: half the issue slots, latency
-// of its barriers and loads between them.  Times of both at 4,096 x 1,000,000: 301 and 155 us.
+// of its barriers and loads between them.  Times of both at 4,096 x 1,000,000: 301 and 131 us.
 #include <algorithm>
 
 #include "rfx_fp4_mma.cuh"
@@ -36,7 +36,7 @@ constexpr int kSpan = 6;                     // tiles of b in a unit of work: tw
 constexpr int kSpanKeys = 4 * kSpan;         // keys of a row and a span
 constexpr float kEps = 1.0f / 32768.0f;
 constexpr uint32_t kAlways = 0xFFFFu;        // key of a chunk that has to be looked at (no float's)
-constexpr int kSmallKeys = 1024;             // keys of a row that 128 threads take
+constexpr int kWarpKeys = 1024;              // keys of a row that a warp can hold
 
 struct KeysArgs {
     F4 a, b;
@@ -432,16 +432,16 @@ __device__ __forceinline__ float f4_estimate64(const int* qa, const float* sa, u
     return v;
 }
 
-// kT threads a row: 256, four rows an SM; 128, eight rows an SM, when a row has few keys (each step
-// then waits for memory or a barrier, and rows hide one another's waits); 1024 when there are too few
-// rows to fill the GPU.
+// kT threads a row: 128, eight rows an SM, which hide one another's waits for memory and barriers
+// (both kernels at 4,096 x 1,000,000, top 50: 411 us, 435 with 256 threads; 100,000 rows: 128, 150); 1024
+// when there are too few rows to fill the GPU.
 template <int kNv, int kT>
 __global__ void __launch_bounds__(kT, kT == 1024 ? 1 : 1024 / kT)
 k_f4_pick(PickArgs p) {
-    constexpr int kUnits = kT == 128 ? kSmallKeys : 4096;  // units of keys: a key, or every kUnits-th vector of 8
+    constexpr int kUnits = kT == 128 ? 2048 : 4096;  // units of keys: a key, or every kUnits-th vector of 8
     constexpr int kFound = kT == 128 ? 512 : 1024;         // columns waiting to be ranked
     constexpr int kScan = kT == 128 ? 128 : 256;           // units a round turns into chunks
-    constexpr int kList = (kT == 128 ? 1 : 8) * kScan + 256;  // chunks waiting to be looked at
+    constexpr int kList = 8 * kScan + 256;  // chunks waiting to be looked at
     __shared__ __align__(16) int qa[kF4TopkK / 4];
     __shared__ float sa[kF4TopkK / 16];
     __shared__ double fv[kFound];       // found: values (4 x) of the first n_known, columns of all
@@ -466,7 +466,7 @@ k_f4_pick(PickArgs p) {
     auto scales_of = [=](int j) {
         return b_scales + (long long)(j >> 7) * tile_bytes + (j & 31) * 16 + ((j >> 5) & 3) * 4;
     };
-    const bool small = kT == 128 || nvec * 8 <= kUnits;  // a unit is a key
+    const bool small = nvec * 8 <= kUnits;  // a unit is a key
     const int nunits = small ? nvec * 8 : min(nvec, kUnits);
 
     // the row, decoded, and its scales
@@ -525,18 +525,47 @@ k_f4_pick(PickArgs p) {
     }
     __syncthreads();
     const bool forced = s_forced != 0;
-    // a thread's units are a group: L is the kp-th largest of the groups' largest keys, by bisection of
+    // the units are dealt to groups: L is the kp-th largest of the groups' largest keys, by bisection of
     // its 16 bits (0: there are fewer), or a little less, as soon as kp groups have it
-    uint32_t top = 0;
-    for (int t = tid; t < nunits; t += kT) {
-        const uint32_t key = tops[t];
-        if (key != kAlways) top = max(top, key);
-    }
     uint32_t s_key = 0;
-    for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
-        const int c = __syncthreads_count(top >= (s_key | bit));
-        if (c >= kp) s_key |= bit;
-        if (c == kp) break;
+    if constexpr (kT == 1024) {
+        uint32_t top = 0;
+        for (int t = tid; t < nunits; t += kT) {
+            const uint32_t key = tops[t];
+            if (key != kAlways) top = max(top, key);
+        }
+        for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
+            const int c = __syncthreads_count(top >= (s_key | bit));
+            if (c >= kp) s_key |= bit;
+            if (c == kp) break;
+        }
+    } else {
+        // two groups a thread (one: 4,096 x 1,000,000, top 50 looks at an eighth more chunks); every warp
+        // finds L for itself, which costs less than a barrier a bit
+        __shared__ __align__(16) uint16_t group[2 * kT];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint32_t top = 0;
+            for (int t = tid + h * kT; t < nunits; t += 2 * kT) {
+                const uint32_t key = tops[t];
+                if (key != kAlways) top = max(top, key);
+            }
+            group[tid + h * kT] = (uint16_t)top;
+        }
+        __syncthreads();
+        constexpr int kW = kT / 32;  // words of two groups a lane
+        uint32_t x[kW];
+#pragma unroll
+        for (int e = 0; e < kW; ++e) x[e] = reinterpret_cast<const uint32_t*>(group)[lane + 32 * e];
+        for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
+            const uint32_t want = s_key | bit;
+            int c = 0;
+#pragma unroll
+            for (int e = 0; e < kW; ++e) c += ((x[e] & 0xFFFFu) >= want) + (x[e] >= want << 16);
+            c = __reduce_add_sync(0xFFFFFFFFu, c);
+            if (c >= kp) s_key = want;
+            if (c == kp) break;
+        }
     }
     const double err = (double)s_err;
     // the k-th value is at least this
@@ -700,7 +729,7 @@ k_f4_pick_warp(PickArgs p, int rows) {
     __shared__ float s_sa[4][kF4TopkK / 16];
     __shared__ double s_fv[4][kWFound];  // as in k_f4_pick
     __shared__ int s_fj[4][kWFound];
-    __shared__ uint16_t s_list[4][kSmallKeys];
+    __shared__ uint16_t s_list[4][kWarpKeys];
     constexpr uint32_t kAll = 0xFFFFFFFFu;
     const double kNegInf = -__longlong_as_double(0x7ff0000000000000ll);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -988,17 +1017,15 @@ cudaError_t f4_topk(const F4& a, const F4& b, int k, long long self, int* idx, f
         if (e != cudaSuccess) return e;
         q.row0 = (int)r0;
         q.nerrs = grid;
-        const bool few_keys = plan.nspan * kSpanKeys <= kSmallKeys;
+        const bool few_keys = plan.nspan * kSpanKeys <= kWarpKeys;
         // A warp takes about 25 us for its row (10,000 columns) to 80 (32,000), a block 3 to 5, so
         // the warps' kernel needs an SM nearly full of rows: at 1,200 rows 32.8 against 23.7 us (both
         // kernels, 10,000 columns) and 90 / 47 (32,000), at 2,400 32.8 / 32.7, at 4,000 100 / 108,
         // at 10,000 62.6 / 89, at 20,000 356 / 458.
-        const int threads = rows <= 2 * sms ? 1024 : !few_keys ? 256 : rows < 24 * sms ? 128 : 32;
+        const int threads = rows <= 2 * sms ? 1024 : few_keys && rows >= 24 * sms ? 32 : 128;
         if (threads == 32) e = b.nv ? launch_pick_warp<1>(q, rows, st) : launch_pick_warp<0>(q, rows, st);
-        else if (b.nv) e = threads == 1024 ? launch_pick<1, 1024>(q, rows, st) : threads == 128 ? launch_pick<1, 128>(q, rows, st)
-                                                                                           : launch_pick<1, 256>(q, rows, st);
-        else e = threads == 1024 ? launch_pick<0, 1024>(q, rows, st) : threads == 128 ? launch_pick<0, 128>(q, rows, st)
-                                                                                      : launch_pick<0, 256>(q, rows, st);
+        else if (threads == 128) e = b.nv ? launch_pick<1, 128>(q, rows, st) : launch_pick<0, 128>(q, rows, st);
+        else e = b.nv ? launch_pick<1, 1024>(q, rows, st) : launch_pick<0, 1024>(q, rows, st);
         if (e != cudaSuccess) return e;
         *launches += 2;
         if ((e = cudaGetLastError()) != cudaSuccess) return e;
