@@ -12,14 +12,14 @@
 //              every row's 32 neighbouring accumulators only the maximum is kept, as the upper 16
 //              bits of its order-preserving integer (rounded down).
 //   k_f4_pick  a block per row of a (k_f4_pick_warp: a warp, for many rows with few keys).  The
-//              keys are dealt to groups; the k-th largest of the groups' largest keys, L, is a lower bound of the k-th largest accumulator: k
-//              columns have L or more, so the k-th value is at least L - err, and a column of the
-//              answer has an accumulator of at least L - 2 err.  Of the chunks whose key reaches that
+//              keys are dealt to groups; the k-th largest of the groups' largest keys, L, is a lower
+//              bound of the k-th largest accumulator: k columns have L or more, so the k-th value is
+//              at least L - err, and a column of the answer has an accumulator of at least L - 2 err.  Of the chunks whose key reaches that
 //              (about k, 1.2 k where groups are few) every column is estimated in fp32; what
 //              reaches L - 2 err is evaluated exactly and ranked by counting who is better.
 //
 // What the first kernel leaves is 2 bytes for 32 pairs.  Rows are taken in batches of 256 MB of keys
-// (4,096 x 1,000,000 in one: 411 us; when it took 441, in batches of 120 MB 490: each batch ends with idle SMs).
+// (4,096 x 1,000,000 in one; when that took 441 us, batches of 120 MB took 490: each ends with idle SMs).
 // k_f4_keys: 300 cycles a tile of 128 x 128, of which the ALU's 128 for maxima (a 3-input maximum
 // takes two issue slots) and 90 for keys and bookkeeping; k_f4_pick: half the issue slots, latency
 // of its barriers and loads between them.  Times of both at 4,096 x 1,000,000: 301 and 131 us.
@@ -409,7 +409,7 @@ __device__ __noinline__ double f4_exact(const int* qa, const float* sa, const ui
     return v;
 }
 
-// 64 columns of the same in fp32, added to v: within the accumulators' own bound (at most 16 blocks,
+// 64 columns of the same (four times the value) in fp32, added to v: within the accumulators' own bound (at most 16 blocks,
 // a few units of 2^-24 of the terms' sum), so that the same err covers it.
 template <int kNv>
 __device__ __forceinline__ float f4_estimate64(const int* qa, const float* sa, uint4 y0, uint4 y1, uint32_t wb, float v) {
@@ -452,6 +452,7 @@ k_f4_pick(PickArgs p) {
     __shared__ int n_list, n_found, n_units, n_valid;
     __shared__ float s_err;
     __shared__ int s_forced;
+    __shared__ uint32_t s_l;
     const double kNegInf = -__longlong_as_double(0x7ff0000000000000ll);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const long long i = (long long)p.row0 + blockIdx.x;
@@ -527,44 +528,64 @@ k_f4_pick(PickArgs p) {
     const bool forced = s_forced != 0;
     // the units are dealt to groups: L is the kp-th largest of the groups' largest keys, by bisection of
     // its 16 bits (0: there are fewer), or a little less, as soon as kp groups have it
-    uint32_t s_key = 0;
-    if constexpr (kT == 1024) {
-        uint32_t top = 0;
-        for (int t = tid; t < nunits; t += kT) {
-            const uint32_t key = tops[t];
-            if (key != kAlways) top = max(top, key);
-        }
-        for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
-            const int c = __syncthreads_count(top >= (s_key | bit));
-            if (c >= kp) s_key |= bit;
-            if (c == kp) break;
-        }
-    } else {
-        // two groups a thread (one: 4,096 x 1,000,000, top 50 looks at an eighth more chunks); every warp
-        // finds L for itself, which costs less than a barrier a bit
-        __shared__ __align__(16) uint16_t group[2 * kT];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            uint32_t top = 0;
-            for (int t = tid + h * kT; t < nunits; t += 2 * kT) {
-                const uint32_t key = tops[t];
-                if (key != kAlways) top = max(top, key);
+    // Fewer chunks than kp bound nothing, and every column would be ranked: then the columns' estimates
+    // are the keys (one row against 1,000, top 50: 19 us, 59 without).
+    const uint16_t* from = tops;
+    int nfrom = nunits;
+    if (p.b.rows < 32 * kp && p.b.rows <= 2048 && !forced) {
+        for (int j = tid; j < p.b.rows; j += kT) {
+            float v = 0.0f;
+            for (int st = 0; st < steps; ++st) {
+                const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(scales_of(j) + (kNv ? st : st >> 1) * kF4Atom));
+                v = f4_estimate64<kNv>(qa + 16 * st, sa + (kNv ? 4 : 2) * st, __ldg(codes_of(j) + 2 * st),
+                                       __ldg(codes_of(j) + 2 * st + 1), !kNv && (st & 1) ? w >> 16 : w, v);
             }
-            group[tid + h * kT] = (uint16_t)top;
+            ulist[j] = j != self && v == v ? (uint16_t)key_of(0.25f * v) : 0;  // (four times the value)
         }
         __syncthreads();
-        constexpr int kW = kT / 32;  // words of two groups a lane
-        uint32_t x[kW];
+        from = ulist;
+        nfrom = p.b.rows;
+    }
+    uint32_t s_key = 0;
+    {
+        constexpr int kGroups = 256;  // with 128: an eighth more chunks to look at for 50 neighbours
+        constexpr int kTops = kT < kGroups ? kGroups : kT;
+        __shared__ __align__(16) uint16_t top[kTops];  // a group: those at its number plus multiples of kGroups
 #pragma unroll
-        for (int e = 0; e < kW; ++e) x[e] = reinterpret_cast<const uint32_t*>(group)[lane + 32 * e];
-        for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
-            const uint32_t want = s_key | bit;
-            int c = 0;
+        for (int h = 0; h < kTops; h += kT) {
+            uint32_t most = 0;
+            for (int t = tid + h; t < nfrom; t += kTops) {
+                const uint32_t key = from[t];
+                if (key != kAlways) most = max(most, key);
+            }
+            top[tid + h] = (uint16_t)most;
+        }
+        __syncthreads();
+        // four warps find L each for itself, which costs less than a barrier a bit; of 32 one does
+        if (kT == 128 || warp == 0) {
+            constexpr int kW = kGroups / 64;  // words of two groups a lane
+            uint32_t x[kW];
 #pragma unroll
-            for (int e = 0; e < kW; ++e) c += ((x[e] & 0xFFFFu) >= want) + (x[e] >= want << 16);
-            c = __reduce_add_sync(0xFFFFFFFFu, c);
-            if (c >= kp) s_key = want;
-            if (c == kp) break;
+            for (int e = 0; e < kW; ++e) {
+                x[e] = reinterpret_cast<const uint32_t*>(top)[lane + 32 * e];
+#pragma unroll
+                for (int h = 1; h < kTops / kGroups; ++h)
+                    x[e] = __vmaxu2(x[e], reinterpret_cast<const uint32_t*>(top)[lane + 32 * e + h * (kGroups / 2)]);
+            }
+            for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
+                const uint32_t want = s_key | bit;
+                int c = 0;
+#pragma unroll
+                for (int e = 0; e < kW; ++e) c += ((x[e] & 0xFFFFu) >= want) + (x[e] >= want << 16);
+                c = __reduce_add_sync(0xFFFFFFFFu, c);
+                if (c >= kp) s_key = want;
+                if (c == kp) break;
+            }
+        }
+        if (kT != 128) {
+            if (tid == 0) s_l = s_key;
+            __syncthreads();
+            s_key = s_l;
         }
     }
     const double err = (double)s_err;
@@ -1021,8 +1042,9 @@ cudaError_t f4_topk(const F4& a, const F4& b, int k, long long self, int* idx, f
         // A warp takes about 25 us for its row (10,000 columns) to 80 (32,000), a block 3 to 5, so
         // the warps' kernel needs an SM nearly full of rows: at 1,200 rows 32.8 against 23.7 us (both
         // kernels, 10,000 columns) and 90 / 47 (32,000), at 2,400 32.8 / 32.7, at 4,000 100 / 108,
-        // at 10,000 62.6 / 89, at 20,000 356 / 458.
-        const int threads = rows <= 2 * sms ? 1024 : few_keys && rows >= 24 * sms ? 32 : 128;
+        // at 10,000 62.6 / 89, at 20,000 356 / 458.  And its groups of 64 columns have to outnumber k:
+        // 10,000 x 1,700, top 50: 355 us against 236; 10,000 x 1,000, top 10: 60 against 87.
+        const int threads = rows <= 2 * sms ? 1024 : few_keys && rows >= 24 * sms && b.rows >= 96 * k ? 32 : 128;
         if (threads == 32) e = b.nv ? launch_pick_warp<1>(q, rows, st) : launch_pick_warp<0>(q, rows, st);
         else if (threads == 128) e = b.nv ? launch_pick<1, 128>(q, rows, st) : launch_pick<0, 128>(q, rows, st);
         else e = b.nv ? launch_pick<1, 1024>(q, rows, st) : launch_pick<0, 1024>(q, rows, st);

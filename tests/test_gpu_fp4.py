@@ -437,3 +437,30 @@ def test_topk_a_warp_a_row(fmt, n, k, top, kind):
         for i in pick:
             wi, wv = ref.topk(ref.values(ca[i:i + 1], sa[i:i + 1], 1.0, fmt), vb, top, int(i) if same else None, fmt)
             assert np.array_equal(idx[i], wi[0]) and np.array_equal(val[i], wv[0]), i
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("m,n", [(2, 33), (3, 1000), (400, 1500), (3800, 700), (5, 2047), (2, 2070), (4, 40)])
+def test_topk_fewer_chunks_than_neighbours(fmt, m, n):
+    """So few rows that 32 times k reach them: the chunks' maxima bound nothing."""
+    import rfx_b200
+    rng = np.random.default_rng(m + n)
+    cb, sb = _parts(rng, n, 72, fmt, spread=2)
+    cb[n // 2: n // 2 + 20] = cb[0]
+    sb[n // 2: n // 2 + 20] = sb[0]
+    sb[7, 0] = 255 if fmt == "mxfp4" else 127
+    which = rng.integers(0, n, m)
+    which[0] = 0
+    ca, sa = cb[which], sb[which]
+    a, b = _matrix(ca, sa, 72, fmt), _matrix(cb, sb, 72, fmt)
+    same = min(m, n)  # these are rows of b, themselves left out
+    pick = np.unique(np.concatenate([[0, same - 1], rng.integers(0, same, 10)]))
+    vb = ref.values(cb, sb, 1.0, fmt)
+    for top in (64, 33):
+        for got, at, va in ((rfx_b200.fp4_topk(a, b, top), None, ref.values(ca, sa, 1.0, fmt)),
+                            (rfx_b200.fp4_topk(b.rows(0, same), b, top, self_offset=0), 0, vb)):
+            rfx_b200.fp4_status()
+            idx, val = (t.cpu().numpy() for t in got)
+            for i in pick:
+                wi, wv = ref.topk(va[i:i + 1], vb, top, None if at is None else int(i), fmt)
+                assert np.array_equal(idx[i], wi[0]) and np.array_equal(val[i], wv[0]), (top, at, i)
