@@ -35,10 +35,10 @@ def _p(a, t):
 
 def reference_tree():
     """The reference source tree: $RFX_REFERENCE, else a directory named ``reference`` beside
-    this repository; None when neither exists."""
+    this repository; None when that holds no sources."""
     cand = os.environ.get("RFX_REFERENCE") or os.path.join(
         os.path.dirname(os.path.dirname(HERE)), "reference")
-    return cand if os.path.isdir(cand) else None
+    return cand if os.path.isdir(os.path.join(cand, "src")) else None
 
 
 def build(ref: bool = False) -> None:
