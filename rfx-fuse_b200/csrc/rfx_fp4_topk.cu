@@ -493,7 +493,7 @@ k_f4_pick(PickArgs p) {
         uint4 x[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            x[e] = t0 + e * kT < nvec ? __ldg(keys + t0 + e * kT) : make_uint4(0, 0, 0, 0);
+            x[e] = t0 + e * kT < nvec ? load_left(keys + t0 + e * kT) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int t = t0 + e * kT;
@@ -512,7 +512,7 @@ k_f4_pick(PickArgs p) {
         float e = 0.0f;
         bool f = false;
         for (int t = lane; t < p.nerrs; t += 32) {
-            const float x = __ldg(p.errs + t);
+            const float x = load_left(p.errs + t);
             f |= x < 0.0f;
             e = fmaxf(e, fabsf(x));
         }
@@ -713,7 +713,7 @@ k_f4_pick(PickArgs p) {
                     const int e = unit & 7;
                     if (tops[unit] >= bar) list[atomicAdd(&n_list, 1)] = (uint32_t)(chunk0 + 4 * kAccs * (e >> 2) + (e & 3));
                 } else {
-                    const uint4 x = __ldg(keys + vec);
+                    const uint4 x = load_left(keys + vec);
                     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
@@ -786,7 +786,7 @@ k_f4_pick_warp(PickArgs p, int rows) {
         uint32_t x[16];  // words of two keys
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const uint4 y = lane + 32 * e < nvec ? __ldg(keys + lane + 32 * e) : make_uint4(0, 0, 0, 0);
+            const uint4 y = lane + 32 * e < nvec ? load_left(keys + lane + 32 * e) : make_uint4(0, 0, 0, 0);
             x[4 * e] = y.x;
             x[4 * e + 1] = y.y;
             x[4 * e + 2] = y.z;
@@ -795,7 +795,7 @@ k_f4_pick_warp(PickArgs p, int rows) {
         float worst = 0.0f;
         bool forced = false;
         for (int t = lane; t < p.nerrs; t += 32) {
-            const float y = __ldg(p.errs + t);
+            const float y = load_left(p.errs + t);
             forced |= y < 0.0f;
             worst = fmaxf(worst, fabsf(y));
         }

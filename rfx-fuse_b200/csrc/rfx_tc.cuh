@@ -145,6 +145,12 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
 // waits for the one before (its memory included) to end.
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// What the kernel before left, after wait_for_previous(): an ordinary load.  Not __ldg, which promises
+// that nobody writes the data while this kernel runs; the compiler may then place it above the wait.
+template <class T>
+__device__ __forceinline__ T load_left(const T* p) {
+    return *p;
+}
 
 // Work by cluster launch control: a running block takes over the index of one that has not started.
 // The 16-byte answer arrives in shared memory at `slot`, completing on `bar`.
