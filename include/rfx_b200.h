@@ -473,7 +473,9 @@ int rfx_fp4_dequantize(const rfx_fp4_matrix* m, int row_begin, int row_end, void
                        long long ld, void* stream);
 /* out <- caller-supplied codes [rows][(cols + 1) / 2] (two a byte, even column low), scale bytes
  * [rows][ceil(cols / block)] (e8m0, or e4m3 whose top bit is ignored) and matrix scale (device,
- * one positive float; NULL = 1), all row-major on the device; and the inverse. */
+ * one float; NULL = 1), all row-major on the device; and the inverse.  A matrix scale that is not
+ * positive and finite is kept as NaN: so are then all values and products, and no row has or is
+ * a neighbour. */
 int rfx_fp4_pack(const uint8_t* codes_dev, const uint8_t* scales_dev, const float* scale_dev,
                  const rfx_fp4_matrix* out, void* stream);
 int rfx_fp4_unpack(const rfx_fp4_matrix* m, uint8_t* codes_dev, uint8_t* scales_dev, void* stream);

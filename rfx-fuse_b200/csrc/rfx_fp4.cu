@@ -328,6 +328,12 @@ k_f4_dequantize(F4 m, int r0, int r1, T* __restrict__ out, long long ld) {
     }
 }
 
+// A caller's matrix scale, NaN unless positive and finite: no order of the products without their
+// scales is that of the products with such a one, and products and values are then NaN as well.
+__device__ __forceinline__ float usable_scale(float g) {
+    return g > 0.0f && g < __int_as_float(0x7f800000) ? g : __int_as_float(0x7fc00000);
+}
+
 // Row-major codes [rows][(cols + 1) / 2] and scales [rows][nblocks] into the layout above.  A
 // block takes 128 rows x up to kQChunk columns, like the quantiser.
 __global__ void __launch_bounds__(kQThreads)
@@ -379,7 +385,7 @@ k_f4_pack(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
     __syncthreads();
     uint32_t* dst = reinterpret_cast<uint32_t*>(m.scales + ((long long)tile * m.natoms + c0 / (m.nv ? 64 : 128)) * kF4Atom);
     for (int i = threadIdx.x; i < atoms * (kF4Atom / 4); i += kQThreads) dst[i] = sf[i];
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) m.gs[0] = g ? *g : 1.0f;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) m.gs[0] = g ? usable_scale(*g) : 1.0f;
     if (bounds) tile_bound(n2, U, nr, m.bounds + tile);
 }
 

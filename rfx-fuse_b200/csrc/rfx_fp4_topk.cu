@@ -432,6 +432,12 @@ __device__ __forceinline__ float f4_estimate64(const int* qa, const float* sa, u
     return v;
 }
 
+// Every product is NaN.
+__device__ __forceinline__ bool nan_scale(const F4& a, const F4& b) {
+    const float x = __ldg(a.gs), y = __ldg(b.gs);
+    return !(x == x && y == y);
+}
+
 // kT threads a row: 128, eight rows an SM, which hide one another's waits for memory and barriers
 // (both kernels at 4,096 x 1,000,000, top 50: 411 us, 435 with 256 threads; 100,000 rows: 128, 150); 1024
 // when there are too few rows to fill the GPU.
@@ -480,6 +486,7 @@ k_f4_pick(PickArgs p) {
     }
     float s0 = 0.0f;
     if (tid < p.a.Kp / (kNv ? 16 : 32)) sa[tid] = s0 = f4_scale_value(kNv, p.a.scales[f4_scale_at(p.a, i, tid)]);
+    if (tid == 0 && nan_scale(p.a, p.b)) s0 = __int_as_float(0x7fc00000);
     wait_for_previous();  // the keys
     if (__syncthreads_or(!(s0 == s0))) {  // a NaN row is nobody's neighbour and has none
         for (int s = tid; s < p.k; s += kT) {
@@ -780,6 +787,7 @@ k_f4_pick_warp(PickArgs p, int rows) {
     }
     float s0 = 0.0f;
     if (lane < p.a.Kp / (kNv ? 16 : 32)) sa[lane] = s0 = f4_scale_value(kNv, p.a.scales[f4_scale_at(p.a, i, lane)]);
+    if (lane == 0 && nan_scale(p.a, p.b)) s0 = __int_as_float(0x7fc00000);
     wait_for_previous();  // the keys
     int n_known = 0, n_found = 0;
     if (!__any_sync(kAll, !(s0 == s0))) {  // a NaN row is nobody's neighbour and has none

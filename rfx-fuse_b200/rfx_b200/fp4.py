@@ -118,7 +118,8 @@ class Fp4Matrix:
         """From codes uint8 [rows, ceil(cols / 2)] (two a byte, even column in the low half),
         scale bytes uint8 [rows, ceil(cols / block)] (e8m0 for "mxfp4", unsigned e4m3 for
         "nvfp4") and the matrix scale: a positive number or one-element float32 tensor on the
-        same device ("nvfp4" only; None: 1)."""
+        same device ("nvfp4" only; None: 1).  A tensor's value is not waited for: where it is not
+        positive and finite, every value of the matrix is NaN."""
         L = _load()
         torch = _torch
         _check_format(format)
