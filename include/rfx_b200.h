@@ -480,8 +480,9 @@ int rfx_fp4_pack(const uint8_t* codes_dev, const uint8_t* scales_dev, const floa
                  const rfx_fp4_matrix* out, void* stream);
 int rfx_fp4_unpack(const rfx_fp4_matrix* m, uint8_t* codes_dev, uint8_t* scales_dev, void* stream);
 /* out_dev[i][j] = a_i . b_j, [a.rows][ld >= b.rows] of `dtype`: block-scaled tensor-core
- * products, fp32 accumulation, then the matrix scales (their product may leave fp32 where the
- * result does not).  a and b share format and cols. */
+ * products, fp32 accumulation, then the matrix scales in fp32 (their product may leave fp32 where
+ * the result does not; scales that are no powers of two round once each), then one rounding to
+ * `dtype`.  a and b share format and cols. */
 int rfx_fp4_product(const rfx_fp4_matrix* a, const rfx_fp4_matrix* b, void* out_dev, int dtype,
                     long long ld, void* stream);
 /* The k <= 64 rows of b with the largest a_i . b_j for every row of a, by exact value

@@ -254,6 +254,18 @@ k_f4_quantize(const T* __restrict__ x, long long ld, F4 m) {
     if (bounds) tile_bound(n2, U, nr, m.bounds + tile);
 }
 
+// x g, rounded once to T.  A 16-bit T from the nearest fp32 would be rounded twice: the fp32 is cut
+// off instead and its last bit set where that lost anything (rounding to odd: Boldo and Melquiond,
+// IEEE Transactions on Computers 57(4), 2008), then the second rounding decides as the only one
+// would.  x has 6 significant bits, so the product is exact in 64.
+template <class T>
+__device__ __forceinline__ T scaled_once(float x, float g) {
+    if (sizeof(T) == 4) return from_f32<T>(x * g);
+    float v = __fmul_rz(x, g);
+    if ((double)v != (double)x * (double)g) v = __uint_as_float(__float_as_uint(v) | 1u);
+    return from_f32<T>(v);
+}
+
 // Values of rows [r0, r1) into out (row r0 first).  A block takes 128 rows x up to kQChunk columns:
 // their codes come into shared memory by 16-byte loads, all in flight at once, their scales decoded
 // beside them.  A thread then writes kV elements at a time: 16 bytes, 4, or one element, as columns
@@ -299,33 +311,38 @@ k_f4_dequantize(F4 m, int r0, int r1, T* __restrict__ out, long long ld) {
     T* o = out + ((long long)tile * kF4Tile - r0 + qa + grp) * ld + c0 + u * kV;
     const long long step = groups * ld;
     const int shift = (u & 1) * 4;
+    auto rows = [&](auto value) {
 #pragma unroll 4
-    for (int q = qa + grp; q < qb; q += groups, o += step) {
-        const float sv = s[q * (kBlocks + 1)];
-        if constexpr (kV >= 4) {
-            uint32_t w;
-            if constexpr (kV == 8) w = *reinterpret_cast<const uint32_t*>(p + q * kRow);
-            else w = *reinterpret_cast<const uint16_t*>(p + q * kRow);
-            float f[kV];
-            e2m1_values<kV>(w, f);
-            T v[kV];
+        for (int q = qa + grp; q < qb; q += groups, o += step) {
+            const float sv = s[q * (kBlocks + 1)];
+            if constexpr (kV >= 4) {
+                uint32_t w;
+                if constexpr (kV == 8) w = *reinterpret_cast<const uint32_t*>(p + q * kRow);
+                else w = *reinterpret_cast<const uint16_t*>(p + q * kRow);
+                float f[kV];
+                e2m1_values<kV>(w, f);
+                T v[kV];
 #pragma unroll
-            for (int i = 0; i < kV; ++i) v[i] = from_f32<T>(f[i] * sv * g);
-            uint4 x;
-            memcpy(&x, v, 16);
-            *reinterpret_cast<uint4*>(o) = x;
-        } else {
-            const uint32_t w = p[q * kRow];
-            if constexpr (kV == 2) {
-                T v[2] = {from_f32<T>(lut[w & 15u] * sv * g), from_f32<T>(lut[w >> 4] * sv * g)};
-                uint32_t x;
-                memcpy(&x, v, 4);
-                *reinterpret_cast<uint32_t*>(o) = x;
+                for (int i = 0; i < kV; ++i) v[i] = value(f[i] * sv);
+                uint4 x;
+                memcpy(&x, v, 16);
+                *reinterpret_cast<uint4*>(o) = x;
             } else {
-                *o = from_f32<T>(lut[w >> shift & 15u] * sv * g);
+                const uint32_t w = p[q * kRow];
+                if constexpr (kV == 2) {
+                    T v[2] = {value(lut[w & 15u] * sv), value(lut[w >> 4] * sv)};
+                    uint32_t x;
+                    memcpy(&x, v, 4);
+                    *reinterpret_cast<uint32_t*>(o) = x;
+                } else {
+                    *o = value(lut[w >> shift & 15u] * sv);
+                }
             }
         }
-    }
+    };
+    // a power of two, as the quantiser's, only shifts (where it does not, the 16-bit result is 0)
+    if (sizeof(T) == 4 || (__float_as_uint(g) & 0x7FFFFFu) == 0) rows([=](float x) { return from_f32<T>(x * g); });
+    else rows([=](float x) { return scaled_once<T>(x, g); });
 }
 
 // A caller's matrix scale, NaN unless positive and finite: no order of the products without their

@@ -238,8 +238,8 @@ def fp4_quantize(x, format="nvfp4"):
 
 
 def fp4_product(a, b, dtype=None, *, out=None):
-    """a b^T [a.rows, b.rows]: fp32 accumulation on the tensor cores, rounded once to ``dtype``
-    (float32 by default, bfloat16 or float16)."""
+    """a b^T [a.rows, b.rows]: fp32 accumulation on the tensor cores, times the matrix scales in
+    fp32, then rounded to ``dtype`` (float32 by default, bfloat16 or float16)."""
     _pair(a, b)
     if dtype is None:
         dtype = _torch.float32 if out is None else out.dtype

@@ -48,3 +48,40 @@ def test_matrix_scale_that_is_not_positive(m, g):
     idx, _ = rfx_b200.fp4_topk(a, good, 7)
     assert (idx >= 0).all()
     rfx_b200.fp4_status()
+
+
+def _round(v, bits, emin):
+    """v (64 bits) to the nearest number of `bits` significant bits, ties to even, with the
+    exponent of the smallest normal number emin."""
+    e = np.maximum(np.frexp(v)[1] - 1, emin)
+    q = np.ldexp(1.0, e - bits + 1)
+    return np.rint(v / q) * q
+
+
+@pytest.mark.parametrize("dtype,bits,emin", [("bfloat16", 8, -126), ("float16", 11, -14), ("float32", 24, -126)])
+def test_dequantize_rounds_once(dtype, bits, emin):
+    """Matrix scales that are no powers of two, chosen so that code x scale x matrix scale lies next to
+    the middle of two numbers of the type: rounding to fp32 on the way would land on it."""
+    import torch
+    codes = np.tile(np.arange(16, dtype=np.uint8), (126, 1))
+    scales = np.arange(1, 127, dtype=np.uint8)[:, None]
+    x = ref.values(codes, scales, 1.0, "nvfp4")  # at most 6 significant bits
+    twice = 0
+    for lo in (1.0, 2.0 ** (emin + 1), 2.0 ** (emin - 3)):
+        # middles of neighbours near lo, one in three above: no multiples of 3
+        q = 2.0 ** (max(np.frexp(lo)[1] - 1, emin) - bits + 1)
+        for i in (0, 1, 2, 4, 5, 9):
+            for base in (3.0, 0.1015625):  # values among x
+                g = np.float32((lo + (i + 0.5) * q) / base)
+                if not 2.0 ** -126 <= g < 2.0 ** 100:
+                    continue
+                v = x * np.float64(g)  # 30 bits: exact
+                want = _round(v, bits, emin)
+                with np.errstate(over="ignore"):
+                    want = np.where(np.abs(want) > float(torch.finfo(getattr(torch, dtype)).max), np.copysign(np.inf, want), want)
+                    twice += int((_round(_round(v, 24, -126), bits, emin) != _round(v, bits, emin)).sum())
+                got = _matrix(codes, scales, 16, "nvfp4", float(g)).dequantize(getattr(torch, dtype))
+                got = got.double().cpu().numpy()
+                bad = np.argwhere(got != want)
+                assert len(bad) == 0, (lo, i, base, len(bad), got[tuple(bad[0])], want[tuple(bad[0])], v[tuple(bad[0])])
+    assert dtype == "float32" or twice > 0  # a second rounding would have been seen
