@@ -345,14 +345,17 @@ int rfx_lowrank4_product(void* ctx, int row_begin, int row_end, float* out_host)
         const F4 m = ctx_matrix(c);
         require(row_begin >= 0 && row_begin <= row_end && row_end <= m.rows, RFX_ERR_ARG, "bad row range");
         require(out_host, RFX_ERR_ARG, "null output");
+        if (row_begin == row_end) return;
         const int R = m.rows;
-        // row blocks of about 256 MB, so that the device scratch stays bounded
-        const int chunk = (int)std::max<long long>(1, ((long long)256 << 20) / ((long long)R * 4));
-        for (int r0 = row_begin; r0 < row_end; r0 += std::min(chunk, row_end - r0)) {
-            const int r1 = r0 + std::min(chunk, row_end - r0);
+        // blocks of whole tiles of rows, so that only the first computes rows that are not asked for:
+        // up to 256 MB of device scratch, or one tile's rows where those take more
+        const int chunk = (int)std::max<long long>(1, ((long long)256 << 20) / ((long long)R * 4 * rfx::kF4Tile)) * rfx::kF4Tile;
+        const int first = row_begin / rfx::kF4Tile * rfx::kF4Tile;
+        float* buf = (float*)c.lr_out_v.get((size_t)std::min(chunk, row_end - first) * R * 4);
+        for (int b0 = first; b0 < row_end; b0 += std::min(chunk, row_end - b0)) {
+            const int r0 = std::max(b0, row_begin), r1 = b0 + std::min(chunk, row_end - b0);
             int skip = 0;
             const F4 a = rows_of(m, r0, r1, &skip);
-            float* buf = (float*)c.lr_out_v.get((size_t)a.rows * R * 4);
             int launches = 0;
             product(a, m, buf, RFX_F32, R, c.st, &launches);
             c.launches += launches;

@@ -85,3 +85,32 @@ def test_dequantize_rounds_once(dtype, bits, emin):
                 bad = np.argwhere(got != want)
                 assert len(bad) == 0, (lo, i, base, len(bad), got[tuple(bad[0])], want[tuple(bad[0])], v[tuple(bad[0])])
     assert dtype == "float32" or twice > 0  # a second rounding would have been seen
+
+
+def test_product_rows_in_several_blocks():
+    """get_lowrank_product over more rows than one block holds: the scratch stays within 256 MB (128
+    rows, where those take more), whatever the first row, and the rows are the same."""
+    import torch
+    import rfx_b200
+    from _helpers import synth
+    n = 300000  # a block of 256 MB: 223 rows
+    X, y = synth("class", n, 6, 3)
+    est = rfx_b200.RandomForestClassifier(nsample=n, ntree=2, mdim=6, mtry=2, compute_proximity=True, compute_importance=False,
+                                          use_qlora=True, quant_mode="nvfp4", rank=8, show_progress=False)
+    est.fit(X, y)
+    A = est.get_lowrank_factors()[0]
+    rfx_b200.empty_cache()
+    torch.cuda.synchronize()
+    before = torch.cuda.mem_get_info()[0]
+    P = est.get_lowrank_product(100, 400)
+    used = before - torch.cuda.mem_get_info()[0]
+    assert P.shape == (300, n)
+    for r0, r1 in ((100, 101), (127, 129), (255, 390)):
+        assert np.array_equal(est.get_lowrank_product(r0, r1), P[r0 - 100:r1 - 100])
+    for r0 in range(100, 400, 50):
+        a = A[r0:r0 + 50]
+        want = a @ A.T
+        # 8 fp32 additions of exact terms, one rounding
+        tol = 8 * 2.0 ** -23 * (np.abs(a) @ np.abs(A).T) + 2.0 ** -24 * np.abs(want)
+        assert (np.abs(P[r0 - 100:r0 - 50] - want) <= tol).all()
+    assert used <= (256 + 8) << 20, used
