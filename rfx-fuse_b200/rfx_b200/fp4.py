@@ -12,7 +12,8 @@ include/rfx_b200.h states the formats and the operators exactly.
 Calls run on the current torch stream of the tensors' device, allocate from torch's caching
 allocator, do not synchronise, and can be captured into a CUDA graph once they have run before.
 Tensors made on another stream need the caller's event or ``wait_stream``, as with torch's own
-operators.  There is no gradient: results never require one.
+operators, and a matrix that is dropped while another stream than its own still reads it needs
+``record_stream``, as a tensor does.  There is no gradient: results never require one.
 """
 from __future__ import annotations
 
@@ -179,6 +180,11 @@ class Fp4Matrix:
                            c.scales_dev + begin // 128 * self._tile_bytes, c.scale_dev,
                            c.bounds_dev + begin // 128 * 4))
         return m
+
+    def record_stream(self, stream):
+        """Tell the allocator that ``stream`` uses this matrix's memory (views share it): it is not
+        given out again before that stream's work so far is done."""
+        self._keep.record_stream(stream)
 
     def dequantize(self, dtype=None, *, out=None):
         """The values [rows, cols]; exact in float32 and bfloat16 for a quantised matrix."""

@@ -114,3 +114,31 @@ def test_product_rows_in_several_blocks():
         tol = 8 * 2.0 ** -23 * (np.abs(a) @ np.abs(A).T) + 2.0 ** -24 * np.abs(want)
         assert (np.abs(P[r0 - 100:r0 - 50] - want) <= tol).all()
     assert used <= (256 + 8) << 20, used
+
+
+def test_memory_used_on_another_stream():
+    """A matrix made on one stream, used on another and dropped: after record_stream its memory is not
+    given out again before the other stream is done."""
+    import torch
+    import rfx_b200
+    made, used = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(made):
+        x = torch.randn(3000, 64, device="cuda")
+        m = rfx_b200.fp4_quantize(x)
+        want = m.dequantize()
+        torch.full((1,), 255, dtype=torch.uint8, device="cuda")  # loading a kernel waits for the device
+    used.wait_stream(made)
+    torch.cuda.synchronize()
+    where, size = m._keep.data_ptr(), m._keep.numel()
+    with torch.cuda.stream(used):
+        torch.cuda._sleep(200_000_000)  # about a tenth of a second
+        view = m.rows(0, 3000)
+        got = view.dequantize()
+        view.record_stream(used)
+    del m, view
+    with torch.cuda.stream(made):
+        new = [torch.full((size,), 255, dtype=torch.uint8, device="cuda") for _ in range(3)]
+    assert not used.query()  # the other stream was still at work
+    assert where not in [t.data_ptr() for t in new]
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
