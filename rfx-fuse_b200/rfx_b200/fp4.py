@@ -212,6 +212,8 @@ def _out(out, shape, dtype, device):
         raise ValueError("out must not require a gradient or be a negated view")
     if out.shape[1] > 1 and out.stride(1) != 1 or out.shape[0] > 1 and out.stride(0) < out.shape[1]:
         raise ValueError("out must have unit stride along its rows and rows that do not overlap")
+    if not out.is_inference():  # a graph that saved it must not take it for unchanged
+        _torch.autograd.graph.increment_version(out)
     return out
 
 
