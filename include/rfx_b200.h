@@ -22,7 +22,7 @@
 extern "C" {
 #endif
 
-#define RFX_ABI_VERSION 6
+#define RFX_ABI_VERSION 7
 
 enum {
     RFX_OK = 0,
@@ -494,9 +494,14 @@ int rfx_fp4_product(const rfx_fp4_matrix* a, const rfx_fp4_matrix* b, void* out_
 int rfx_fp4_topk_workspace(const rfx_fp4_matrix* a, const rfx_fp4_matrix* b, int k, long long* bytes);
 int rfx_fp4_topk(const rfx_fp4_matrix* a, const rfx_fp4_matrix* b, int k, long long self, int* idx_dev,
                  float* val_dev, void* ws_dev, long long ws_bytes, void* stream);
-/* Waits for the current device; RFX_ERR_DEVICE when a product or top-k kernel has reported a
- * pipeline wait that timed out since the last call (its outputs are then incomplete). */
+/* Waits for the current device; RFX_ERR_DEVICE when a kernel of rfx_fp4_product or rfx_fp4_topk has
+ * reported a pipeline wait that timed out since the last call (its outputs are then incomplete).
+ * One word a device for all streams, read and cleared in one step; calls with a context report
+ * their own and leave it alone. */
 int rfx_fp4_status(void);
+/* The current device's word: 0, or the code of such a wait.  For reading in stream order (a copy, a
+ * node of a graph) without waiting for the device; rfx_fp4_status clears it. */
+int rfx_fp4_status_word(int** word_dev);
 
 /* ---- Low-rank proximity in 4 bits (quant_mode "mxfp4" / "nvfp4") ------------------------
  * rfx_lowrank_pack4 quantises the float factors of the last rfx_lowrank_build to `format`

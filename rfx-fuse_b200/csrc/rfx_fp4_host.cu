@@ -7,13 +7,6 @@
 #include "rfx_fp4.h"
 #include "rfx_tma_host.h"
 
-namespace {
-
-// Set by a kernel whose pipeline wait timed out; read and cleared by rfx_fp4_status.
-__device__ int g_f4_err[4];
-
-}  // namespace
-
 namespace rfx {
 
 bool f4_map(CUtensorMap* tm, const F4& m, int box_rows, int box_bytes) {
@@ -36,6 +29,13 @@ namespace rfxh {
 namespace {
 
 using rfx::F4;
+
+// [0] set by a kernel of the calls without a context whose pipeline wait timed out, taken by
+// rfx_fp4_status; [1] what that took.  Contexts have words of their own.
+__device__ int g_f4_err[4];
+
+// Reads and clears in one step: a code that is set meanwhile is in this answer or the next.
+__global__ void k_f4_take_err(int* err) { err[1] = atomicExch(err, 0); }
 
 constexpr int kMaxDevices = 64;
 constexpr int kMaxCols = 65535 * 256;  // a grid's second axis of 256 columns a block
@@ -102,9 +102,8 @@ void check_launch(cudaError_t e, const char* what) {
     if (e != cudaSuccess) throw RfxError(RFX_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
 }
 
-void product(const F4& a, const F4& b, void* out, int dtype, long long ld, cudaStream_t st, int* launches) {
-    const DeviceInfo d = device_info();
-    check_launch(rfx::f4_product(a, b, out, dtype, ld, d.err, d.sms, st, launches), "rfx_fp4_product");
+void product(const F4& a, const F4& b, void* out, int dtype, long long ld, int* err, cudaStream_t st, int* launches) {
+    check_launch(rfx::f4_product(a, b, out, dtype, ld, err, device_info().sms, st, launches), "rfx_fp4_product");
 }
 
 long long topk_bytes(const F4& a, const F4& b, int k) { return rfx::f4_topk_workspace(a, b, k, device_info().sms); }
@@ -115,21 +114,25 @@ void check_topk(const F4& a, const F4& b, int k) {
     require(a.Kp <= rfx::kF4TopkK, RFX_ERR_UNSUPPORTED, "top-k needs at most 256 columns");
 }
 
-void topk(const F4& a, const F4& b, int k, long long self, int* idx, float* val, void* ws, cudaStream_t st,
-          int* launches) {
-    const DeviceInfo d = device_info();
-    check_launch(rfx::f4_topk(a, b, k, self, idx, val, ws, d.err, d.sms, st, launches), "rfx_fp4_topk");
+void topk(const F4& a, const F4& b, int k, long long self, int* idx, float* val, void* ws, int* err,
+          cudaStream_t st, int* launches) {
+    check_launch(rfx::f4_topk(a, b, k, self, idx, val, ws, err, device_info().sms, st, launches), "rfx_fp4_topk");
 }
 
-// Reads and clears the device's error flag (the stream's work is done).
-void raise_if_timed_out(cudaStream_t st) {
-    const DeviceInfo d = device_info();
+// Waits for the stream and throws if *err says that a wait of its kernels timed out.
+void raise_if_timed_out(const int* err, cudaStream_t st) {
     int h = 0;
-    RFX_CUDA(cudaMemcpyAsync(&h, d.err, 4, cudaMemcpyDeviceToHost, st));
+    RFX_CUDA(cudaMemcpyAsync(&h, err, 4, cudaMemcpyDeviceToHost, st));
     RFX_CUDA(cudaStreamSynchronize(st));
-    if (h == 0) return;
-    RFX_CUDA(cudaMemsetAsync(d.err, 0, 4, st));
-    throw RfxError(RFX_ERR_DEVICE, "4-bit product kernel: a pipeline wait timed out (code " + std::to_string(h) + ")");
+    if (h != 0)
+        throw RfxError(RFX_ERR_DEVICE, "4-bit product kernel: a pipeline wait timed out (code " + std::to_string(h) + ")");
+}
+
+// A context's error word, cleared for a call.
+int* ctx_err(Ctx& c) {
+    int* err = (int*)c.lr_err.get(16);
+    RFX_CUDA(cudaMemsetAsync(err, 0, 16, c.st));
+    return err;
 }
 
 // The low-rank factors of a context in 4 bits.
@@ -234,7 +237,7 @@ int rfx_fp4_product(const rfx_fp4_matrix* a_, const rfx_fp4_matrix* b_, void* ou
         check_elements(out_dev, dtype, "out");
         require(((long long)a.tiles() + 1) * b.tiles() < (1ll << 31), RFX_ERR_UNSUPPORTED, "product too large");
         int launches = 0;
-        product(a, b, out_dev, dtype, ld, static_cast<cudaStream_t>(stream), &launches);
+        product(a, b, out_dev, dtype, ld, device_info().err, static_cast<cudaStream_t>(stream), &launches);
     });
 }
 
@@ -260,14 +263,26 @@ int rfx_fp4_topk(const rfx_fp4_matrix* a_, const rfx_fp4_matrix* b_, int k, long
         require(ws_bytes >= need && (need == 0 || (ws_dev && aligned(ws_dev, 16))), RFX_ERR_ARG,
                 "the workspace is smaller than rfx_fp4_topk_workspace, null or unaligned");
         int launches = 0;
-        topk(a, b, k, self, idx_dev, val_dev, ws_dev, static_cast<cudaStream_t>(stream), &launches);
+        topk(a, b, k, self, idx_dev, val_dev, ws_dev, device_info().err, static_cast<cudaStream_t>(stream), &launches);
     });
 }
 
 int rfx_fp4_status(void) {
     return guarded([&] {
+        static std::mutex mu;  // of what k_f4_take_err leaves
+        std::lock_guard<std::mutex> lock(mu);
+        int* err = device_info().err;
         RFX_CUDA(cudaDeviceSynchronize());
-        raise_if_timed_out(nullptr);
+        k_f4_take_err<<<1, 1>>>(err);
+        check_launch(cudaGetLastError(), "rfx_fp4_status");
+        raise_if_timed_out(err + 1, nullptr);
+    });
+}
+
+int rfx_fp4_status_word(int** word_dev) {
+    return guarded([&] {
+        require(word_dev != nullptr, RFX_ERR_ARG, "null output");
+        *word_dev = device_info().err;
     });
 }
 
@@ -329,13 +344,14 @@ int rfx_lowrank4_topk(void* ctx, int k, int row_begin, int row_end, int* idx_hos
         int* oi = (int*)c.lr_out_i.get((size_t)a.rows * k * 4);
         float* ov = (float*)c.lr_out_v.get((size_t)a.rows * k * 4);
         void* ws = c.lr_part.get((size_t)topk_bytes(a, m, k));
+        int* err = ctx_err(c);
         int launches = 0;
-        topk(a, m, k, row_begin - skip, oi, ov, ws, c.st, &launches);
+        topk(a, m, k, row_begin - skip, oi, ov, ws, err, c.st, &launches);
         c.launches += launches;
         const size_t n = (size_t)(row_end - row_begin) * k * 4;
         RFX_CUDA(cudaMemcpyAsync(idx_host, oi + (size_t)skip * k, n, cudaMemcpyDeviceToHost, c.st));
         RFX_CUDA(cudaMemcpyAsync(val_host, ov + (size_t)skip * k, n, cudaMemcpyDeviceToHost, c.st));
-        raise_if_timed_out(c.st);
+        raise_if_timed_out(err, c.st);
     });
 }
 
@@ -351,17 +367,18 @@ int rfx_lowrank4_product(void* ctx, int row_begin, int row_end, float* out_host)
         // up to 256 MB of device scratch, or one tile's rows where those take more
         const int chunk = (int)std::max<long long>(1, ((long long)256 << 20) / ((long long)R * 4 * rfx::kF4Tile)) * rfx::kF4Tile;
         const int first = row_begin / rfx::kF4Tile * rfx::kF4Tile;
+        int* err = ctx_err(c);
         float* buf = (float*)c.lr_out_v.get((size_t)std::min(chunk, row_end - first) * R * 4);
         for (int b0 = first; b0 < row_end; b0 += std::min(chunk, row_end - b0)) {
             const int r0 = std::max(b0, row_begin), r1 = b0 + std::min(chunk, row_end - b0);
             int skip = 0;
             const F4 a = rows_of(m, r0, r1, &skip);
             int launches = 0;
-            product(a, m, buf, RFX_F32, R, c.st, &launches);
+            product(a, m, buf, RFX_F32, R, err, c.st, &launches);
             c.launches += launches;
             RFX_CUDA(cudaMemcpyAsync(out_host + (size_t)(r0 - row_begin) * R, buf + (size_t)skip * R,
                                      (size_t)(r1 - r0) * R * 4, cudaMemcpyDeviceToHost, c.st));
-            raise_if_timed_out(c.st);
+            raise_if_timed_out(err, c.st);
         }
     });
 }

@@ -90,6 +90,7 @@ SYMBOLS = (
     "rfx_rank_scores_desc", "rfx_predict_outlier_scores",
     "rfx_fp4_sizes", "rfx_fp4_quantize", "rfx_fp4_dequantize", "rfx_fp4_pack", "rfx_fp4_unpack",
     "rfx_fp4_product", "rfx_fp4_topk_workspace", "rfx_fp4_topk", "rfx_fp4_status",
+    "rfx_fp4_status_word",
     "rfx_lowrank_pack4", "rfx_lowrank4_factors", "rfx_lowrank4_topk", "rfx_lowrank4_product",
 )
 
@@ -172,6 +173,7 @@ def load_library(path: str = LIB_PATH):
     L.rfx_fp4_product.argtypes = [pm, pm, vp, C.c_int, ll, vp]
     L.rfx_fp4_topk_workspace.argtypes = [pm, pm, C.c_int, C.POINTER(ll)]
     L.rfx_fp4_topk.argtypes = [pm, pm, C.c_int, ll, vp, vp, vp, ll, vp]
+    L.rfx_fp4_status_word.argtypes = [C.POINTER(vp)]
     L.rfx_load_forest.argtypes = [vp, C.POINTER(Forest)]
     L.rfx_impute_round.argtypes = [vp, _pf, _pu8, _pu8, C.c_int, C.c_int, _pi, C.c_int, _pf]
     L.rfx_impute_round_ex.argtypes = [vp, _pf, _pu8, _pu8, C.c_int, C.c_int, _pi, C.c_int,
@@ -205,7 +207,8 @@ def load_library(path: str = LIB_PATH):
                  "rfx_leaf_outlier_scores", "rfx_rank_scores_desc",
                  "rfx_predict_outlier_scores", "rfx_fp4_sizes", "rfx_fp4_quantize",
                  "rfx_fp4_dequantize", "rfx_fp4_pack", "rfx_fp4_unpack", "rfx_fp4_product",
-                 "rfx_fp4_topk_workspace", "rfx_fp4_topk", "rfx_fp4_status", "rfx_lowrank_pack4",
+                 "rfx_fp4_topk_workspace", "rfx_fp4_topk", "rfx_fp4_status",
+                 "rfx_fp4_status_word", "rfx_lowrank_pack4",
                  "rfx_lowrank4_factors", "rfx_lowrank4_topk", "rfx_lowrank4_product"):
         getattr(L, name).restype = C.c_int
     _LIB = L

@@ -290,8 +290,8 @@ def _workspace(a, b, k, need, _stream):
 
 
 def fp4_status(device=None):
-    """Wait for the device and raise RfxError if a 4-bit product or top-k kernel on it reported a
-    pipeline wait that timed out since the last call."""
+    """Wait for the device and raise RfxError if a kernel of fp4_product or fp4_topk on it, on any
+    stream, reported a pipeline wait that timed out since the last call (its outputs are incomplete)."""
     _load()
     d = _torch.device("cuda" if device is None else (("cuda:%d" % device) if isinstance(device, int) else device))
     if d.index is None:

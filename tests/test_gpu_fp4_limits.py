@@ -142,3 +142,32 @@ def test_memory_used_on_another_stream():
     assert where not in [t.data_ptr() for t in new]
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+def test_errors_reach_their_own_callers():
+    """The device's status word belongs to the calls without a context: an error in it is neither
+    raised nor erased by an estimator's calls, and rfx_fp4_status reports it once."""
+    import ctypes as C
+    import torch
+    import rfx_b200
+    from rfx_b200.shard import _DeviceInts
+    from _helpers import synth
+    X, y = synth("class", 500, 6, 3)
+    est = rfx_b200.RandomForestClassifier(nsample=500, ntree=4, mdim=6, mtry=2, compute_proximity=True, compute_importance=False,
+                                          use_qlora=True, quant_mode="mxfp4", rank=8, show_progress=False)
+    est.fit(X, y)
+    first = (*est.get_lowrank_topk(5), est.get_lowrank_product(3, 9))
+    at = C.c_void_p()
+    assert rfx_b200.load_library().rfx_fp4_status_word(C.byref(at)) == 0
+    word = torch.as_tensor(_DeviceInts(at.value, 1), device="cuda")
+    rfx_b200.fp4_status()
+    assert int(word) == 0
+    word.fill_(5)  # as a kernel on another stream would
+    torch.cuda.synchronize()
+    again = (*est.get_lowrank_topk(5), est.get_lowrank_product(3, 9))
+    assert all(np.array_equal(s, t) for s, t in zip(first, again))
+    assert int(word) == 5
+    with pytest.raises(rfx_b200.RfxError, match="code 5"):
+        rfx_b200.fp4_status()
+    rfx_b200.fp4_status()
+    assert int(word) == 0
