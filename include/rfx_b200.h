@@ -438,6 +438,11 @@ int rfx_prox_apply(void* ctx, const float* X_dev, int ncols, const int* nout_dev
  *               below 2^-126, 1 for zeros), block scale = e4m3(largest magnitude / (6 g)).
  * Codes are value / scale rounded to the nearest, ties to the even code, at most 6.  A block
  * with an infinity or NaN gets a NaN scale (its values read back as NaN); g ignores it.
+ * RFX_FP4_MX's scale never saturates a value; the usual choice for this format, the largest power
+ * of two up to a quarter of the largest magnitude, cuts what lies between 6 and 8 scales to 6.
+ * Floats hold what the codes stand for exactly, but at two ends: the code next to a magnitude from
+ * 2.9e38 on can stand for 2^128 or more, which reads back as infinity, and RFX_FP4_NV values below
+ * 2^-128 can have more bits than bf16 has there.
  *
  * These functions need no context: device pointers, the caller's current device and stream
  * (NULL = the legacy default stream).  They enqueue and return, allocate nothing, and can be
@@ -468,7 +473,7 @@ int rfx_fp4_sizes(int format, int rows, int cols, rfx_fp4_layout* out);
 int rfx_fp4_quantize(const void* x_dev, int dtype, long long row_stride, const rfx_fp4_matrix* out,
                      void* stream);
 /* Values of rows [row_begin, row_end), rounded once to `dtype` (RFX_F32 and RFX_BF16 hold what
- * rfx_fp4_quantize made exactly): out_dev [rows][ld >= cols]. */
+ * rfx_fp4_quantize made exactly, but at the two ends above): out_dev [rows][ld >= cols]. */
 int rfx_fp4_dequantize(const rfx_fp4_matrix* m, int row_begin, int row_end, void* out_dev, int dtype,
                        long long ld, void* stream);
 /* out <- caller-supplied codes [rows][(cols + 1) / 2] (two a byte, even column low), scale bytes

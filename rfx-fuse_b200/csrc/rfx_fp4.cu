@@ -5,7 +5,7 @@
 // value saturates.  nvfp4: the matrix scale g is the smallest power of two with max |x| <=
 // 6 * 448 g (not below 2^-126; 1 for a matrix of zeros), and a block's scale is e4m3(max |x| /
 // (6 g)).  With g a power of two, scale times code has 6 significant bits: values come back
-// exactly in fp32 and bf16, and the 24-bit input's quotients decide every rounding exactly as
+// exactly in fp32 and bf16 (but where they reach 2^128, or lie below 2^-128), and the 24-bit input's quotients decide every rounding exactly as
 // real arithmetic does (max |x| / 6 and x / scale, rounded once to fp32, are never a false tie:
 // the divisors have at most 4 bits).  Codes round to the nearest, ties to the even code.
 // A block that holds an infinity or NaN gets a NaN scale; g ignores such values.

@@ -187,7 +187,9 @@ class Fp4Matrix:
         self._keep.record_stream(stream)
 
     def dequantize(self, dtype=None, *, out=None):
-        """The values [rows, cols]; exact in float32 and bfloat16 for a quantised matrix."""
+        """The values [rows, cols], rounded once to ``dtype``: exact in float32 and bfloat16 for a
+        quantised matrix (magnitudes from 2.9e38 on can read back as infinite; bfloat16 rounds some
+        below 2^-128)."""
         if dtype is None:
             dtype = _torch.float32 if out is None else out.dtype
         code = _dtype_code(dtype)

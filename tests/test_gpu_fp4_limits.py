@@ -171,3 +171,37 @@ def test_errors_reach_their_own_callers():
         rfx_b200.fp4_status()
     rfx_b200.fp4_status()
     assert int(word) == 0
+
+
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+def test_values_at_the_ends_of_the_range(fmt):
+    """Next to the largest float the nearest code can stand for 2^128 or more, and nvfp4's smallest
+    values have more bits than bf16 has there: each type gets the value, rounded once."""
+    import torch
+    import rfx_b200
+    f = np.finfo(np.float32)
+    tops = [2.8e38, 2.92e38, 2.93e38, 3.5 * 2.0 ** 126, 3.0e38, 2016 * 2.0 ** 117, 3.36e38, float(f.max)]
+    for top in tops:
+        x = np.zeros((3, 64), np.float32)
+        x[0, ::3], x[1, 40:] = np.float32(top), -np.float32(top) * np.float32(0.87)
+        x[2] = 1.0
+        codes, scales, g = ref.quantize(x, fmt)
+        v = ref.values(codes, scales, g, fmt)
+        m = rfx_b200.fp4_quantize(torch.from_numpy(x).cuda(), format=fmt)
+        assert np.array_equal(m.parts()[1].cpu().numpy(), scales)
+        for dtype in (torch.float32, torch.bfloat16):
+            got = m.dequantize(dtype).double().cpu().numpy()
+            want = np.where(np.abs(v) >= 2.0 ** 128, np.copysign(np.inf, v), v)
+            assert np.array_equal(got, want), (top, dtype)
+            assert np.isfinite(got[np.abs(x) < 2.9e38]).all()
+    rng = np.random.default_rng(5)
+    for top in (2.0 ** -117, 2.0 ** -120, 2.0 ** -126, 2.0 ** -130):
+        x = (rng.uniform(-top, top, (40, 64)) * 2.0 ** -rng.integers(0, 16, (40, 1)).astype(np.float64)).astype(np.float32)
+        codes, scales, g = ref.quantize(x, fmt)
+        v = ref.values(codes, scales, g, fmt)
+        m = rfx_b200.fp4_quantize(torch.from_numpy(x).cuda(), format=fmt)
+        assert np.array_equal(m.dequantize().double().cpu().numpy(), v)
+        half = m.dequantize(torch.bfloat16).double().cpu().numpy()
+        assert np.array_equal(half, _round(v, 8, -126))
+        held = np.abs(v) >= 2.0 ** -128 if fmt == "nvfp4" else np.ones_like(v, bool)
+        assert np.array_equal(half[held], v[held])
