@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import enum
 import math
+import warnings
 
 import numpy as np
 
@@ -290,10 +291,13 @@ class _Forest:
 
     def save(self, filepath):
         """Write the model as the reference's RFX0 v1 file (RandomForest::save,
-        src/rf_random_forest.cpp:6037-6140); RFXFuse.load() reads it."""
+        src/rf_random_forest.cpp:6037-6140); RFXFuse.load() reads it.  The file holds no low-rank
+        factors, and names a 4-bit quant_mode as "nf4", the format's only 4-bit code (a warning)."""
         if not self._fitted:
             raise RuntimeError("Model must be fitted before saving")
         from . import model_io
+        if self._lowrank_rank() and self._lowrank4():
+            warnings.warn(f"the model file has no code for quant_mode '{self._lowrank4()}': it says 'nf4'", stacklevel=2)
         model_io.write(str(filepath), model_io.from_estimator(self))
 
     # ---- reference getters

@@ -22,3 +22,26 @@ def test_written_outputs_are_seen_by_autograd():
     assert buf._version > before
     with pytest.raises(ValueError, match="out must"):
         fp4._out(buf, (4, 3), torch.float32, cpu)
+
+
+@pytest.mark.parametrize("mode,told", [("nvfp4", True), ("mxfp4", True), ("int8", False)])
+def test_saving_tells_what_the_file_cannot_say(mode, told, monkeypatch, tmp_path):
+    """The model file's only 4-bit code is nf4's: a 4-bit quant_mode is written as that, with a warning."""
+    import warnings
+    import rfx_b200
+    from rfx_b200 import model_io
+    written = []
+    monkeypatch.setattr(model_io, "from_estimator", lambda est: {"of": est})
+    monkeypatch.setattr(model_io, "write", lambda path, m: written.append((path, m["of"])))
+    est = rfx_b200.RandomForestClassifier(quant_mode=mode, compute_proximity=True, use_qlora=True, rank=8)
+    est._fitted = True
+    with warnings.catch_warnings(record=True) as seen:
+        warnings.simplefilter("always")
+        est.save(tmp_path / "m.rfx")
+    assert [w for w in seen if "nf4" in str(w.message) and mode in str(w.message)] if told else not seen
+    assert written == [(str(tmp_path / "m.rfx"), est)]
+    plain = rfx_b200.RandomForestClassifier(quant_mode=mode)  # no low-rank factors: nothing is lost
+    plain._fitted = True
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        plain.save(tmp_path / "m.rfx")
