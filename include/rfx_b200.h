@@ -511,7 +511,9 @@ int rfx_fp4_status_word(int** word_dev);
 /* ---- Low-rank proximity in 4 bits (quant_mode "mxfp4" / "nvfp4") ------------------------
  * rfx_lowrank_pack4 quantises the float factors of the last rfx_lowrank_build to `format`
  * (beside the int8 factors); the others are rfx_lowrank_factors / _topk / _product on them:
- * A_host [R][rank]; idx_host / val_host [rows][k]; out_host [rows][R]. */
+ * A_host [R][rank]; idx_host / val_host [rows][k]; out_host [rows][R].  Rows are computed from the
+ * multiple of 128 before row_begin on; the product's device scratch is 256 MB, or 128 rows where
+ * those take more. */
 int rfx_lowrank_pack4(void* ctx, int format);
 int rfx_lowrank4_factors(void* ctx, float* A_host, int* rank_out, int* rows_out);
 int rfx_lowrank4_topk(void* ctx, int k, int row_begin, int row_end, int* idx_host, float* val_host);

@@ -143,7 +143,7 @@ k_f4_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CU
             if (!*abort) atomicExch(p.err, 1);
             *abort = 1;
         }
-        // drain this warp's answer and copies still in flight (after next_tile the answer has been read)
+        // drain this warp's answer and copies still in flight (after next_unit the answer has been read)
         if (!ok && asked) mbar_wait<false>(sfull(sched.slot), sched.parity, nullptr);
         for (int i = step > p.nstage ? step - p.nstage : 0; i < step; ++i)
             mbar_wait<false>(full(i % p.nstage), (uint32_t)(i / p.nstage) & 1u, nullptr);

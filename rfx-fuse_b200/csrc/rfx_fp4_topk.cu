@@ -23,8 +23,12 @@
 // What the first kernel leaves is 2 bytes for 32 pairs.  Rows are taken in batches of 256 MB of keys
 // (4,096 x 1,000,000 in one; when that took 441 us, batches of 120 MB took 490: each ends with idle SMs).
 // k_f4_keys: 300 cycles a tile of 128 x 128, of which the ALU's 128 for maxima (a 3-input maximum
-// takes two issue slots) and 90 for keys and bookkeeping; k_f4_pick: half the issue slots, latency
-// of its barriers and loads between them.  Times of both at 4,096 x 1,000,000: 301 and 131 us.
+// takes two issue slots) and 90 for keys and bookkeeping; k_f4_pick: two thirds of the issue slots,
+// latency of its barriers and loads between them.  Alone and cold at 4,096 x 1,000,000 they take 305
+// and 141 us, together 417.
+// err is one number for a batch, from its largest bound of a tile of a times its largest of a tile of b:
+// rows of very different norms keep the answer and lose the filter (one row of b of 10 times the
+// others' norm: 421 us; of 100 times: 38 ms; of 1,000: 231 ms).
 #include <algorithm>
 
 #include "rfx_fp4_mma.cuh"
@@ -441,8 +445,9 @@ __device__ __forceinline__ bool nan_scale(const F4& a, const F4& b) {
 }
 
 // kT threads a row: 128, eight rows an SM, which hide one another's waits for memory and barriers
-// (both kernels at 4,096 x 1,000,000, top 50: 411 us, 435 with 256 threads; 100,000 rows: 128, 150); 1024
-// when there are too few rows to fill the GPU.
+// (both kernels at 4,096 x 1,000,000, top 50: 417 us, 439 with 256 threads; 100,000 rows: 131, 150); 1024
+// when there are too few rows to fill the GPU.  128 threads are held to 64 registers and spill 84 bytes
+// (nvfp4) or 60 (mxfp4).
 template <int kNv, int kT>
 __global__ void __launch_bounds__(kT, kT == 1024 ? 1 : 1024 / kT)
 k_f4_pick(PickArgs p) {
@@ -747,9 +752,9 @@ k_f4_pick(PickArgs p) {
 }
 
 // The same for rows with few keys, a warp a row: the keys stay in registers, nothing waits for a
-// barrier, and an SM works on 32 rows (10,000 x 10,000, top 10: 52 us, 81 with a block of 128 threads a
-// row; it issues 0.84 instructions a cycle and scheduler, 4,200 a row, half of them estimates).  A group
-// is a word of two keys.
+// barrier, and an SM works on 32 rows (10,000 x 10,000, top 10, both kernels: 67 us, 105 with a block of
+// 128 threads a row; alone and cold it takes 60, at 0.83 instructions a cycle and scheduler, 4,800 a row,
+// half of them estimates).  A group is a word of two keys.
 constexpr int kWFound = 128;  // columns waiting to be ranked: 32 more always fit beside the best 64
 
 template <int kNv>
@@ -1049,11 +1054,12 @@ cudaError_t f4_topk(const F4& a, const F4& b, int k, long long self, int* idx, f
         q.row0 = (int)r0;
         q.nerrs = grid;
         const bool few_keys = plan.nspan * kSpanKeys <= kWarpKeys;
-        // A warp takes about 25 us for its row (10,000 columns) to 80 (32,000), a block 3 to 5, so
-        // the warps' kernel needs an SM nearly full of rows: at 1,200 rows 32.8 against 23.7 us (both
-        // kernels, 10,000 columns) and 90 / 47 (32,000), at 2,400 32.8 / 32.7, at 4,000 100 / 108,
-        // at 10,000 62.6 / 89, at 20,000 356 / 458.  And its groups of 64 columns have to outnumber k:
-        // 10,000 x 1,700, top 50: 355 us against 236; 10,000 x 1,000, top 10: 60 against 87.
+        // A warp is slow for one row, so the warps' kernel needs an SM nearly full of rows.  Both kernels,
+        // a warp a row against 128 threads (mxfp4, rank 48, top 10): 1,200 x 10,000 33.8 / 25.6 us, 2,400
+        // 35.6 / 35.8, 4,000 37.9 / 50.2, 10,000 66.6 / 105; 1,200 x 32,000 39.7 / 31.6, 4,000 48.1 / 60.4;
+        // 20,000 x 20,000 132 / 212.  And its groups of 64 columns have to outnumber k: 10,000 x 1,700,
+        // top 50 369 / 241; 10,000 x 1,000, top 10 60.4 / 91.1.  Few rows, 128 against 1,024 threads (1,000,000
+        // x 64, top 50): one 37.9 / 29.5 us, 148 63.5 / 39.9, 296 74.5 / 62.3, 592 93.2 / 103.
         const int threads = rows <= 2 * sms ? 1024 : few_keys && rows >= 24 * sms && b.rows >= 96 * k ? 32 : 128;
         if (threads == 32) e = b.nv ? launch_pick_warp<1>(q, rows, st) : launch_pick_warp<0>(q, rows, st);
         else if (threads == 128) e = b.nv ? launch_pick<1, 128>(q, rows, st) : launch_pick<0, 128>(q, rows, st);

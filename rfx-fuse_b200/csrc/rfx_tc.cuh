@@ -178,7 +178,8 @@ __device__ __forceinline__ int clc_answer(uint32_t slot) {
     return ok ? (int)x : -1;
 }
 
-// 2-D tiled TMA load (box 64 x 128 of bf16) into shared memory, completing on `bar`.
+// 2-D tiled TMA load of a map's box into shared memory, completing on `bar`; x times the element size
+// is a multiple of 16 bytes.
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* tm, int x, int y,
                                          uint32_t bar) {
     asm volatile(
