@@ -18,6 +18,7 @@ operators, and a matrix that is dropped while another stream than its own still 
 from __future__ import annotations
 
 import ctypes as C
+import operator
 
 from . import _abi as A
 
@@ -168,6 +169,7 @@ class Fp4Matrix:
     def rows(self, begin, end):
         """Rows [begin, end) as a matrix that shares this one's memory; begin a multiple of 128."""
         n = self.shape[0]
+        begin, end = operator.index(begin), operator.index(end)
         if not 0 <= begin <= end <= n:
             raise ValueError(f"rows [{begin}, {end}) are not in [0, {n}]")
         if begin % 128:

@@ -45,3 +45,26 @@ def test_saving_tells_what_the_file_cannot_say(mode, told, monkeypatch, tmp_path
     with warnings.catch_warnings():
         warnings.simplefilter("error")
         plain.save(tmp_path / "m.rfx")
+
+
+def test_views_take_any_whole_numbers():
+    """Bounds from numpy or torch make the view that plain ones make; others are refused."""
+    import numpy as np
+    import torch
+    from rfx_b200 import _abi as A
+    fp4._load()
+    m = object.__new__(fp4.Fp4Matrix)  # of made-up addresses: nothing here reads them
+    m.format, m.shape, m.device = "nvfp4", (400, 64), torch.device("cpu")
+    m._pitch, m._tile_bytes, m._keep = 32, 512, torch.zeros(4)
+    m._set(A.Fp4Struct(1, 400, 64, 1 << 20, 2 << 20, 3 << 20, 4 << 20))
+    want = m.rows(128, 300)
+    for begin, end in ((np.int64(128), np.int32(300)), (torch.tensor(128), torch.tensor(300))):
+        got = m.rows(begin, end)
+        assert got.shape == want.shape == (172, 64)
+        assert all(getattr(got._c, f) == getattr(want._c, f) for f, _ in A.Fp4Struct._fields_)
+    for begin, end in ((128.0, 300), (0, 300.5), ("0", 300)):
+        with pytest.raises(TypeError, match="integer"):
+            m.rows(begin, end)
+    for begin, end in ((np.int64(128), np.int64(401)), (np.int64(-128), 5), (np.int64(64), 100)):
+        with pytest.raises(ValueError):
+            m.rows(begin, end)
