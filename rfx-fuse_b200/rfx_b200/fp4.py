@@ -141,9 +141,9 @@ class Fp4Matrix:
             if format == "mxfp4":
                 raise ValueError("mxfp4 has no matrix scale")
         elif scale is not None:
-            scale = float(scale)
+            scale = C.c_float(float(scale)).value  # as it is kept
             if not 0.0 < scale < float("inf"):
-                raise ValueError("scale must be positive and finite")
+                raise ValueError("scale must be positive and finite in float32")
             if format == "mxfp4" and scale != 1.0:
                 raise ValueError("mxfp4 has no matrix scale")
         m = cls._empty(codes.shape[0], cols, format, codes.device)

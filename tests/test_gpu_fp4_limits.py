@@ -205,3 +205,16 @@ def test_values_at_the_ends_of_the_range(fmt):
         assert np.array_equal(half, _round(v, 8, -126))
         held = np.abs(v) >= 2.0 ** -128 if fmt == "nvfp4" else np.ones_like(v, bool)
         assert np.array_equal(half[held], v[held])
+
+
+def test_matrix_scale_numbers_that_fp32_cannot_hold():
+    """A number is checked as it is kept: one that rounds to 0 or infinity in fp32 is refused."""
+    rng = np.random.default_rng(1)
+    c, s = _random(rng, 3, 40, "nvfp4")
+    top = float(np.finfo(np.float32).max)  # 2^128 (1 - 2^-24); from 2^128 (1 - 2^-25) on numbers round to infinity
+    for g in (1e39, 1e-50, 2.0 ** -151, 2.0 ** 128 * (1 - 2.0 ** -25), -1e-50, 0.0, float("nan")):
+        with pytest.raises(ValueError, match="positive and finite"):
+            _matrix(c, s, 40, "nvfp4", g)
+    # (1 - 2^-24) (1 + 2^-25) = 1 - 2^-25 - 2^-49: below that border, so it rounds to the largest number
+    for g, kept in ((2.0 ** -149, 2.0 ** -149), (top, top), (top * (1 + 2.0 ** -25), top)):
+        assert float(_matrix(c, s, 40, "nvfp4", g).parts()[2]) == kept
