@@ -140,6 +140,7 @@ class Fp4Matrix:
                 raise ValueError("scale must be one float32 on the codes' device")
             if format == "mxfp4":
                 raise ValueError("mxfp4 has no matrix scale")
+            scale = scale.resolve_neg()
         elif scale is not None:
             scale = C.c_float(float(scale)).value  # as it is kept
             if not 0.0 < scale < float("inf"):

@@ -218,3 +218,15 @@ def test_matrix_scale_numbers_that_fp32_cannot_hold():
     # (1 - 2^-24) (1 + 2^-25) = 1 - 2^-25 - 2^-49: below that border, so it rounds to the largest number
     for g, kept in ((2.0 ** -149, 2.0 ** -149), (top, top), (top * (1 + 2.0 ** -25), top)):
         assert float(_matrix(c, s, 40, "nvfp4", g).parts()[2]) == kept
+
+
+def test_matrix_scale_of_a_negated_view():
+    """A lazily negated tensor (the imaginary part of a conjugate is one) counts by its value."""
+    import torch
+    rng = np.random.default_rng(2)
+    c, s = _random(rng, 5, 40, "nvfp4")
+    g = torch.tensor([1 - 0.375j], device="cuda").conj().imag
+    assert g.is_neg() and float(g) == 0.375
+    m = _matrix(c, s, 40, "nvfp4", g)
+    assert float(m.parts()[2]) == 0.375
+    assert np.array_equal(m.dequantize().double().cpu().numpy(), ref.values(c, s, 0.375, "nvfp4"))
