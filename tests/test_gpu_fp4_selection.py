@@ -141,3 +141,23 @@ def test_accumulators_within_the_bound(fmt, m, k):
         if kind != "small":
             worst = max(worst, float((off[size > 0] / size[size > 0]).max()))
     print(f"largest error / (|a| |b|): 2^{np.log2(max(worst, 2.0 ** -60)):.1f}")
+
+
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("m,begin,end", [(3, 128, 129), (5, 256, 2011), (400, 128, 1500), (3700, 384, 3999)])
+def test_a_view_as_rows(fmt, m, begin, end):
+    """The rows searched are a view that starts at a later tile and ends inside one; what lies outside
+    (rows of larger norms, rows of NaN) is neither found nor felt."""
+    rng = np.random.default_rng(m + begin + end)
+    n, k, top = 4000, 72, 12
+    c, s = _random(rng, n, k, fmt)
+    va_c, va_s = _random(rng, m, k, fmt)
+    out = np.r_[0:begin, end:n]
+    s[out] += 40 if fmt == "nvfp4" else 20
+    s[rng.choice(out, 30), 0] = 127 if fmt == "nvfp4" else 255
+    s[min(end, n - 1), 1] = 127 if fmt == "nvfp4" else 255  # in the view's last tile
+    b = _matrix(c, s, k, fmt)
+    a = _matrix(va_c, va_s, k, fmt)
+    rows = _sample(rng, m)
+    _check(a, b.rows(begin, end), ref.values(va_c[rows], va_s[rows], 1.0, fmt), ref.values(c[begin:end], s[begin:end], 1.0, fmt),
+           top, fmt, rows)
